@@ -74,6 +74,12 @@ uint32_t orca_version(void);
 
 /* ---- context: one per device (GpuBackend::new, orca-backend-gpu/src/backend.rs:53-80) */
 orca_status orca_ctx_create(int device, orca_ctx** out);
+/* The same on the caller's stream (a cudaStream_t of that device; NULL is the
+ * legacy default stream) instead of a stream of its own, so that this
+ * library's calls are ordered with the caller's other work without events and
+ * can be captured into a CUDA graph with it.  The stream stays the caller's and
+ * must outlive the context. */
+orca_status orca_ctx_create_on_stream(int device, void* stream, orca_ctx** out);
 orca_status orca_ctx_destroy(orca_ctx* ctx);
 /* Wait for all enqueued work; ORCA_TIMEOUT after timeout_s seconds (<=0: 600 s). */
 orca_status orca_ctx_sync(orca_ctx* ctx, double timeout_s);
@@ -256,6 +262,77 @@ orca_status orca_sgd_step(orca_ctx* ctx, orca_buf* p, const orca_buf* g, orca_bu
 orca_status orca_adamw_step(orca_ctx* ctx, orca_buf* p, const orca_buf* g, orca_buf* m,
                             orca_buf* v, double lr, double beta1, double beta2, double eps,
                             double weight_decay, int64_t t);
+
+/* ---- feed-forward operators: linear with activation and residual, 8-bit activation
+ * checkpoints (no counterpart in the reference) -------------------------------------
+ * Beside orca_linear_fwd / orca_linear_bwd: BF16, F16 and F32 operands (sums in
+ * F32; F32 operands give F32-accurate products), any of the activations below,
+ * a residual, and the pre-activation kept for the backward pass plainly or in
+ * 8 bits.  Inputs and outputs are spans: memory of the context's device that
+ * the caller owns (an orca_buf's orca_buf_device_ptr, or another allocator's),
+ * row-major and contiguous, of any alignment to whole elements.  Nothing is
+ * allocated that outlives the call, so the calls can be captured into a CUDA
+ * graph.  Outputs must not overlap inputs or one another, except that out (dx)
+ * may be the residual's memory itself.  A call touches no more of a span than the sizes
+ * say.  Memory must stay valid until the context's stream has passed the call. */
+typedef struct {
+  void* data;                /* device memory (NULL only when len is 0) */
+  size_t len;                /* elements */
+  orca_dtype dtype;
+} orca_span;
+
+typedef enum {
+  ORCA_ACT_NONE = 0,
+  ORCA_ACT_RELU = 1,         /* z > 0 ? z : 0 */
+  ORCA_ACT_GELU = 2,         /* z (1 + erf(z / sqrt 2)) / 2 */
+  ORCA_ACT_GELU_TANH = 3,    /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
+  ORCA_ACT_SILU = 4          /* z / (1 + exp(-z)) */
+} orca_act;
+
+typedef enum { ORCA_KEEP_NONE = 0, ORCA_KEEP_Z = 1, ORCA_KEEP_CKPT8 = 2 } orca_keep;
+
+/* Bytes of the 8-bit checkpoint of an [m, n] matrix (0 for negative sizes): m*n
+ * signed codes, row after row, then from the next multiple of 16 bytes one
+ * exponent byte E per row and group of 32 columns (the last group of a row may
+ * be shorter).  A code q stands for q * 2^(E - 127), exact in BF16.  Packing
+ * takes 2^(E - 127) = 2^(floor(log2 amax) - 6), at least 2^-126, for the group's
+ * largest magnitude amax and rounds to the nearest code, ties to even, within
+ * +-127.  E = 255 marks a group that held an infinity or a NaN; all of it
+ * decodes to NaN. */
+size_t orca_ckpt8_bytes(int64_t m, int64_t n);
+/* ckpt (U8, orca_ckpt8_bytes(m, n)) = the checkpoint of x [m, n]. */
+orca_status orca_ckpt8_pack(orca_ctx* ctx, const orca_span* x, int64_t m, int64_t n,
+                            const orca_span* ckpt);
+/* out [m, n] = act(the values of ckpt), rounded to out's type. */
+orca_status orca_ckpt8_unpack(orca_ctx* ctx, const orca_span* ckpt, int64_t m, int64_t n,
+                              orca_act act, const orca_span* out);
+
+/* out = act(z) + residual with z = x @ w + b, in one pass: x [m, k], w [k, n]
+ * ([in, out]), b [n] (nullable), residual [m, n] (nullable), all of one type;
+ * bias, activation and residual are applied to the F32 sums and rounded once.
+ * keep says what is written to z (NULL for ORCA_KEEP_NONE): the
+ * pre-activation in the operands' type, or its 8-bit checkpoint (U8), both of the
+ * unrounded sums.  k = 0 gives z = b. */
+orca_status orca_linear_act_fwd(orca_ctx* ctx, const orca_span* x, const orca_span* w,
+                                const orca_span* b, const orca_span* residual, int64_t m,
+                                int64_t k, int64_t n, orca_act act, const orca_span* out,
+                                orca_keep keep, const orca_span* z);
+/* Backward of y = a @ w + b with a = act(x), from dy [m, n]:
+ *   dx = (dy @ w^T) * act'(x) + residual   [m, k], in the operands' type
+ *   dw = a^T @ dy                          [k, n], F32 or the operands' type
+ *   db = the column sums of dy             [n],    F32 or the operands' type
+ * each of the three nullable.  x is what the layer below kept: its
+ * pre-activation with that layer's activation (dx is then the gradient of
+ * that pre-activation), or the layer's input with ORCA_ACT_NONE.  A U8 span is
+ * an 8-bit checkpoint, any other the plain values in the type of w.  Only dw
+ * (and dx with an activation) reads x, only dx reads w and residual; what is
+ * not read may be NULL.  a is rounded to the operands' type, as the forward
+ * pass rounds it.  residual [m, k] (nullable) is a gradient that reaches x's
+ * layer by another way. */
+orca_status orca_linear_act_bwd(orca_ctx* ctx, const orca_span* x, const orca_span* w,
+                                const orca_span* dy, const orca_span* residual, int64_t m,
+                                int64_t k, int64_t n, orca_act act, const orca_span* dx,
+                                const orca_span* dw, const orca_span* db);
 
 /* ---- data-parallel step runner -------------------------------------------------
  * Sequential(Linear, ReLU, ..., Linear) + CrossEntropyLoss + SGD/AdamW on

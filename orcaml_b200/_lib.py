@@ -62,12 +62,21 @@ class orca_mlp_config(ctypes.Structure):
     ]
 
 
+class orca_span(ctypes.Structure):
+    """Device memory of `len` elements that the caller owns."""
+    _fields_ = [("data", c_void_p), ("len", c_size_t), ("dtype", c_int)]
+
+
+P_span = ctypes.POINTER(orca_span)
+
+
 # Argument types of every exported function (status-returning unless noted).
 _SIGS = {
     "orca_last_error": ([], c_char_p),
     "orca_status_string": ([c_int], c_char_p),
     "orca_version": ([], c_uint32),
     "orca_ctx_create": ([c_int, PP], c_int),
+    "orca_ctx_create_on_stream": ([c_int, c_void_p, PP], c_int),
     "orca_ctx_destroy": ([c_void_p], c_int),
     "orca_ctx_sync": ([c_void_p, c_double], c_int),
     "orca_ctx_device": ([c_void_p, ctypes.POINTER(c_int)], c_int),
@@ -122,6 +131,13 @@ _SIGS = {
     "orca_softmax_ce_fwd_bwd": ([c_void_p, c_void_p, c_void_p, c_int64, c_int64, PP, PP], c_int),
     "orca_softmax_ce_fwd_bwd_noalloc": ([c_void_p, c_void_p, c_void_p, c_int64, c_int64, c_void_p,
                                          c_void_p], c_int),
+    "orca_ckpt8_bytes": ([c_int64, c_int64], c_size_t),
+    "orca_ckpt8_pack": ([c_void_p, P_span, c_int64, c_int64, P_span], c_int),
+    "orca_ckpt8_unpack": ([c_void_p, P_span, c_int64, c_int64, c_int, P_span], c_int),
+    "orca_linear_act_fwd": ([c_void_p, P_span, P_span, P_span, P_span, c_int64, c_int64, c_int64,
+                             c_int, P_span, c_int, P_span], c_int),
+    "orca_linear_act_bwd": ([c_void_p, P_span, P_span, P_span, P_span, c_int64, c_int64, c_int64,
+                             c_int, P_span, P_span, P_span], c_int),
     "orca_sgd_step": ([c_void_p, c_void_p, c_void_p, c_void_p, c_double, c_double, c_double,
                        c_double, c_int], c_int),
     "orca_adamw_step": ([c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_double, c_double,

@@ -17,6 +17,8 @@ import numpy as np
 from . import _lib as L
 
 F32, F64, F16, BF16, I32, I64, U8, BOOL = range(8)   # orca-core/src/dtype.rs:5-22
+ACTS = {"none": 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
+KEEPS = {None: 0, "none": 0, "z": 1, "ckpt8": 2}
 _NP = {F32: np.float32, F64: np.float64, F16: np.float16, I32: np.int32, I64: np.int64,
        U8: np.uint8, BOOL: np.bool_}
 
@@ -55,10 +57,16 @@ class CudaBackend:
     """One per device, like the reference's GpuBackend singleton
     (orca-python/src/lib.rs:23-33)."""
 
-    def __init__(self, device: int = 0):
+    def __init__(self, device: int = 0, stream: int | None = None):
+        """stream: a CUDA stream handle of that device (0: the legacy default
+        stream) that the calls run on, the caller's and alive as long as this
+        backend; None gives the backend a stream of its own."""
         lib = L.load()
         h = ctypes.c_void_p()
-        L.check(lib.orca_ctx_create(int(device), ctypes.byref(h)))
+        if stream is None:
+            L.check(lib.orca_ctx_create(int(device), ctypes.byref(h)))
+        else:
+            L.check(lib.orca_ctx_create_on_stream(int(device), int(stream), ctypes.byref(h)))
         self._ctx = h
         self.device_index = int(device)
 
@@ -244,6 +252,91 @@ class CudaBackend:
     def gemm_ex(self, m, n, k, a, a_mn_major, b, b_mn_major, path=0):
         return self._out(L.load().orca_gemm_ex, int(m), int(n), int(k), a._h,
                          1 if a_mn_major else 0, b._h, 1 if b_mn_major else 0, int(path))
+
+    # -- feed-forward operators: linear with activation and residual, 8-bit
+    # activation checkpoints.  Their arguments are storages or spans; an output
+    # that is not given is a new storage.  Inside a graph capture, give them all.
+    @staticmethod
+    def span(ptr: int, n: int, dtype: int) -> L.orca_span:
+        """n elements of device memory at ptr that the caller owns and keeps
+        alive until the backend's stream has passed the calls that use it."""
+        return L.orca_span(ptr, n, dtype)
+
+    @staticmethod
+    def _span(x):
+        if x is None or isinstance(x, L.orca_span):
+            return x
+        s = L.orca_span(x.device_ptr, len(x), x.dtype)
+        s.owner = x          # the storage lives as long as its span
+        return s
+
+    def _result(self, out, numel, dtype):
+        return out if out is not None else self.zeros([int(numel)], dtype)
+
+    @staticmethod
+    def _choice(table, value, what):
+        try:
+            return table[value]
+        except KeyError:
+            raise L.OrcaError(7, f"{what}: {value!r} is none of "
+                                 f"{', '.join(repr(v) for v in table)}") from None
+
+    @staticmethod
+    def ckpt8_bytes(m, n) -> int:
+        """Bytes of the 8-bit checkpoint of an [m, n] matrix."""
+        return int(L.load().orca_ckpt8_bytes(m, n))
+
+    def ckpt8_pack(self, x, m, n, out=None):
+        """The 8-bit checkpoint (U8) of x [m, n]: groups of 32 columns share a
+        power of two, each value a signed 8-bit code."""
+        x = self._span(x)
+        out = self._result(out, self.ckpt8_bytes(m, n), U8)
+        L.check(L.load().orca_ckpt8_pack(self._ctx, x, m, n, self._span(out)))
+        return out
+
+    def ckpt8_unpack(self, ckpt, m, n, act="none", dtype=F32, out=None):
+        """act(the values of a checkpoint of [m, n]), in dtype (or out's)."""
+        a = self._choice(ACTS, act, "act")
+        ckpt = self._span(ckpt)
+        out = self._result(out, m * n, dtype)
+        L.check(L.load().orca_ckpt8_unpack(self._ctx, ckpt, m, n, a, self._span(out)))
+        return out
+
+    def linear_act_fwd(self, x, w, b, m, k, n, act="none", residual=None, keep=None, out=None,
+                       z=None):
+        """(out, kept): out = act(x @ w + b) + residual, x [m, k], w [k, n],
+        b [n] or None, residual [m, n] or None, all BF16, F16 or F32.  keep:
+        None, "z" (the pre-activation in the same type) or "ckpt8" (its 8-bit
+        checkpoint), written to z."""
+        a = self._choice(ACTS, act, "act")
+        kp = self._choice(KEEPS, keep, "keep")
+        x = self._span(x)
+        out = self._result(out, m * n, x.dtype)
+        if kp:
+            z = self._result(z, m * n if kp == 1 else self.ckpt8_bytes(m, n), x.dtype if kp == 1 else U8)
+        L.check(L.load().orca_linear_act_fwd(self._ctx, x, self._span(w), self._span(b),
+                                             self._span(residual), m, k, n, a, self._span(out), kp,
+                                             self._span(z)))
+        return out, z
+
+    def linear_act_bwd(self, x, w, dy, m, k, n, act="none", x_ckpt8=False, residual=None, dx=None,
+                       dw=None, db=None, need_dx=True, need_dw=True, need_db=True, grad_dtype=F32):
+        """(dx, dw, db) of y = a @ w + b with a = act(x), from dy [m, n]:
+        dx = (dy @ w^T) * act'(x) + residual, dw = a^T @ dy and db = the column
+        sums of dy in grad_dtype (F32, or dy's dtype).  x is what the layer
+        below kept: plain values, or with x_ckpt8 an 8-bit checkpoint."""
+        a = self._choice(ACTS, act, "act")
+        x, dy = self._span(x), self._span(dy)
+        if x is not None and x_ckpt8 != (x.dtype == U8):
+            raise L.OrcaError(4, "linear_act_bwd: x_ckpt8 says "
+                                 f"{'a checkpoint' if x_ckpt8 else 'plain values'}, x has dtype {x.dtype}")
+        dx = self._result(dx, m * k, dy.dtype) if need_dx else None
+        dw = self._result(dw, k * n, grad_dtype) if need_dw else None
+        db = self._result(db, n, grad_dtype) if need_db else None
+        L.check(L.load().orca_linear_act_bwd(self._ctx, x, self._span(w), dy, self._span(residual), m,
+                                             k, n, a, self._span(dx), self._span(dw),
+                                             self._span(db)))
+        return dx, dw, db
 
     def softmax_ce_fwd_bwd(self, logits, target, batch, classes):
         loss = ctypes.c_void_p()

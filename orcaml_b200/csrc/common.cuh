@@ -67,6 +67,7 @@ struct orca_ctx {
   int device = 0;
   int sm_count = 0;
   cudaStream_t stream = nullptr;        // compute stream
+  bool owns_stream = true;              // false: the caller's (orca_ctx_create_on_stream)
   cudaStream_t comm_stream = nullptr;   // collectives
   int* dev_err = nullptr;               // device error word (DeviceError)
   int* tile_ctr = nullptr;              // tile counter of the persistent GEMM (reset per launch)

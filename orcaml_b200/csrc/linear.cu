@@ -1,0 +1,403 @@
+// linear.cu -- fused linear operators: out = act(x @ w + b) + residual and its
+// backward, in BF16, F16 and F32.
+#include <algorithm>
+
+#include "linear.cuh"
+
+namespace orca {
+
+// ---------------------------------------------------------------- checks
+orca_status need_dim(int64_t v, const char* what) {
+  // Below 2^31 a size fits the TMA coordinates and products of two stay far from 2^63.
+  if (v < 0 || v > INT32_MAX - 4096)
+    return fail(ORCA_INVALID_ARGUMENT, "%s: size %lld is out of range", what, (long long)v);
+  return ORCA_OK;
+}
+
+orca_status need_float(const orca_span* s, const char* what) {
+  if (s->dtype != ORCA_F32 && s->dtype != ORCA_F16 && s->dtype != ORCA_BF16)
+    return fail(ORCA_UNSUPPORTED_DTYPE, "%s: dtype %d is none of F32, F16, BF16", what, (int)s->dtype);
+  return ORCA_OK;
+}
+
+orca_status need_span(orca_ctx* ctx, const orca_span* s, int64_t len, const char* what) {
+  if (!s) return fail(ORCA_INVALID_ARGUMENT, "%s: null span", what);
+  const size_t es = dtype_size(s->dtype);
+  if (!es) return fail(ORCA_UNSUPPORTED_DTYPE, "%s: unknown dtype %d", what, (int)s->dtype);
+  if (s->len < (size_t)len)
+    return fail(ORCA_SHAPE_MISMATCH, "%s: the span holds %zu elements, the sizes need %lld", what,
+                s->len, (long long)len);
+  if (len == 0) return ORCA_OK;
+  if (!s->data) return fail(ORCA_INVALID_ARGUMENT, "%s: null data", what);
+  if (reinterpret_cast<uintptr_t>(s->data) % es)
+    return fail(ORCA_INVALID_ARGUMENT, "%s: data is not aligned to its elements", what);
+  cudaPointerAttributes at;
+  ORCA_CUDA_TRY(cudaPointerGetAttributes(&at, s->data));
+  if (at.type != cudaMemoryTypeDevice && at.type != cudaMemoryTypeManaged)
+    return fail(ORCA_DEVICE_MISMATCH, "%s: data is not device memory", what);
+  if (at.type == cudaMemoryTypeDevice && at.device != ctx->device)
+    return fail(ORCA_DEVICE_MISMATCH, "%s: data is on device %d, the context on %d", what, at.device,
+                ctx->device);
+  return ORCA_OK;
+}
+
+orca_status need_apart(const orca_span* out, const orca_span* other, const char* what) {
+  if (!out || !other || !out->len || !other->len) return ORCA_OK;
+  const uintptr_t a = reinterpret_cast<uintptr_t>(out->data), b = reinterpret_cast<uintptr_t>(other->data);
+  if (a < b + other->len * dtype_size(other->dtype) && b < a + out->len * dtype_size(out->dtype))
+    return fail(ORCA_INVALID_ARGUMENT, "%s overlap", what);
+  return ORCA_OK;
+}
+
+namespace lin {
+
+// ---------------------------------------------------------------- operands
+// Element (i, c) of an operand, i along the output and c along the sum:
+// at c * ld + i when mn_major, else at i * ld + c.
+struct Operand {
+  const void* p = nullptr;
+  int64_t ld = 0;
+  int mn_major = 0;
+};
+
+// Stream-ordered scratch of one call; in a captured graph it becomes the
+// graph's own allocation, so graphs share nothing.
+struct Scratch {
+  orca_ctx* ctx;
+  void* p = nullptr;
+  explicit Scratch(orca_ctx* c) : ctx(c) {}
+  ~Scratch() { if (p) cudaFreeAsync(p, ctx->stream); }
+  Scratch(const Scratch&) = delete;
+  Scratch& operator=(const Scratch&) = delete;
+  orca_status get(size_t bytes) {
+    ORCA_CUDA_TRY(cudaMallocAsync(&p, bytes, ctx->stream));
+    return ORCA_OK;
+  }
+};
+
+// ---------------------------------------------------------------- FFMA tiles
+// 64 x 64 tiles of F32 sums, each a sequential FMA chain over the sum's
+// index, 4 x 4 per thread; operands in any orientation and alignment.
+constexpr int SM = 64, SN = 64, SK = 16;
+
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256)
+tile_kernel(int64_t M, int64_t N, int64_t K, Operand A, Operand B, Epilogue e) {
+  __shared__ float As[SK][SM + 4];
+  __shared__ float Bs[SK][SN + 4];
+  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
+  const int64_t num_n = cdiv(N, SN);
+  const int64_t m0 = blockIdx.x / num_n * SM, n0 = blockIdx.x % num_n * SN;
+  const T* a = (const T*)A.p;
+  const T* b = (const T*)B.p;
+  float acc[4][4] = {};
+  for (int64_t k0 = 0; k0 < K; k0 += SK) {
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      const int el = tid + r * 256;
+      const int mm = A.mn_major ? el % SM : el / SK, ka = A.mn_major ? el / SM : el % SK;
+      const int64_t gm = m0 + mm, gk = k0 + ka;
+      As[ka][mm] = gm < M && gk < K ? to_f32(a[A.mn_major ? gk * A.ld + gm : gm * A.ld + gk]) : 0.0f;
+      const int nn = B.mn_major ? el % SN : el / SK, kb = B.mn_major ? el / SN : el % SK;
+      const int64_t gn = n0 + nn, gj = k0 + kb;
+      Bs[kb][nn] = gn < N && gj < K ? to_f32(b[B.mn_major ? gj * B.ld + gn : gn * B.ld + gj]) : 0.0f;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int kk = 0; kk < SK; ++kk) {
+      float av[4], bv[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) av[i] = As[kk][ty * 4 + i];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) bv[j] = Bs[kk][tx * 4 + j];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) epilogue<T, MODE, 4>(e, m0 + ty * 4 + i, n0 + tx * 4, acc[i]);
+}
+
+// ---------------------------------------------------------------- column sums
+// db: rows [r0, r1) of a block summed per column in F32, 8 columns a thread and
+// 8 row lanes joined in order; row blocks joined in order by sum_parts, so the
+// result does not depend on timing.
+constexpr int CS_COLS = 256;
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+colsum_kernel(const T* __restrict__ x, int64_t m, int64_t n, int64_t rows, int vec,
+              float* __restrict__ part) {
+  __shared__ float s[8][CS_COLS + 8];
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
+  const int64_t col = (int64_t)blockIdx.x * CS_COLS + tx * 8;
+  const int valid = col >= n ? 0 : (n - col < 8 ? (int)(n - col) : 8);
+  const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = std::min<int64_t>(m, r0 + rows);
+  float acc[8] = {};
+  if (valid > 0)
+#pragma unroll 4
+    for (int64_t r = r0 + ty; r < r1; r += 8) {
+      float v[8];
+      load_row<T, 8>(x + r * n + col, valid, vec && valid == 8, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[i] += v[i];
+    }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) s[ty][tx * 8 + i] = acc[i];
+  __syncthreads();
+  const int64_t c = (int64_t)blockIdx.x * CS_COLS + threadIdx.x;
+  if (c >= n) return;
+  float t = 0.0f;
+#pragma unroll
+  for (int y = 0; y < 8; ++y) t += s[y][threadIdx.x];
+  part[(int64_t)blockIdx.y * n + c] = t;
+}
+
+template <typename G>
+__global__ void __launch_bounds__(256)
+sum_parts_kernel(const float* __restrict__ part, int64_t n, int parts, G* __restrict__ out) {
+  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (c >= n) return;
+  float t = 0.0f;
+  for (int p = 0; p < parts; ++p) t += part[(int64_t)p * n + c];
+  out[c] = from_f32<G>(t);
+}
+
+template <typename T>
+static orca_status colsum(orca_ctx* ctx, const T* x, int64_t m, int64_t n, const orca_span* out) {
+  if (n <= 0) return ORCA_OK;
+  const int64_t bx = cdiv(n, CS_COLS);
+  int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cdiv(m, 64), (int64_t)ctx->sm_count * 4 / bx));
+  const int64_t rows = std::max<int64_t>(1, cdiv(m, parts));
+  parts = std::max<int64_t>(1, cdiv(m, rows));
+  Scratch part(ctx);
+  ORCA_TRY(part.get((size_t)(parts * n) * 4));
+  const bool vec = byte_alignment(x, n * (int64_t)sizeof(T)) == 16;
+  colsum_kernel<T><<<dim3((unsigned)bx, (unsigned)parts), 256, 0, ctx->stream>>>(
+      x, m, n, rows, vec ? 1 : 0, (float*)part.p);
+  const unsigned g = (unsigned)cdiv(n, 256);
+  if (out->dtype == ORCA_F32)
+    sum_parts_kernel<<<g, 256, 0, ctx->stream>>>((const float*)part.p, n, (int)parts, (float*)out->data);
+  else
+    sum_parts_kernel<<<g, 256, 0, ctx->stream>>>((const float*)part.p, n, (int)parts, (T*)out->data);
+  count_launch(ctx, 2);
+  ORCA_CUDA_TRY(cudaGetLastError());
+  return ORCA_OK;
+}
+
+// ---------------------------------------------------------------- products
+template <typename T, int MODE>
+static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const Operand& A,
+                           const Operand& B, Epilogue e) {
+  if (M <= 0 || N <= 0) return ORCA_OK;
+  e.rows = M;
+  e.cols = N;
+  int al = 16;
+  for (const void* p : {(const void*)e.out, e.residual, (const void*)e.z, e.x})
+    if (p) al = std::min(al, byte_alignment(p, N * (int64_t)sizeof(T)));
+  if (e.bias) al = std::min(al, byte_alignment(e.bias, 0));
+  e.vec = al == 16;
+  if (e.codes) e.ckpt_align = byte_alignment(e.codes, N);
+  const int64_t tiles = cdiv(M, SM) * cdiv(N, SN);
+  if (tiles > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
+  tile_kernel<T, MODE><<<(unsigned)tiles, 256, 0, ctx->stream>>>(M, N, K, A, B, e);
+  count_launch(ctx);
+  ORCA_CUDA_TRY(cudaGetLastError());
+  return ORCA_OK;
+}
+
+template <typename T>
+static orca_status forward(orca_ctx* ctx, const orca_span* x, const orca_span* w, int64_t m,
+                           int64_t k, int64_t n, const Epilogue& e) {
+  Operand a, b;
+  a.p = x->data; a.ld = k;
+  b.p = w->data; b.ld = n; b.mn_major = 1;
+  return product<T, FWD>(ctx, m, n, k, a, b, e);
+}
+
+template <typename T>
+static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* w,
+                            const orca_span* dy, const orca_span* residual, int64_t m, int64_t k,
+                            int64_t n, int act, const orca_span* dx, const orca_span* dw,
+                            const orca_span* db) {
+  const bool packed = x && x->dtype == ORCA_U8;
+  if (dx) {
+    Operand a, b;
+    a.p = dy->data; a.ld = n;
+    b.p = w->data; b.ld = n;
+    Epilogue e;
+    e.act = act;
+    e.out = dx->data;
+    if (residual) e.residual = residual->data;
+    if (act != ORCA_ACT_NONE) {
+      if (packed) {
+        e.codes = (uint8_t*)x->data;
+        e.exps = e.codes + ckpt_exps_at(m, k);
+      } else {
+        e.x = x->data;
+      }
+    }
+    ORCA_TRY((product<T, DX>(ctx, m, k, n, a, b, e)));
+  }
+  if (dw) {
+    Scratch act_x(ctx);
+    Operand a, b;
+    a.ld = k; a.mn_major = 1;
+    if (!packed && act == ORCA_ACT_NONE) {
+      a.p = x ? x->data : nullptr;
+    } else if (m * k > 0) {
+      ORCA_TRY(act_x.get((size_t)(m * k) * sizeof(T)));
+      if (packed)
+        ORCA_TRY(ckpt8_unpack_launch(ctx, (const uint8_t*)x->data, m, k, act, act_x.p, w ? w->dtype : dy->dtype));
+      else
+        ORCA_TRY(act_launch(ctx, x->data, x->dtype, m * k, act, act_x.p));
+      a.p = act_x.p;
+    }
+    b.p = dy->data; b.ld = n; b.mn_major = 1;
+    Epilogue e;
+    e.out = dw->data;
+    e.out_f32 = dw->dtype == ORCA_F32;
+    ORCA_TRY((product<T, DW>(ctx, k, n, m, a, b, e)));
+  }
+  if (db) ORCA_TRY(colsum<T>(ctx, (const T*)dy->data, m, n, db));
+  return ORCA_OK;
+}
+
+}  // namespace lin
+}  // namespace orca
+
+using namespace orca;
+
+static orca_status need_type(const orca_span* s, orca_dtype t, const char* what) {
+  if (s->dtype != t) return fail(ORCA_DTYPE_MISMATCH, "%s: dtype %d, expected %d", what, (int)s->dtype, (int)t);
+  return ORCA_OK;
+}
+
+static orca_status need_act(orca_act act, const char* what) {
+  if ((int)act < ORCA_ACT_NONE || (int)act > ORCA_ACT_SILU)
+    return fail(ORCA_INVALID_ARGUMENT, "%s: unknown activation %d", what, (int)act);
+  return ORCA_OK;
+}
+
+// out may be the residual's memory itself: each element is read before the
+// same thread writes it.
+static orca_status need_apart_or_same(const orca_span* out, const orca_span* residual, const char* what) {
+  if (out && residual && out->data == residual->data) return ORCA_OK;
+  return need_apart(out, residual, what);
+}
+
+extern "C" {
+
+orca_status orca_linear_act_fwd(orca_ctx* ctx, const orca_span* x, const orca_span* w,
+                                const orca_span* b, const orca_span* residual, int64_t m,
+                                int64_t k, int64_t n, orca_act act, const orca_span* out,
+                                orca_keep keep, const orca_span* z) {
+  ORCA_TRY(check_ctx(ctx));
+  std::lock_guard<std::mutex> lk(ctx->mu);
+  ORCA_TRY(need_dim(m, "linear_act_fwd: m"));
+  ORCA_TRY(need_dim(k, "linear_act_fwd: k"));
+  ORCA_TRY(need_dim(n, "linear_act_fwd: n"));
+  ORCA_TRY(need_act(act, "linear_act_fwd"));
+  ORCA_TRY(need_span(ctx, x, m * k, "linear_act_fwd: x"));
+  ORCA_TRY(need_float(x, "linear_act_fwd: x"));
+  ORCA_TRY(need_span(ctx, w, k * n, "linear_act_fwd: w"));
+  ORCA_TRY(need_type(w, x->dtype, "linear_act_fwd: w"));
+  if (b) {
+    ORCA_TRY(need_span(ctx, b, n, "linear_act_fwd: b"));
+    ORCA_TRY(need_type(b, x->dtype, "linear_act_fwd: b"));
+  }
+  if (residual) {
+    ORCA_TRY(need_span(ctx, residual, m * n, "linear_act_fwd: residual"));
+    ORCA_TRY(need_type(residual, x->dtype, "linear_act_fwd: residual"));
+  }
+  ORCA_TRY(need_span(ctx, out, m * n, "linear_act_fwd: out"));
+  ORCA_TRY(need_type(out, x->dtype, "linear_act_fwd: out"));
+  if ((int)keep < ORCA_KEEP_NONE || (int)keep > ORCA_KEEP_CKPT8)
+    return fail(ORCA_INVALID_ARGUMENT, "linear_act_fwd: unknown keep %d", (int)keep);
+  if ((keep != ORCA_KEEP_NONE) != (z != nullptr))
+    return fail(ORCA_INVALID_ARGUMENT, "linear_act_fwd: z is given exactly when something is kept");
+  if (z) {
+    const bool packed = keep == ORCA_KEEP_CKPT8;
+    ORCA_TRY(need_span(ctx, z, packed ? (int64_t)orca_ckpt8_bytes(m, n) : m * n, "linear_act_fwd: z"));
+    ORCA_TRY(need_type(z, packed ? ORCA_U8 : x->dtype, "linear_act_fwd: z"));
+  }
+  for (const orca_span* o : {out, z}) {
+    ORCA_TRY(need_apart(o, x, "linear_act_fwd: an output and x"));
+    ORCA_TRY(need_apart(o, w, "linear_act_fwd: an output and w"));
+    ORCA_TRY(need_apart(o, b, "linear_act_fwd: an output and b"));
+  }
+  ORCA_TRY(need_apart_or_same(out, residual, "linear_act_fwd: out and residual"));
+  ORCA_TRY(need_apart(z, residual, "linear_act_fwd: z and residual"));
+  ORCA_TRY(need_apart(out, z, "linear_act_fwd: out and z"));
+  lin::Epilogue e;
+  e.act = act;
+  e.out = out->data;
+  if (b) e.bias = b->data;
+  if (residual) e.residual = residual->data;
+  if (keep == ORCA_KEEP_Z) e.z = z->data;
+  if (keep == ORCA_KEEP_CKPT8) {
+    e.codes = (uint8_t*)z->data;
+    e.exps = e.codes + lin::ckpt_exps_at(m, n);
+  }
+  if (x->dtype == ORCA_F32) return lin::forward<float>(ctx, x, w, m, k, n, e);
+  if (x->dtype == ORCA_F16) return lin::forward<__half>(ctx, x, w, m, k, n, e);
+  return lin::forward<__nv_bfloat16>(ctx, x, w, m, k, n, e);
+}
+
+orca_status orca_linear_act_bwd(orca_ctx* ctx, const orca_span* x, const orca_span* w,
+                                const orca_span* dy, const orca_span* residual, int64_t m,
+                                int64_t k, int64_t n, orca_act act, const orca_span* dx,
+                                const orca_span* dw, const orca_span* db) {
+  ORCA_TRY(check_ctx(ctx));
+  std::lock_guard<std::mutex> lk(ctx->mu);
+  ORCA_TRY(need_dim(m, "linear_act_bwd: m"));
+  ORCA_TRY(need_dim(k, "linear_act_bwd: k"));
+  ORCA_TRY(need_dim(n, "linear_act_bwd: n"));
+  ORCA_TRY(need_act(act, "linear_act_bwd"));
+  ORCA_TRY(need_span(ctx, dy, m * n, "linear_act_bwd: dy"));
+  ORCA_TRY(need_float(dy, "linear_act_bwd: dy"));
+  const orca_dtype t = dy->dtype;
+  if (dw || (dx && act != ORCA_ACT_NONE)) {
+    if (!x) return fail(ORCA_INVALID_ARGUMENT, "linear_act_bwd: x: null span");
+    const bool packed = x->dtype == ORCA_U8;
+    ORCA_TRY(need_span(ctx, x, packed ? (int64_t)orca_ckpt8_bytes(m, k) : m * k, "linear_act_bwd: x"));
+    if (!packed) ORCA_TRY(need_type(x, t, "linear_act_bwd: x"));
+  }
+  if (dx) {
+    ORCA_TRY(need_span(ctx, w, k * n, "linear_act_bwd: w"));
+    ORCA_TRY(need_type(w, t, "linear_act_bwd: w"));
+    if (residual) {
+      ORCA_TRY(need_span(ctx, residual, m * k, "linear_act_bwd: residual"));
+      ORCA_TRY(need_type(residual, t, "linear_act_bwd: residual"));
+    }
+    ORCA_TRY(need_span(ctx, dx, m * k, "linear_act_bwd: dx"));
+    ORCA_TRY(need_type(dx, t, "linear_act_bwd: dx"));
+  }
+  if (dw) {
+    ORCA_TRY(need_span(ctx, dw, k * n, "linear_act_bwd: dw"));
+    if (dw->dtype != ORCA_F32) ORCA_TRY(need_type(dw, t, "linear_act_bwd: dw"));
+  }
+  if (db) {
+    ORCA_TRY(need_span(ctx, db, n, "linear_act_bwd: db"));
+    if (db->dtype != ORCA_F32) ORCA_TRY(need_type(db, t, "linear_act_bwd: db"));
+  }
+  for (const orca_span* o : {dx, dw, db}) {
+    ORCA_TRY(need_apart(o, x, "linear_act_bwd: an output and x"));
+    ORCA_TRY(need_apart(o, w, "linear_act_bwd: an output and w"));
+    ORCA_TRY(need_apart(o, dy, "linear_act_bwd: an output and dy"));
+  }
+  ORCA_TRY(need_apart_or_same(dx, residual, "linear_act_bwd: dx and residual"));
+  ORCA_TRY(need_apart(dw, residual, "linear_act_bwd: dw and residual"));
+  ORCA_TRY(need_apart(db, residual, "linear_act_bwd: db and residual"));
+  ORCA_TRY(need_apart(dx, dw, "linear_act_bwd: dx and dw"));
+  ORCA_TRY(need_apart(dx, db, "linear_act_bwd: dx and db"));
+  ORCA_TRY(need_apart(dw, db, "linear_act_bwd: dw and db"));
+  if (t == ORCA_F32) return lin::backward<float>(ctx, x, w, dy, residual, m, k, n, act, dx, dw, db);
+  if (t == ORCA_F16) return lin::backward<__half>(ctx, x, w, dy, residual, m, k, n, act, dx, dw, db);
+  return lin::backward<__nv_bfloat16>(ctx, x, w, dy, residual, m, k, n, act, dx, dw, db);
+}
+
+}  // extern "C"

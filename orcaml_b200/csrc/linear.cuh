@@ -1,0 +1,328 @@
+// linear.cuh -- device pieces shared by the fused linear operators (linear.cu)
+// and the 8-bit activation checkpoints (ckpt8.cu): element types, activations
+// and their slopes, the checkpoint's group code, and the epilogue.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace orca {
+namespace lin {
+
+// ---------------------------------------------------------------- element types
+__device__ __forceinline__ float to_f32(float v) { return v; }
+__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
+__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) {
+  return __float2bfloat16_rn(v);
+}
+
+// V consecutive elements at p as f32.  `vec` (uniform): p is aligned to
+// min(16, V * sizeof(T)) bytes and all V elements are inside.
+template <typename T, int V>
+__device__ __forceinline__ void load_row(const T* p, int valid, bool vec, float (&v)[V]) {
+  constexpr int BYTES = V * (int)sizeof(T);
+  if (vec && V > 1) {
+    union { uint4 q[(BYTES + 15) / 16]; uint2 d; T e[V]; } u;
+    if (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) u.q[i] = reinterpret_cast<const uint4*>(p)[i];
+    } else {
+      u.d = *reinterpret_cast<const uint2*>(p);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = to_f32(u.e[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < valid ? to_f32(p[i]) : 0.0f;
+  }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_row(T* p, int valid, bool vec, const float (&v)[V]) {
+  constexpr int BYTES = V * (int)sizeof(T);
+  if (vec && V > 1) {
+    union { uint4 q[(BYTES + 15) / 16]; uint2 d; T e[V]; } u;
+#pragma unroll
+    for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
+    if (BYTES >= 16) {
+#pragma unroll
+      for (int i = 0; i < BYTES / 16; ++i) reinterpret_cast<uint4*>(p)[i] = u.q[i];
+    } else {
+      *reinterpret_cast<uint2*>(p) = u.d;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < valid) p[i] = from_f32<T>(v[i]);
+  }
+}
+
+// ---------------------------------------------------------------- activations
+// f(z) and f'(z) in f32.  ReLU is z > 0 ? z : 0, as the F32 path's.
+template <int ACT> __device__ __forceinline__ float act_value(float z) {
+  if (ACT == ORCA_ACT_RELU) return z > 0.0f ? z : 0.0f;
+  if (ACT == ORCA_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
+  if (ACT == ORCA_ACT_GELU_TANH) {
+    const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
+    return 0.5f * z * (1.0f + tanhf(u));
+  }
+  if (ACT == ORCA_ACT_SILU) return z / (1.0f + expf(-z));
+  return z;
+}
+template <int ACT> __device__ __forceinline__ float act_slope(float z) {
+  if (ACT == ORCA_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+  if (ACT == ORCA_ACT_GELU)
+    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
+           z * (expf(-0.5f * z * z) * 0.39894228040143268f);
+  if (ACT == ORCA_ACT_GELU_TANH) {
+    // Beyond |z| = 10 tanh is +-1 in f32 and the second term 0; the bound
+    // keeps z * z finite there.
+    const float y = fminf(fmaxf(z, -10.0f), 10.0f);
+    const float t = tanhf(0.79788456080286536f * (y + 0.044715f * y * y * y));
+    return 0.5f * (1.0f + t) +
+           0.5f * y * (1.0f - t * t) * (0.79788456080286536f * (1.0f + 0.134145f * y * y)) +
+           (z - z);   // NaN and infinities stay NaN
+  }
+  if (ACT == ORCA_ACT_SILU) {
+    const float g = 1.0f / (1.0f + expf(-z));
+    return g * (1.0f + z * (1.0f - g));
+  }
+  return 1.0f;
+}
+
+// v = f(v), or v = f'(v), for V values with one uniform branch for all.
+template <int V> __device__ __forceinline__ void apply_act(int act, float (&v)[V]) {
+#define ORCA_EACH(A)          \
+  case A:                     \
+    _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = act_value<A>(v[i]); \
+    break;
+  switch (act) {
+    ORCA_EACH(ORCA_ACT_RELU)
+    ORCA_EACH(ORCA_ACT_GELU)
+    ORCA_EACH(ORCA_ACT_GELU_TANH)
+    ORCA_EACH(ORCA_ACT_SILU)
+    default: break;
+  }
+#undef ORCA_EACH
+}
+template <int V> __device__ __forceinline__ void mul_slope(int act, const float (&z)[V], float (&v)[V]) {
+#define ORCA_EACH(A)          \
+  case A:                     \
+    _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] *= act_slope<A>(z[i]); \
+    break;
+  switch (act) {
+    ORCA_EACH(ORCA_ACT_RELU)
+    ORCA_EACH(ORCA_ACT_GELU)
+    ORCA_EACH(ORCA_ACT_GELU_TANH)
+    ORCA_EACH(ORCA_ACT_SILU)
+    default: break;
+  }
+#undef ORCA_EACH
+}
+
+// ---------------------------------------------------------------- 8-bit checkpoints
+// A matrix [m, n] in 8 bits: codes [m * n], then at the next multiple of 16
+// bytes one exponent byte per row and group of 32 columns.  value =
+// code * 2^(E - 127); the power of two makes both the scaling and the decoded
+// value exact (7 bits and a sign fit BF16), so rounding to the code is the only
+// error: at most half a step, one step where 127.5 and above saturate.  A
+// step is 2^-6 of the power of two at or below the group's largest value.
+constexpr int GROUP = 32;
+constexpr uint32_t E_NONFINITE = 255;
+
+__host__ __device__ inline int64_t ckpt_groups(int64_t n) { return (n + GROUP - 1) / GROUP; }
+__host__ __device__ inline int64_t ckpt_exps_at(int64_t m, int64_t n) { return (m * n + 15) / 16 * 16; }
+
+// amax_bits: the largest of the values' bits without the sign; as integers a
+// NaN is above an infinity and that above every finite value.
+__device__ __forceinline__ uint32_t ckpt_exponent(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return E_NONFINITE;
+  const int e = (int)(amax_bits >> 23) - 6;
+  return (uint32_t)(e < 1 ? 1 : e);
+}
+__device__ __forceinline__ float ckpt_up(uint32_t e) {      // 2^(127 - E); 0 for a marked group
+  return e == E_NONFINITE ? 0.0f : __uint_as_float((254u - e) << 23);
+}
+__device__ __forceinline__ float ckpt_down(uint32_t e) {    // 2^(E - 127); NaN for a marked group
+  return e == E_NONFINITE ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
+}
+__device__ __forceinline__ int ckpt_code(float v, float up) {
+  const int q = __float2int_rn(v * up);
+  return up == 0.0f ? 0 : (q < -127 ? -127 : (q > 127 ? 127 : q));
+}
+
+// Codes the V values of one lane, 32 / V adjacent lanes sharing a group (all
+// of them call this), and stores codes and exponent.  Columns from `valid` on
+// are outside.  `words`: 4-byte (V >= 4) stores are aligned; `quads`: 16-byte.
+template <int V>
+__device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_t row, int64_t n,
+                                           int64_t col, int valid, bool row_ok, int align,
+                                           const float (&v)[V]) {
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+    if (i < valid) amax = a > amax ? a : amax;
+  }
+#pragma unroll
+  for (int o = 1; o < GROUP / V; o <<= 1) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, amax, o);
+    amax = other > amax ? other : amax;
+  }
+  if (!row_ok || valid <= 0) return;
+  const uint32_t e = ckpt_exponent(amax);
+  const float up = ckpt_up(e);
+  if (col % GROUP == 0) exps[row * ckpt_groups(n) + col / GROUP] = (uint8_t)e;
+  uint8_t* p = codes + row * n + col;
+  if (V >= 4 && valid >= V && align >= 4) {
+    uint32_t w[(V + 3) / 4];
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i)
+      w[i] = (uint32_t)(ckpt_code(v[4 * i], up) & 255) |
+             (uint32_t)(ckpt_code(v[4 * i + 1], up) & 255) << 8 |
+             (uint32_t)(ckpt_code(v[4 * i + 2], up) & 255) << 16 |
+             (uint32_t)(ckpt_code(v[4 * i + 3], up) & 255) << 24;
+    if (V >= 16 && align >= 16) {
+#pragma unroll
+      for (int i = 0; i < V / 16; ++i)
+        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
+    } else if (V >= 8 && align >= 8) {
+#pragma unroll
+      for (int i = 0; i < V / 8; ++i)
+        reinterpret_cast<uint2*>(p)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (i < valid) p[i] = (uint8_t)(ckpt_code(v[i], up) & 255);
+  }
+}
+
+// The V values at (row, col .. col + V) of a checkpoint; V divides 32 and col
+// is a multiple of V, so they share one exponent.
+template <int V>
+__device__ __forceinline__ void ckpt_load(const uint8_t* codes, const uint8_t* exps, int64_t row,
+                                          int64_t n, int64_t col, int valid, int align,
+                                          float (&v)[V]) {
+  const float down = valid > 0 ? ckpt_down(exps[row * ckpt_groups(n) + col / GROUP]) : 0.0f;
+  const uint8_t* p = codes + row * n + col;
+  if (V >= 4 && valid >= V && align >= 4) {
+    uint32_t w[(V + 3) / 4];
+    if (V >= 16 && align >= 16) {
+#pragma unroll
+      for (int i = 0; i < V / 16; ++i) {
+        const uint4 q = reinterpret_cast<const uint4*>(p)[i];
+        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
+      }
+    } else if (V >= 8 && align >= 8) {
+#pragma unroll
+      for (int i = 0; i < V / 8; ++i) {
+        const uint2 q = reinterpret_cast<const uint2*>(p)[i];
+        w[2 * i] = q.x; w[2 * i + 1] = q.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < V / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * down;
+  } else {
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = i < valid ? (float)(int8_t)p[i] * down : 0.0f;
+  }
+}
+
+// Largest of 16, 8, 4, 1 that divides both the pointer and the row stride.
+inline int byte_alignment(const void* p, int64_t stride) {
+  const uint64_t v = reinterpret_cast<uintptr_t>(p) | (uint64_t)stride;
+  return v % 16 == 0 ? 16 : (v % 8 == 0 ? 8 : (v % 4 == 0 ? 4 : 1));
+}
+
+// ---------------------------------------------------------------- epilogue
+enum Mode : int { FWD = 0, DX = 1, DW = 2 };
+
+// What becomes of the f32 sums D[rows, cols]; every matrix is row-major with
+// `cols` columns.
+struct Epilogue {
+  int64_t rows = 0, cols = 0;
+  int act = ORCA_ACT_NONE;
+  int vec = 0;                        // 16-byte accesses are aligned in every T matrix below
+  int ckpt_align = 1;                 // of a checkpoint's rows, in bytes
+  void* out = nullptr;                // T; DW with out_f32: float
+  int out_f32 = 0;
+  const void* bias = nullptr;         // FWD: T [cols]
+  const void* residual = nullptr;     // FWD, DX: T
+  void* z = nullptr;                  // FWD: the pre-activation in T, kept
+  uint8_t* codes = nullptr;           // FWD: kept in 8 bits; DX: x in 8 bits
+  uint8_t* exps = nullptr;
+  const void* x = nullptr;            // DX: x in T (with an activation only)
+};
+
+// V consecutive columns of one row per thread, 32 / V adjacent lanes on
+// adjacent columns.  All lanes of a warp call it together.
+template <typename T, int MODE, int V>
+__device__ __forceinline__ void epilogue(const Epilogue& e, int64_t row, int64_t col, float (&v)[V]) {
+  const bool row_ok = row < e.rows;
+  const int valid = !row_ok || col >= e.cols ? 0 : (e.cols - col < V ? (int)(e.cols - col) : V);
+  const bool vec = e.vec && valid == V;
+  const int64_t at = row * e.cols + col;
+  if (MODE == DW) {
+    if (valid <= 0) return;
+    if (e.out_f32) store_row<float, V>((float*)e.out + at, valid, vec, v);
+    else store_row<T, V>((T*)e.out + at, valid, vec, v);
+    return;
+  }
+  float t[V];
+  if (MODE == FWD) {
+    if (e.bias && valid > 0) {
+      load_row<T, V>((const T*)e.bias + col, valid, vec, t);
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] += t[i];
+    }
+    if (e.z && valid > 0) store_row<T, V>((T*)e.z + at, valid, vec, v);
+    if (e.codes) ckpt_store<V>(e.codes, e.exps, row, e.cols, col, valid, row_ok, e.ckpt_align, v);
+    if (valid <= 0) return;
+    apply_act<V>(e.act, v);
+  } else {
+    if (valid <= 0) return;
+    if (e.act != ORCA_ACT_NONE) {
+      if (e.codes) ckpt_load<V>(e.codes, e.exps, row, e.cols, col, valid, e.ckpt_align, t);
+      else load_row<T, V>((const T*)e.x + at, valid, vec, t);
+      mul_slope<V>(e.act, t, v);
+    }
+  }
+  if (e.residual) {
+    load_row<T, V>((const T*)e.residual + at, valid, vec, t);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] += t[i];
+  }
+  store_row<T, V>((T*)e.out + at, valid, vec, v);
+}
+
+}  // namespace lin
+
+// ckpt8.cu: enqueue on ctx->stream; checked arguments.
+orca_status ckpt8_pack_launch(orca_ctx* ctx, const void* x, orca_dtype dtype, int64_t m, int64_t n,
+                              uint8_t* ckpt);
+orca_status ckpt8_unpack_launch(orca_ctx* ctx, const uint8_t* ckpt, int64_t m, int64_t n, int act,
+                                void* out, orca_dtype dtype);
+// out = act(x), rounded to the type once (the operand of dW from a plainly kept x).
+orca_status act_launch(orca_ctx* ctx, const void* x, orca_dtype dtype, int64_t len, int act, void* out);
+
+// Checks of spans (linear.cu).
+orca_status need_span(orca_ctx* ctx, const orca_span* s, int64_t len, const char* what);
+orca_status need_apart(const orca_span* out, const orca_span* other, const char* what);
+orca_status need_float(const orca_span* s, const char* what);
+orca_status need_dim(int64_t v, const char* what);
+
+}  // namespace orca

@@ -67,7 +67,7 @@ void ctx_release(orca_ctx* ctx) {
   cudaFree(ctx->dev_err);
   cudaFree(ctx->tile_ctr);
   if (ctx->sync_event) cudaEventDestroy(ctx->sync_event);
-  cudaStreamDestroy(ctx->stream);
+  if (ctx->owns_stream) cudaStreamDestroy(ctx->stream);
   cudaStreamDestroy(ctx->comm_stream);
   delete ctx;
 }
@@ -387,7 +387,7 @@ const char* orca_status_string(orca_status s) {
 
 uint32_t orca_version(void) { return 0x000100u; }
 
-orca_status orca_ctx_create(int device, orca_ctx** out) {
+static orca_status ctx_create(int device, bool own_stream, cudaStream_t stream, orca_ctx** out) {
   if (!out) return fail(ORCA_INVALID_ARGUMENT, "null output pointer");
   int count = 0;
   ORCA_CUDA_TRY(cudaGetDeviceCount(&count));
@@ -399,10 +399,18 @@ orca_status orca_ctx_create(int device, orca_ctx** out) {
   if (prop.major != 10)
     return fail(ORCA_UNSUPPORTED_DTYPE, "device %d is sm_%d%d; this library is built for sm_100a",
                 device, prop.major, prop.minor);
+  if (!own_stream && stream) {
+    int at = -1;
+    ORCA_CUDA_TRY(cudaStreamGetDevice(stream, &at));
+    if (at != device)
+      return fail(ORCA_DEVICE_MISMATCH, "the stream belongs to device %d, not %d", at, device);
+  }
   orca_ctx* c = new orca_ctx();
   c->device = device;
   c->sm_count = prop.multiProcessorCount;
-  ORCA_CUDA_TRY(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
+  c->owns_stream = own_stream;
+  if (own_stream) ORCA_CUDA_TRY(cudaStreamCreateWithFlags(&c->stream, cudaStreamNonBlocking));
+  else c->stream = stream;
   // Collectives get the highest stream priority: when a GEMM CTA retires, a
   // waiting all-reduce takes the SM before more GEMM CTAs do (the GEMM's
   // dynamic tile scheduler lets the CTAs that start later take fewer tiles).
@@ -427,6 +435,14 @@ orca_status orca_ctx_create(int device, orca_ctx** out) {
   }
   *out = c;
   return ORCA_OK;
+}
+
+orca_status orca_ctx_create(int device, orca_ctx** out) {
+  return ctx_create(device, true, nullptr, out);
+}
+
+orca_status orca_ctx_create_on_stream(int device, void* stream, orca_ctx** out) {
+  return ctx_create(device, false, (cudaStream_t)stream, out);
 }
 
 orca_status orca_ctx_destroy(orca_ctx* ctx) {
