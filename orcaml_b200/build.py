@@ -17,7 +17,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 LIB = os.path.join(HERE, "liborca_cuda.so")
-SOURCES = ["ops.cu", "gemm.cu", "mlp.cu", "comm.cu", "ckpt8.cu", "linear.cu"]
+SOURCES = ["ops.cu", "gemm.cu", "mlp.cu", "comm.cu", "ckpt8.cu", "linear.cu",
+           "linear_mma.cu"]
 HEADERS = ["common.cuh", "gemm.cuh", "linear.cuh"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

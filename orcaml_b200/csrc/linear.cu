@@ -1,6 +1,7 @@
 // linear.cu -- fused linear operators: out = act(x @ w + b) + residual and its
 // backward, in BF16, F16 and F32.
 #include <algorithm>
+#include <type_traits>
 
 #include "linear.cuh"
 
@@ -50,30 +51,6 @@ orca_status need_apart(const orca_span* out, const orca_span* other, const char*
 }
 
 namespace lin {
-
-// ---------------------------------------------------------------- operands
-// Element (i, c) of an operand, i along the output and c along the sum:
-// at c * ld + i when mn_major, else at i * ld + c.
-struct Operand {
-  const void* p = nullptr;
-  int64_t ld = 0;
-  int mn_major = 0;
-};
-
-// Stream-ordered scratch of one call; in a captured graph it becomes the
-// graph's own allocation, so graphs share nothing.
-struct Scratch {
-  orca_ctx* ctx;
-  void* p = nullptr;
-  explicit Scratch(orca_ctx* c) : ctx(c) {}
-  ~Scratch() { if (p) cudaFreeAsync(p, ctx->stream); }
-  Scratch(const Scratch&) = delete;
-  Scratch& operator=(const Scratch&) = delete;
-  orca_status get(size_t bytes) {
-    ORCA_CUDA_TRY(cudaMallocAsync(&p, bytes, ctx->stream));
-    return ORCA_OK;
-  }
-};
 
 // ---------------------------------------------------------------- FFMA tiles
 // 64 x 64 tiles of F32 sums, each a sequential FMA chain over the sum's
@@ -201,6 +178,10 @@ static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   if (e.bias) al = std::min(al, byte_alignment(e.bias, 0));
   e.vec = al == 16;
   if (e.codes) e.ckpt_align = byte_alignment(e.codes, N);
+  if (K > 0) {
+    const orca_dtype t = std::is_same<T, float>::value ? ORCA_F32 : (std::is_same<T, __half>::value ? ORCA_F16 : ORCA_BF16);
+    return mma_product(ctx, MODE, t, M, N, K, A, B, e);
+  }
   const int64_t tiles = cdiv(M, SM) * cdiv(N, SN);
   if (tiles > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
   tile_kernel<T, MODE><<<(unsigned)tiles, 256, 0, ctx->stream>>>(M, N, K, A, B, e);

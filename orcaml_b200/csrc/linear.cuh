@@ -319,6 +319,36 @@ orca_status ckpt8_unpack_launch(orca_ctx* ctx, const uint8_t* ckpt, int64_t m, i
 // out = act(x), rounded to the type once (the operand of dW from a plainly kept x).
 orca_status act_launch(orca_ctx* ctx, const void* x, orca_dtype dtype, int64_t len, int act, void* out);
 
+namespace lin {
+// Element (i, c) of an operand, i along the output and c along the sum: at
+// c * ld + i when mn_major, else at i * ld + c.
+struct Operand {
+  const void* p = nullptr;
+  int64_t ld = 0;
+  int mn_major = 0;
+};
+
+// Stream-ordered scratch of one call; in a captured graph it becomes the
+// graph's own allocation, so graphs share nothing.
+struct Scratch {
+  orca_ctx* ctx;
+  void* p = nullptr;
+  explicit Scratch(orca_ctx* c) : ctx(c) {}
+  ~Scratch() { if (p) cudaFreeAsync(p, ctx->stream); }
+  Scratch(const Scratch&) = delete;
+  Scratch& operator=(const Scratch&) = delete;
+  orca_status get(size_t bytes) {
+    ORCA_CUDA_TRY(cudaMallocAsync(&p, bytes, ctx->stream));
+    return ORCA_OK;
+  }
+};
+}  // namespace lin
+
+// linear_mma.cu: D[M, N] = A @ B on the tensor cores, through the epilogue.
+// K > 0; operands of element type `dtype`, any alignment.
+orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, int64_t N, int64_t K,
+                        const lin::Operand& A, const lin::Operand& B, const lin::Epilogue& e);
+
 // Checks of spans (linear.cu).
 orca_status need_span(orca_ctx* ctx, const orca_span* s, int64_t len, const char* what);
 orca_status need_apart(const orca_span* out, const orca_span* other, const char* what);

@@ -1,0 +1,546 @@
+// linear_mma.cu -- the products of the fused linear operators on the 5th-generation
+// tensor cores.
+//
+// BF16 and F16 operands go to tcgen05.mma kind::f16 as they are.  An F32 operand
+// is split exactly into three BF16 planes, x = x0 + x1 + x2 (8 significant bits
+// each, by truncation), and the product is the sum of six plane products,
+// x2*y0 + x0*y2 + x1*y1 + x1*y0 + x0*y1 + x0*y0; the three left out are below
+// 2^-24 of |x||y|.  Both kinds run through the same kernels: a step of the sum
+// is one 64-deep block of one plane pair.
+//
+//  * pair_kernel: 256 x 256 output tiles on clusters of two CTAs
+//    (cta_group::2), persistent; for outputs with enough tiles.
+//  * split_kernel: 128 columns x 16..128 rows of the output per cluster, the sum
+//    split over the cluster's CTAs and joined through their shared memory; for
+//    few rows, where the weights are read once at HBM speed, and for outputs
+//    with few tiles.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <type_traits>
+
+#include "linear.cuh"
+
+namespace orca {
+namespace lin {
+
+constexpr int BK = 64;                       // 128 bytes of 16-bit elements: one swizzle row
+constexpr int ROWS = 128;                    // rows of an operand tile
+constexpr int TILE = ROWS * BK * 2;          // 16 KB
+
+// F32 plane pairs in the order they are added, smallest first; 4 bits each.
+constexpr uint32_t PAIR_A = 0x001102u, PAIR_B = 0x010120u;   // pair p: (x >> 4 * p) & 15
+constexpr int F32_PAIRS = 6;
+
+// Steps (of four MMAs) per accumulation chunk of an F32 result.
+constexpr int CHUNK = 8;
+
+// Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
+//  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
+//    offset); the 16-deep step s starts 32 * s bytes further.
+//  MN-major: boxes of 64 mn x 64 k, k row at 128 bytes, 8-row groups of k 1024
+//    bytes apart (stride offset), boxes 8 KB apart (leading offset); step s
+//    starts 16 rows = 2 KB further.
+__device__ __forceinline__ uint64_t desc(uint32_t base, int mn_major, int step) {
+  const uint32_t addr = base + (mn_major ? step * 2048 : step * 32);
+  const uint32_t lbo = mn_major ? 8192 : 16;
+  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 |
+         (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+
+// kind::f16 instruction descriptor: F32 accumulator, operand types (1 = BF16,
+// 0 = F16), orientations, N and M.
+__device__ __forceinline__ uint32_t idesc(int bf16, int a_mn, int b_mn, int n, int m) {
+  return (1u << 4) | ((uint32_t)bf16 << 7) | ((uint32_t)bf16 << 10) | ((uint32_t)a_mn << 15) |
+         ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t id, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+      "r"(id), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t id,
+                                             uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
+      "r"(id), "r"(acc)
+      : "memory");
+}
+
+struct Params {
+  int64_t M, N, K;
+  int a_mn, b_mn;
+  int bf16;
+  int pairs;               // plane pairs: 1, or F32_PAIRS
+  int chunk;               // steps per accumulation chunk
+  int group_m;             // tile rows per raster group
+  int* dev_err;
+  Epilogue e;
+};
+
+// Tile row 0 of `rows` (64 or 128, 16.. for K-major) of an operand: one box, or
+// one box per 64 when MN-major.
+__device__ __forceinline__ void load_tile(uint8_t* dst, const CUtensorMap* map, uint64_t* bar,
+                                          int mn_major, int rows, int64_t mn0, int64_t k0, int plane) {
+  if (mn_major) {
+    for (int c = 0; c < rows / 64; ++c)
+      tma_load_3d(dst + c * 8192, map, bar, (int)(mn0 + 64 * c), (int)k0, plane);
+  } else {
+    tma_load_3d(dst, map, bar, (int)k0, (int)mn0, plane);
+  }
+}
+__device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* map, uint32_t bar_cl,
+                                               int mn_major, int rows, int64_t mn0, int64_t k0,
+                                               int plane) {
+  if (mn_major) {
+    for (int c = 0; c < rows / 64; ++c)
+      tma_load_3d_pair(dst + c * 8192, map, bar_cl, (int)(mn0 + 64 * c), (int)k0, plane);
+  } else {
+    tma_load_3d_pair(dst, map, bar_cl, (int)k0, (int)mn0, plane);
+  }
+}
+
+__device__ __forceinline__ void tile_at(int64_t tile, int64_t num_m, int64_t num_n, int group_m,
+                                        int64_t& tm, int64_t& tn) {
+  const int64_t size = (int64_t)group_m * num_n;
+  const int64_t first = tile / size * group_m;
+  const int64_t gm = num_m - first < group_m ? num_m - first : group_m;
+  const int64_t r = tile % size;
+  tm = first + r % gm;
+  tn = r / gm;
+}
+
+// ---------------------------------------------------------------- CTA pairs
+// Roles: warp 0 loads, warp 1 (of the even CTA) issues the MMAs, warps 2-9
+// drain one of two 256-column accumulators while the MMAs fill the other.  The
+// even CTA's full barrier counts both CTAs' bytes; the MMA's commits free the
+// stage and publish the accumulator in both.  CHUNKED (F32 results): the
+// accumulator is emptied every `chunk` steps into F32 registers, because the
+// tensor core adds with a few bits less than F32 and one long chain would lose
+// them.  Every wait is bounded; a role that gives up raises the abort flag of
+// both CTAs, and both pass the same two cluster barriers in every case.
+constexpr int EPI_WARPS = 8;
+constexpr int PAIR_THREADS = 64 + 32 * EPI_WARPS;
+constexpr int PAIR_STAGES = 6;
+constexpr int PAIR_STAGE = 2 * TILE;                     // A and B, this CTA's halves
+constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024 + 256;
+constexpr int ACC_COLS = 256;
+
+template <typename T, int MODE, bool CHUNKED>
+__global__ void __launch_bounds__(PAIR_THREADS, 1)
+pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+            const __grid_constant__ Params p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PAIR_STAGES * PAIR_STAGE);
+  uint64_t* full_bar = bars;                              // (even) both CTAs' bytes
+  uint64_t* empty_bar = bars + PAIR_STAGES;
+  uint64_t* tfull_bar = bars + 2 * PAIR_STAGES;           // [2]
+  uint64_t* tempty_bar = bars + 2 * PAIR_STAGES + 2;      // [2] (even)
+  uint64_t* drain_bar = bars + 2 * PAIR_STAGES + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PAIR_STAGES + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const uint32_t rank = cluster_ctarank();
+  const bool even = rank == 0;
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int64_t num_m = cdiv(p.M, 256), num_n = cdiv(p.N, 256), tiles = num_m * num_n;
+  const int64_t cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  const int steps = (int)cdiv(p.K, BK) * p.pairs;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < PAIR_STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 2 * EPI_WARPS);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&map_a);
+    prefetch_tmap(&map_b);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, 2 * ACC_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const uint32_t peer_abort = cluster_addr(const_cast<int*>(abort_flag), rank ^ 1u);
+  auto raise_abort = [&]() {
+    *abort_flag = 1;
+    st_remote_u32(peer_abort, 1u);
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued[PAIR_STAGES];
+      for (int s = 0; s < PAIR_STAGES; ++s) issued[s] = -1;
+      uint64_t last_issue = 0;
+      bool ok = true;
+      for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
+        int64_t tm, tn;
+        tile_at(tile, num_m, num_n, p.group_m, tm, tn);
+        const int64_t row = tm * 256 + (int64_t)rank * 128, col = tn * 256 + (int64_t)rank * 128;
+        int pair = 0;
+        int64_t k0 = 0;
+        for (int it = 0; it < steps; ++it) {
+          const int pa = p.pairs == 1 ? 0 : (int)(PAIR_A >> (4 * pair)) & 15;
+          const int pb = p.pairs == 1 ? 0 : (int)(PAIR_B >> (4 * pair)) & 15;
+          if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.dev_err)) {
+            ok = false;
+            break;
+          }
+          uint8_t* a_dst = smem + stage * PAIR_STAGE;
+          if (even) {
+            mbar_arrive_expect_tx(&full_bar[stage], 2 * PAIR_STAGE);
+            load_tile(a_dst, &map_a, &full_bar[stage], p.a_mn, ROWS, row, k0, pa);
+            load_tile(a_dst + TILE, &map_b, &full_bar[stage], p.b_mn, ROWS, col, k0, pb);
+            issued[stage] = (int)phase;
+          } else {
+            const uint32_t bar = cluster_addr(&full_bar[stage], 0);
+            load_tile_pair(a_dst, &map_a, bar, p.a_mn, ROWS, row, k0, pa);
+            load_tile_pair(a_dst + TILE, &map_b, bar, p.b_mn, ROWS, col, k0, pb);
+            last_issue = global_ns();
+          }
+          if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
+          if (++pair == p.pairs) { pair = 0; k0 += BK; }
+        }
+      }
+      if (!ok) {
+        raise_abort();
+        // The odd CTA's copies count on the even CTA's barrier: after an abort
+        // it cannot see them land and waits far longer than a copy takes.
+        if (!even && last_issue)
+          while (global_ns() - last_issue < 50000ull) {
+          }
+      }
+      // Never leave with copies in flight into this CTA's shared memory.
+      for (int s = 0; s < PAIR_STAGES; ++s) {
+        if (issued[s] < 0) continue;
+        const uint64_t t0 = global_ns();
+        while (!mbar_try_wait(&full_bar[s], (uint32_t)issued[s]) && global_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (even && lane == 0) {
+      const uint32_t id = idesc(p.bf16, p.a_mn, p.b_mn, 256, 256);
+      int stage = 0;
+      uint32_t phase = 0, chunks = 0;
+      bool ok = true;
+      for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
+        int in_chunk = 0;
+        for (int it = 0; it < steps; ++it) {
+          const int buf = (int)(chunks & 1u);
+          if (in_chunk == 0) {
+            if (!mbar_wait(&tempty_bar[buf], ((chunks >> 1) & 1u) ^ 1u, abort_flag, p.dev_err)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+          }
+          if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) { ok = false; break; }
+          tc_fence_after();
+          const uint32_t a = smem_u32(smem + stage * PAIR_STAGE), b = a + TILE;
+          const uint32_t d = tmem + (uint32_t)(buf * ACC_COLS);
+#pragma unroll
+          for (int s = 0; s < BK / 16; ++s)
+            mma_f16_pair(d, desc(a, p.a_mn, s), desc(b, p.b_mn, s), id, (in_chunk | s) ? 1u : 0u);
+          tc_commit_pair(cluster_addr(&empty_bar[stage], 0));
+          tc_commit_pair(cluster_addr(&empty_bar[stage], 1));
+          if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
+          if (++in_chunk == p.chunk || it == steps - 1) {
+            tc_commit_pair(cluster_addr(&tfull_bar[buf], 0));
+            tc_commit_pair(cluster_addr(&tfull_bar[buf], 1));
+            ++chunks;
+            in_chunk = 0;
+          }
+        }
+      }
+      if (!ok) raise_abort();
+      tc_commit_pair(cluster_addr(drain_bar, 0));
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(drain_bar, 0) && global_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+  } else {
+    // Warp w reads TMEM lanes [32 * (w % 4), +32) and columns [128 * half, +128).
+    const int quarter = warp & 3, half = (warp - 2) / 4;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    const uint32_t tempty[2] = {cluster_addr(&tempty_bar[0], 0), cluster_addr(&tempty_bar[1], 0)};
+    const int nchunks = (steps + p.chunk - 1) / p.chunk;
+    uint32_t chunks = 0;
+    bool ok = true;
+    for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
+      int64_t tm, tn;
+      tile_at(tile, num_m, num_n, p.group_m, tm, tn);
+      const int64_t row = tm * 256 + (int64_t)rank * 128 + quarter * 32 + lane;
+      const int64_t col = tn * 256 + half * 128;
+      if (CHUNKED) {
+        float acc[128];
+#pragma unroll
+        for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+        for (int c = 0; c < nchunks; ++c) {
+          const int buf = (int)(chunks & 1u);
+          if (!mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+#pragma unroll
+          for (int q = 0; q < 8; ++q) {
+            float v[16];
+            tmem_ld_32x32b_x16(lanes + (uint32_t)(buf * ACC_COLS + q * 16), v);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) acc[q * 16 + j] = __fadd_rn(acc[q * 16 + j], v[j]);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_remote(tempty[buf]);
+          ++chunks;
+        }
+        if (!ok) break;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          if (col + q * 32 < p.N) {
+            float v[32];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = acc[q * 32 + j];
+            epilogue<T, MODE, 32>(p.e, row, col + q * 32, v);
+          }
+        }
+      } else {
+        const int buf = (int)(chunks & 1u);
+        if (!mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int q = 0; q < 4; ++q) {
+          if (col + q * 32 < p.N) {
+            float v[32];
+            tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
+            epilogue<T, MODE, 32>(p.e, row, col + q * 32, v);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(tempty[buf]);
+        ++chunks;
+      }
+    }
+    if (!ok) raise_abort();
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync_all();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, 2 * ACC_COLS);
+}
+
+// ---------------------------------------------------------------- operand preparation
+// [rows, cols] (row stride ld) -> planes of BF16 / F16 with row stride ldp (a
+// multiple of 8): F32 is split, 16-bit types are copied.  The padding is outside
+// the tensor map and not written.
+template <typename S>
+__global__ void __launch_bounds__(256)
+prepare_kernel(const S* __restrict__ x, int64_t rows, int64_t cols, int64_t ld, uint16_t* __restrict__ out,
+               int64_t ldp) {
+  const int64_t plane = rows * ldp, per_row = ldp / 8, vecs = rows * per_row;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * 256) {
+    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
+    const S* p = x + r * ld + c;
+    union { uint4 q; uint16_t e[8]; } u[3];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      if (sizeof(S) == 4) {
+        const float v = c + j < cols ? (float)to_f32(p[j]) : 0.0f;
+        const uint32_t b0 = __float_as_uint(v) & 0xffff0000u;
+        const float r1 = v - __uint_as_float(b0);
+        const uint32_t b1 = __float_as_uint(r1) & 0xffff0000u;
+        const float r2 = r1 - __uint_as_float(b1);
+        // An infinity or a NaN has no remainder: its first plane carries it.
+        const bool fine = (b0 & 0x7f800000u) != 0x7f800000u;
+        u[0].e[j] = (uint16_t)((fine ? b0 : (__float_as_uint(v) | (v != v ? 0x400000u : 0u))) >> 16);
+        u[1].e[j] = fine ? (uint16_t)(b1 >> 16) : (uint16_t)0;
+        u[2].e[j] = fine ? (uint16_t)(__float_as_uint(r2) >> 16) : (uint16_t)0;
+      } else {
+        u[0].e[j] = c + j < cols ? reinterpret_cast<const uint16_t*>(p)[j] : (uint16_t)0;
+      }
+    }
+    uint4* o = reinterpret_cast<uint4*>(out + r * ldp + c);
+    o[0] = u[0].q;
+    if (sizeof(S) == 4) {
+      *reinterpret_cast<uint4*>(out + plane + r * ldp + c) = u[1].q;
+      *reinterpret_cast<uint4*>(out + 2 * plane + r * ldp + c) = u[2].q;
+    }
+  }
+}
+
+// An operand as the tensor maps take it: 16-bit planes, rows 16-byte aligned.
+struct Planes {
+  const void* p;
+  int64_t ld, plane;      // elements
+  int64_t rows, cols;     // rows of cols contiguous elements
+};
+
+static orca_status prepare(orca_ctx* ctx, orca_dtype dtype, const Operand& op, int64_t mn, int64_t k,
+                           Scratch& scratch, Planes* out) {
+  out->rows = op.mn_major ? k : mn;
+  out->cols = op.mn_major ? mn : k;
+  out->ld = op.ld;
+  out->plane = out->rows * out->ld;
+  out->p = op.p;
+  if (dtype != ORCA_F32 && byte_alignment(op.p, op.ld * 2) == 16) return ORCA_OK;
+  out->ld = cdiv(out->cols, 8) * 8;
+  out->plane = out->rows * out->ld;
+  const int planes = dtype == ORCA_F32 ? 3 : 1;
+  ORCA_TRY(scratch.get((size_t)(planes * out->plane) * 2));
+  out->p = scratch.p;
+  const int64_t vecs = out->plane / 8;
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(vecs, 256), (int64_t)ctx->sm_count * 16);
+  if (dtype == ORCA_F32)
+    prepare_kernel<float><<<grid, 256, 0, ctx->stream>>>((const float*)op.p, out->rows, out->cols, op.ld,
+                                                         (uint16_t*)scratch.p, out->ld);
+  else
+    prepare_kernel<__half><<<grid, 256, 0, ctx->stream>>>((const __half*)op.p, out->rows, out->cols, op.ld,
+                                                          (uint16_t*)scratch.p, out->ld);
+  count_launch(ctx);
+  ORCA_CUDA_TRY(cudaGetLastError());
+  return ORCA_OK;
+}
+
+// ---------------------------------------------------------------- tensor maps
+static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
+}
+
+// Boxes of 64 columns (one 128-byte swizzle row) x box_rows rows of one plane.
+static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int bf16, int box_rows) {
+  auto encode = encode_fn();
+  if (!encode) return fail(ORCA_CUDA_ERROR, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[3] = {(cuuint64_t)x.cols, (cuuint64_t)x.rows, (cuuint64_t)planes};
+  cuuint64_t strides[2] = {(cuuint64_t)(x.ld * 2), (cuuint64_t)(x.plane * 2)};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1};
+  cuuint32_t step[3] = {1, 1, 1};
+  const CUresult r = encode(map, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
+                            3, const_cast<void*>(x.p), dims, strides, box, step,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(ORCA_CUDA_ERROR, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return ORCA_OK;
+}
+
+// ---------------------------------------------------------------- launches
+template <typename T, int MODE, bool CHUNKED>
+static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, const Params& p) {
+  const auto kernel = pair_kernel<T, MODE, CHUNKED>;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(ctx->sm_count / 2 * 2));
+  cfg.blockDim = dim3(PAIR_THREADS);
+  cfg.dynamicSmemBytes = PAIR_SMEM;
+  cfg.stream = ctx->stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  static std::atomic<int> fits[64];      // clusters that are resident at once, per device
+  std::atomic<int>& fit = fits[ctx->device & 63];
+  if (fit.load() == 0) {
+    ORCA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
+    int n = 0;
+    ORCA_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    if (n < 1) return fail(ORCA_CUDA_ERROR, "no cluster of two CTAs fits on the device");
+    fit.store(n);
+  }
+  const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
+  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, fit.load())));
+  ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p));
+  count_launch(ctx);
+  return ORCA_OK;
+}
+
+template <typename T, int MODE>
+static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, const Planes& b, Params& p) {
+  const int planes = dtype == ORCA_F32 ? 3 : 1;
+  CUtensorMap ma, mb;
+  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : ROWS));
+  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
+  const int64_t steps = cdiv(p.K, BK) * p.pairs;
+  if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
+  if constexpr (std::is_same<T, float>::value) {
+    p.chunk = CHUNK;
+    return launch_pair<T, MODE, true>(ctx, ma, mb, p);
+  } else {
+    if constexpr (MODE == DW) {
+      if (p.e.out_f32) {
+        p.chunk = CHUNK;
+        return launch_pair<T, MODE, true>(ctx, ma, mb, p);
+      }
+    }
+    p.chunk = (int)steps;
+    return launch_pair<T, MODE, false>(ctx, ma, mb, p);
+  }
+}
+
+}  // namespace lin
+
+orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, int64_t N, int64_t K,
+                        const lin::Operand& A, const lin::Operand& B, const lin::Epilogue& e) {
+  using namespace lin;
+  Scratch sa(ctx), sb(ctx);
+  Planes a, b;
+  ORCA_TRY(prepare(ctx, dtype, A, M, K, sa, &a));
+  ORCA_TRY(prepare(ctx, dtype, B, N, K, sb, &b));
+  Params p;
+  p.M = M; p.N = N; p.K = K;
+  p.a_mn = A.mn_major;
+  p.b_mn = B.mn_major;
+  p.bf16 = dtype != ORCA_F16;
+  p.pairs = dtype == ORCA_F32 ? F32_PAIRS : 1;
+  p.group_m = 8;
+  p.dev_err = ctx->dev_err;
+  p.e = e;
+#define ORCA_MODE(MODE)                                                            \
+  if (dtype == ORCA_F32) return dispatch<float, MODE>(ctx, dtype, a, b, p);        \
+  if (dtype == ORCA_F16) return dispatch<__half, MODE>(ctx, dtype, a, b, p);       \
+  return dispatch<__nv_bfloat16, MODE>(ctx, dtype, a, b, p);
+  switch (mode) {
+    case FWD: { ORCA_MODE(FWD) }
+    case DX: { ORCA_MODE(DX) }
+    default: { ORCA_MODE(DW) }
+  }
+#undef ORCA_MODE
+}
+
+}  // namespace orca
