@@ -357,6 +357,182 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   if (warp == 1) tmem_dealloc_pair(tmem, 2 * ACC_COLS);
 }
 
+// ---------------------------------------------------------------- few rows, few tiles
+// One output tile of 128 columns x NT rows per cluster: the columns (weights) are
+// the MMA's 128 rows, so few rows of the output cost little.  The cluster's CTAs
+// take equal parts of the sum; their F32 parts meet in shared memory and each CTA
+// adds, in rank order, and stores a share of the rows.  Warp 0 loads, warp 1
+// issues the MMAs, warps 2-5 (one TMEM lane quarter each) hold a column per
+// thread.  With few rows the weights' bytes are all the work, and the stages
+// keep ~190 KB of them in flight per SM.
+constexpr int SPLIT_THREADS = 192;
+template <int NT> constexpr int split_stage() { return TILE + NT * BK * 2; }
+template <int NT> constexpr int split_stages() { return 196608 / split_stage<NT>() < 12 ? 196608 / split_stage<NT>() : 12; }
+template <int NT> constexpr int split_smem() { return split_stages<NT>() * split_stage<NT>() + 1024 + 256; }
+
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+template <typename T, int MODE, int NT>
+__global__ void __launch_bounds__(SPLIT_THREADS, 1)
+split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
+             const __grid_constant__ Params p, int ranks) {
+  constexpr int STAGES = split_stages<NT>(), STAGE = split_stage<NT>();
+  constexpr uint32_t COLS = 2 * NT;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE);
+  uint64_t* full_bar = bars;
+  uint64_t* empty_bar = bars + STAGES;
+  uint64_t* tfull_bar = bars + 2 * STAGES;        // [2]
+  uint64_t* tempty_bar = bars + 2 * STAGES + 2;   // [2]
+  uint64_t* drain_bar = bars + 2 * STAGES + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  float* part = reinterpret_cast<float*>(smem);   // [NT][128], once the stages are done with
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int rank = (int)cluster_ctarank();
+  const int64_t tile = blockIdx.x / ranks, num_n = cdiv(p.N, 128);
+  const int64_t col0 = tile % num_n * 128, row0 = tile / num_n * NT;
+  const int64_t steps = cdiv(p.K, BK) * p.pairs;
+  const int begin = (int)(steps * rank / ranks), end = (int)(steps * (rank + 1) / ranks);
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int a = 0; a < 2; ++a) {
+      mbar_init(&tfull_bar[a], 1);
+      mbar_init(&tempty_bar[a], 4);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tmap(&map_p);
+    prefetch_tmap(&map_q);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  float acc[NT];
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int stage = 0;
+      uint32_t phase = 0;
+      int issued = 0;
+      int pair = begin % p.pairs;
+      int64_t k0 = (int64_t)(begin / p.pairs) * BK;
+      for (int it = begin; it < end; ++it) {
+        const int pq = p.pairs == 1 ? 0 : (int)(PAIR_A >> (4 * pair)) & 15;
+        const int pp = p.pairs == 1 ? 0 : (int)(PAIR_B >> (4 * pair)) & 15;
+        if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.dev_err)) break;
+        uint8_t* dst = smem + stage * STAGE;
+        mbar_arrive_expect_tx(&full_bar[stage], STAGE);
+        load_tile(dst, &map_p, &full_bar[stage], p.b_mn, 128, col0, k0, pp);
+        load_tile(dst + TILE, &map_q, &full_bar[stage], p.a_mn, NT, row0, k0, pq);
+        ++issued;
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        if (++pair == p.pairs) { pair = 0; k0 += BK; }
+      }
+      // Never leave with copies in flight: every stage's last use has landed.
+      for (int s = 0; s < STAGES && s < issued; ++s) {
+        const uint32_t uses = (uint32_t)((issued - 1 - s) / STAGES);
+        const uint64_t t0 = global_ns();
+        while (!mbar_try_wait(&full_bar[s], uses & 1u) && global_ns() - t0 < kWaitLimitNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t id = idesc(p.bf16, p.b_mn, p.a_mn, NT, 128);
+      int stage = 0, in_chunk = 0;
+      uint32_t phase = 0, chunks = 0;
+      for (int it = begin; it < end; ++it) {
+        const int buf = (int)(chunks & 1u);
+        if (in_chunk == 0) {
+          if (!mbar_wait(&tempty_bar[buf], ((chunks >> 1) & 1u) ^ 1u, abort_flag, p.dev_err)) break;
+          tc_fence_after();
+        }
+        if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) break;
+        tc_fence_after();
+        const uint32_t a = smem_u32(smem + stage * STAGE), b = a + TILE;
+#pragma unroll
+        for (int s = 0; s < BK / 16; ++s)
+          mma_f16(tmem + (uint32_t)(buf * NT), desc(a, p.b_mn, s), desc(b, p.a_mn, s), id,
+                  (in_chunk | s) ? 1u : 0u);
+        tc_commit(&empty_bar[stage]);
+        if (++stage == STAGES) { stage = 0; phase ^= 1u; }
+        if (++in_chunk == p.chunk || it == end - 1) {
+          tc_commit(&tfull_bar[buf]);
+          ++chunks;
+          in_chunk = 0;
+        }
+      }
+      tc_commit(drain_bar);
+      const uint64_t t0 = global_ns();
+      while (!mbar_try_wait(drain_bar, 0) && global_ns() - t0 < kWaitLimitNs) {
+      }
+    }
+  } else {
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const int nchunks = (end - begin + p.chunk - 1) / p.chunk;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
+    for (int c = 0; c < nchunks; ++c) {
+      const int buf = c & 1;
+      if (!mbar_wait(&tfull_bar[buf], (uint32_t)(c >> 1) & 1u, abort_flag, p.dev_err)) break;
+      tc_fence_after();
+#pragma unroll
+      for (int q = 0; q < NT / 16; ++q) {
+        float v[16];
+        tmem_ld_32x32b_x16(lanes + (uint32_t)(buf * NT + q * 16), v);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) acc[q * 16 + j] = __fadd_rn(acc[q * 16 + j], v[j]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&tempty_bar[buf]);
+    }
+  }
+  // All MMAs of this CTA are done (drain) and all copies have landed.
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, COLS);
+  const int lane_col = (warp & 3) * 32 + lane;
+  if (warp >= 2) {
+#pragma unroll
+    for (int j = 0; j < NT; ++j) part[j * 128 + lane_col] = acc[j];
+  }
+  cluster_sync_all();
+  if (warp >= 2 && !*abort_flag) {
+    const int j1 = NT * (rank + 1) / ranks;
+    for (int j = NT * rank / ranks; j < j1 && row0 + j < p.M; ++j) {
+      float v[1] = {0.0f};
+      for (int r = 0; r < ranks; ++r)
+        v[0] = __fadd_rn(v[0], ld_cluster_f32(cluster_addr(part + j * 128 + lane_col, (uint32_t)r)));
+      epilogue<T, MODE, 1>(p.e, row0 + j, col0 + lane_col, v);
+    }
+  }
+  __syncwarp();
+  cluster_sync_all();   // no CTA leaves while another still reads its part
+}
+
 // ---------------------------------------------------------------- operand preparation
 // [rows, cols] (row stride ld) -> planes of BF16 / F16 with row stride ldp (a
 // multiple of 8): F32 is split, 16-bit types are copied.  The padding is outside
@@ -490,25 +666,80 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   return ORCA_OK;
 }
 
+template <typename T, int MODE, int NT>
+static orca_status launch_split(orca_ctx* ctx, const CUtensorMap& mp, const CUtensorMap& mq, const Params& p,
+                                int ranks) {
+  const auto kernel = split_kernel<T, MODE, NT>;
+  static std::atomic<bool> ready[64];
+  if (!ready[ctx->device & 63].load()) {
+    ORCA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem<NT>()));
+    ready[ctx->device & 63].store(true);
+  }
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  const int64_t blocks = cdiv(p.N, 128) * cdiv(p.M, NT) * ranks;
+  if (blocks > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
+  cfg.gridDim = dim3((unsigned)blocks);
+  cfg.blockDim = dim3(SPLIT_THREADS);
+  cfg.dynamicSmemBytes = split_smem<NT>();
+  cfg.stream = ctx->stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mp, mq, p, ranks));
+  count_launch(ctx);
+  return ORCA_OK;
+}
+
+// Which kernel, by an estimate of its time in clocks.  A pair step (256 x 256 x
+// 64 on two SMs) takes 512 clocks of the tensor pipe; a split step 2 * NT, or
+// its bytes at what an SM gets from L2 when all of them load (about 40 a clock).
+struct Plan {
+  int nt;       // 0: pair_kernel
+  int ranks;
+};
+static Plan choose(orca_ctx* ctx, const Params& p, int64_t steps, bool q_mn) {
+  const int64_t pair_waves = cdiv(cdiv(p.M, 256) * cdiv(p.N, 256), ctx->sm_count / 2);
+  double best = (double)pair_waves * ((double)steps * 512 + 3000) + 8000;
+  Plan plan{0, 1};
+  int nt = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
+  if (q_mn && nt < 64) nt = 64;
+  const int64_t tiles = cdiv(p.N, 128) * cdiv(p.M, nt);
+  const double step = std::max(2.0 * nt, (TILE + nt * 128) / 40.0);
+  for (int ranks = 1; ranks <= 8 && ranks <= steps; ranks *= 2) {
+    const double waves = (double)cdiv(tiles * ranks, ctx->sm_count);
+    const double t = waves * ((double)cdiv(steps, ranks) * step + 4000 + (ranks > 1 ? 2000 + 16 * nt : 0)) + 4000;
+    if (t < best) { best = t; plan = {nt, ranks}; }
+  }
+  return plan;
+}
+
 template <typename T, int MODE>
 static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, const Planes& b, Params& p) {
   const int planes = dtype == ORCA_F32 ? 3 : 1;
-  CUtensorMap ma, mb;
-  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : ROWS));
-  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
   const int64_t steps = cdiv(p.K, BK) * p.pairs;
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
+  const bool f32_out = dtype == ORCA_F32 || (MODE == DW && p.e.out_f32);
+  p.chunk = f32_out ? CHUNK : (int)steps;
+  const Plan plan = choose(ctx, p, steps, p.a_mn != 0);
+  CUtensorMap ma, mb;
+  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : (plan.nt ? plan.nt : ROWS)));
+  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
+  if constexpr (MODE != DW) {
+    if (plan.nt == 16) return launch_split<T, MODE, 16>(ctx, mb, ma, p, plan.ranks);
+    if (plan.nt == 32) return launch_split<T, MODE, 32>(ctx, mb, ma, p, plan.ranks);
+  }
+  if (plan.nt == 64) return launch_split<T, MODE, 64>(ctx, mb, ma, p, plan.ranks);
+  if (plan.nt == 128) return launch_split<T, MODE, 128>(ctx, mb, ma, p, plan.ranks);
   if constexpr (std::is_same<T, float>::value) {
-    p.chunk = CHUNK;
     return launch_pair<T, MODE, true>(ctx, ma, mb, p);
   } else {
     if constexpr (MODE == DW) {
-      if (p.e.out_f32) {
-        p.chunk = CHUNK;
-        return launch_pair<T, MODE, true>(ctx, ma, mb, p);
-      }
+      if (f32_out) return launch_pair<T, MODE, true>(ctx, ma, mb, p);
     }
-    p.chunk = (int)steps;
     return launch_pair<T, MODE, false>(ctx, ma, mb, p);
   }
 }
