@@ -64,34 +64,69 @@ __device__ __forceinline__ void store_row(T* p, int valid, bool vec, const float
 }
 
 // ---------------------------------------------------------------- activations
-// f(z) and f'(z) in f32.  ReLU is z > 0 ? z : 0, as the F32 path's.
+// f(z) and f'(z) in f32, off by about 2^-22 of |z|.  They run in epilogues and
+// in passes bound by HBM, so they are built from the fast exponential and
+// reciprocal and have no branches.  ReLU is z > 0 ? z : 0, as the F32 path's.
+//
+// Normal upper tail Q(|z|) = erfc(|z| / sqrt 2) / 2 by formula 7.1.26 of
+// Abramowitz and Stegun (|error| of erf <= 1.5e-7): a polynomial in
+// t = 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2.  *e = e^(-z^2 / 2).
+__device__ __forceinline__ float rcp(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+constexpr float LOG2_E = 1.44269504f;
+__device__ __forceinline__ float normal_tail(float z, float* e) {
+  const float x = fabsf(z);
+  const float t = rcp(fmaf(0.3275911f * 0.70710678f, x, 1.0f));
+  float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  q = fmaf(t, q, 0.5f * 1.421413741f);
+  q = fmaf(t, q, 0.5f * -0.284496736f);
+  q = fmaf(t, q, 0.5f * 0.254829592f);
+  *e = exp2_fast((-0.5f * LOG2_E) * x * x);
+  return q * t * *e;
+}
+// 1 / (1 + e^-x); 0 below about -88, where e^-x is infinite.
+__device__ __forceinline__ float sigmoid(float x) { return rcp(1.0f + exp2_fast(-LOG2_E * x)); }
+// 2 sqrt(2 / pi) (z + 0.044715 z^3): (1 + tanh(half of it)) / 2 is its sigmoid.
+__device__ __forceinline__ float tanh_arg(float z) {
+  return z * fmaf(0.0713548163f * z, z, 1.59576912f);
+}
+
 template <int ACT> __device__ __forceinline__ float act_value(float z) {
   if (ACT == ORCA_ACT_RELU) return z > 0.0f ? z : 0.0f;
-  if (ACT == ORCA_ACT_GELU) return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-  if (ACT == ORCA_ACT_GELU_TANH) {
-    const float u = 0.79788456080286536f * (z + 0.044715f * z * z * z);
-    return 0.5f * z * (1.0f + tanhf(u));
+  if (ACT == ORCA_ACT_GELU) {
+    float e;
+    const float q = normal_tail(z, &e);
+    return z * (z < 0.0f ? q : 1.0f - q);
   }
-  if (ACT == ORCA_ACT_SILU) return z / (1.0f + expf(-z));
+  if (ACT == ORCA_ACT_GELU_TANH) return z * sigmoid(tanh_arg(z));
+  if (ACT == ORCA_ACT_SILU) return z * sigmoid(z);
   return z;
 }
 template <int ACT> __device__ __forceinline__ float act_slope(float z) {
   if (ACT == ORCA_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
-  if (ACT == ORCA_ACT_GELU)
-    return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) +
-           z * (expf(-0.5f * z * z) * 0.39894228040143268f);
+  if (ACT == ORCA_ACT_GELU) {
+    float e;
+    const float q = normal_tail(z, &e);
+    return fmaf(z * 0.39894228f, e, z < 0.0f ? q : 1.0f - q);
+  }
   if (ACT == ORCA_ACT_GELU_TANH) {
-    // Beyond |z| = 10 tanh is +-1 in f32 and the second term 0; the bound
-    // keeps z * z finite there.
+    // Beyond |z| = 10 the sigmoid is 0 or 1 in f32 and the second term 0; the
+    // bound keeps z * z finite there.  A NaN stays one through z - z.
     const float y = fminf(fmaxf(z, -10.0f), 10.0f);
-    const float t = tanhf(0.79788456080286536f * (y + 0.044715f * y * y * y));
-    return 0.5f * (1.0f + t) +
-           0.5f * y * (1.0f - t * t) * (0.79788456080286536f * (1.0f + 0.134145f * y * y)) +
-           (z - z);   // NaN and infinities stay NaN
+    const float s = sigmoid(tanh_arg(y));
+    return fmaf(y * s * (1.0f - s), fmaf(0.2140644489f * y, y, 1.59576912f), s) + (z - z);
   }
   if (ACT == ORCA_ACT_SILU) {
-    const float g = 1.0f / (1.0f + expf(-z));
-    return g * (1.0f + z * (1.0f - g));
+    const float s = sigmoid(z);
+    return s * fmaf(z, 1.0f - s, 1.0f);
   }
   return 1.0f;
 }
@@ -152,9 +187,18 @@ __device__ __forceinline__ float ckpt_up(uint32_t e) {      // 2^(127 - E); 0 fo
 __device__ __forceinline__ float ckpt_down(uint32_t e) {    // 2^(E - 127); NaN for a marked group
   return e == E_NONFINITE ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
 }
-__device__ __forceinline__ int ckpt_code(float v, float up) {
-  const int q = __float2int_rn(v * up);
-  return up == 0.0f ? 0 : (q < -127 ? -127 : (q > 127 ? 127 : q));
+// The code in the low byte.  v * up is exact, and adding 1.5 * 2^23 rounds it to
+// the nearest whole number, ties to even, into the low mantissa bits: no
+// conversion instruction (those share a slow pipe with the exponentials).
+__device__ __forceinline__ uint32_t ckpt_code(float v, float up) {
+  const float q = fminf(fmaxf(v * up, -127.0f), 127.0f);
+  return __float_as_uint(q + 12582912.0f);
+}
+// Four codes as a word; none in a marked group.
+__device__ __forceinline__ uint32_t ckpt_word(const float* v, float up) {
+  const uint32_t a = __byte_perm(ckpt_code(v[0], up), ckpt_code(v[1], up), 0x0040);
+  const uint32_t b = __byte_perm(ckpt_code(v[2], up), ckpt_code(v[3], up), 0x0040);
+  return up == 0.0f ? 0u : __byte_perm(a, b, 0x5410);
 }
 
 // Codes the V values of one lane, 32 / V adjacent lanes sharing a group (all
@@ -184,10 +228,7 @@ __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_
     uint32_t w[(V + 3) / 4];
 #pragma unroll
     for (int i = 0; i < V / 4; ++i)
-      w[i] = (uint32_t)(ckpt_code(v[4 * i], up) & 255) |
-             (uint32_t)(ckpt_code(v[4 * i + 1], up) & 255) << 8 |
-             (uint32_t)(ckpt_code(v[4 * i + 2], up) & 255) << 16 |
-             (uint32_t)(ckpt_code(v[4 * i + 3], up) & 255) << 24;
+      w[i] = ckpt_word(v + 4 * i, up);
     if (V >= 16 && align >= 16) {
 #pragma unroll
       for (int i = 0; i < V / 16; ++i)
@@ -203,7 +244,7 @@ __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < valid) p[i] = (uint8_t)(ckpt_code(v[i], up) & 255);
+      if (i < valid) p[i] = up == 0.0f ? (uint8_t)0 : (uint8_t)ckpt_code(v[i], up);
   }
 }
 
@@ -307,6 +348,140 @@ __device__ __forceinline__ void epilogue(const Epilogue& e, int64_t row, int64_t
     for (int i = 0; i < V; ++i) v[i] += t[i];
   }
   store_row<T, V>((T*)e.out + at, valid, vec, v);
+}
+
+// ---------------------------------------------------------------- 32 x 32 blocks
+// A warp's 32 rows x 32 columns, a row per lane (as TMEM gives them), and
+// row-major memory: the block goes through the warp's 4 KB of shared memory so
+// that the 16-byte accesses of a warp cover whole rows of the block (64 or 128
+// bytes, full sectors) instead of one piece in each of 32 rows.  16-byte pieces
+// are placed at (piece ^ f(row)), free of bank conflicts both ways.
+constexpr int BLOCK_SMEM = 32 * 32 * 4;
+
+__device__ __forceinline__ uint4 lds_v4(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a));
+  return v;
+}
+__device__ __forceinline__ void sts_v4(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// P pieces of 16 bytes a row.
+template <int P> __device__ __forceinline__ uint32_t piece_at(uint32_t smem, int row, int piece) {
+  const int f = P == 8 ? row & 7 : (P == 4 ? (row >> 1) & 3 : (row >> 2) & 1);
+  return smem + (uint32_t)(row * P + (piece ^ f)) * 16;
+}
+// u: this lane's row.  Rows from `rows` on are not written.
+template <int P>
+__device__ __forceinline__ void block_store(uint8_t* p, int64_t stride, int rows, const uint4 (&u)[P],
+                                            uint32_t smem, int lane) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, lane, i), u[i]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int r = i * (32 / P) + lane / P;
+    const uint4 v = lds_v4(piece_at<P>(smem, r, lane % P));
+    if (r < rows) *reinterpret_cast<uint4*>(p + r * stride + (lane % P) * 16) = v;
+  }
+  __syncwarp();
+}
+template <int P>
+__device__ __forceinline__ void block_load(const uint8_t* p, int64_t stride, int rows, uint4 (&u)[P],
+                                           uint32_t smem, int lane) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    const int r = i * (32 / P) + lane / P;
+    u[i] = r < rows ? *reinterpret_cast<const uint4*>(p + r * stride + (lane % P) * 16) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, i * (32 / P) + lane / P, lane % P), u[i]);
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < P; ++i) u[i] = lds_v4(piece_at<P>(smem, lane, i));
+  __syncwarp();
+}
+template <typename T>
+__device__ __forceinline__ void block_store_f32(T* p, int64_t ld, int rows, const float (&v)[32],
+                                                uint32_t smem, int lane) {
+  constexpr int P = 2 * (int)sizeof(T);
+  union { uint4 q[P]; T e[32]; } u;
+#pragma unroll
+  for (int i = 0; i < 32; ++i) u.e[i] = from_f32<T>(v[i]);
+  block_store<P>(reinterpret_cast<uint8_t*>(p), ld * (int64_t)sizeof(T), rows, u.q, smem, lane);
+}
+template <typename T>
+__device__ __forceinline__ void block_load_f32(const T* p, int64_t ld, int rows, float (&v)[32],
+                                               uint32_t smem, int lane) {
+  constexpr int P = 2 * (int)sizeof(T);
+  union { uint4 q[P]; T e[32]; } u;
+  block_load<P>(reinterpret_cast<const uint8_t*>(p), ld * (int64_t)sizeof(T), rows, u.q, smem, lane);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) v[i] = to_f32(u.e[i]);
+}
+
+// The epilogue of one block: rows row0 + lane, columns col .. col + 32.  Blocks
+// that reach past the last column or whose memory is not 16-byte aligned take
+// the row-per-lane form.
+template <typename T, int MODE>
+__device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, int64_t col, float (&v)[32],
+                                               uint32_t smem, int lane) {
+  const bool packed = e.codes != nullptr;
+  if (!e.vec || col + 32 > e.cols || (packed && e.ckpt_align < 16)) {
+    epilogue<T, MODE, 32>(e, row0 + lane, col, v);
+    return;
+  }
+  if (row0 >= e.rows) return;
+  const int rows = e.rows - row0 < 32 ? (int)(e.rows - row0) : 32;
+  const int64_t at = row0 * e.cols + col;
+  if (MODE == DW) {
+    if (e.out_f32) block_store_f32<float>((float*)e.out + at, e.cols, rows, v, smem, lane);
+    else block_store_f32<T>((T*)e.out + at, e.cols, rows, v, smem, lane);
+    return;
+  }
+  float t[32];
+  if (MODE == FWD) {
+    if (e.bias) {
+      load_row<T, 32>((const T*)e.bias + col, 32, true, t);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] += t[i];
+    }
+    if (e.z) block_store_f32<T>((T*)e.z + at, e.cols, rows, v, smem, lane);
+    if (packed) {
+      uint32_t amax = 0;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
+        amax = a > amax ? a : amax;
+      }
+      const uint32_t x = ckpt_exponent(amax);
+      const float up = ckpt_up(x);
+      if (lane < rows) e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP] = (uint8_t)x;
+      union { uint4 q[2]; uint32_t w[8]; } u;
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        u.w[i] = ckpt_word(v + 4 * i, up);
+      block_store<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
+    }
+    apply_act<32>(e.act, v);
+  } else if (e.act != ORCA_ACT_NONE) {
+    if (packed) {
+      const float down = lane < rows ? ckpt_down(e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP]) : 0.0f;
+      union { uint4 q[2]; uint32_t w[8]; } u;
+      block_load<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) t[i] = (float)(int8_t)(u.w[i / 4] >> (8 * (i % 4))) * down;
+    } else {
+      block_load_f32<T>((const T*)e.x + at, e.cols, rows, t, smem, lane);
+    }
+    mul_slope<32>(e.act, t, v);
+  }
+  if (e.residual) {
+    block_load_f32<T>((const T*)e.residual + at, e.cols, rows, t, smem, lane);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] += t[i];
+  }
+  block_store_f32<T>((T*)e.out + at, e.cols, rows, v, smem, lane);
 }
 
 }  // namespace lin

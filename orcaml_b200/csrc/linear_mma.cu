@@ -33,7 +33,7 @@ constexpr uint32_t PAIR_A = 0x001102u, PAIR_B = 0x010120u;   // pair p: (x >> 4 
 constexpr int F32_PAIRS = 6;
 
 // Steps (of four MMAs) per accumulation chunk of an F32 result.
-constexpr int CHUNK = 8;
+constexpr int CHUNK = 16;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -41,12 +41,19 @@ constexpr int CHUNK = 8;
 //  MN-major: boxes of 64 mn x 64 k, k row at 128 bytes, 8-row groups of k 1024
 //    bytes apart (stride offset), boxes 8 KB apart (leading offset); step s
 //    starts 16 rows = 2 KB further.
-__device__ __forceinline__ uint64_t desc(uint32_t base, int mn_major, int step) {
-  const uint32_t addr = base + (mn_major ? step * 2048 : step * 32);
-  const uint32_t lbo = mn_major ? 8192 : 16;
-  return (uint64_t)((addr >> 4) & 0x3FFFu) | (uint64_t)(lbo >> 4) << 16 |
-         (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// The issuing thread has ~500 clocks per 64-deep step, so the descriptors are
+// kept as a low word (address and leading offset) that is advanced by adds and a
+// constant high word.
+__device__ __forceinline__ uint32_t desc_lo(uint32_t base, int mn_major) {
+  return ((base >> 4) & 0x3FFFu) | (uint32_t)((mn_major ? 8192 : 16) >> 4) << 16;
 }
+constexpr uint32_t DESC_HI = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint64_t desc(uint32_t lo) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"(lo), "r"(DESC_HI));
+  return d;
+}
+__device__ __forceinline__ uint32_t desc_step(int mn_major) { return (mn_major ? 2048u : 32u) >> 4; }
 
 // kind::f16 instruction descriptor: F32 accumulator, operand types (1 = BF16,
 // 0 = F16), orientations, N and M.
@@ -70,6 +77,25 @@ __device__ __forceinline__ void mma_f16_pair(uint32_t d, uint64_t a, uint64_t b,
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b),
       "r"(id), "r"(acc)
+      : "memory");
+}
+
+// One lane of the (converged) warp.  The MMA warp runs its loop with all lanes, so
+// that the compiler keeps descriptors and counters in uniform registers, which is
+// where the instructions take them from; only the issue itself is one lane's.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+
+// Arrive once on the mbarrier at this offset in both CTAs of the pair when the
+// MMAs issued so far have completed.
+__device__ __forceinline__ void commit_both(uint64_t* bar) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          smem_u32(bar)),
+      "h"((uint16_t)3)
       : "memory");
 }
 
@@ -129,7 +155,8 @@ constexpr int EPI_WARPS = 8;
 constexpr int PAIR_THREADS = 64 + 32 * EPI_WARPS;
 constexpr int PAIR_STAGES = 6;
 constexpr int PAIR_STAGE = 2 * TILE;                     // A and B, this CTA's halves
-constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + 1024 + 256;
+constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + EPI_WARPS * BLOCK_SMEM + 1024 + 256;
+static_assert(PAIR_SMEM <= 232448, "shared memory of one CTA");
 constexpr int ACC_COLS = 256;
 
 template <typename T, int MODE, bool CHUNKED>
@@ -139,7 +166,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PAIR_STAGES * PAIR_STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PAIR_STAGES * PAIR_STAGE + EPI_WARPS * BLOCK_SMEM);
   uint64_t* full_bar = bars;                              // (even) both CTAs' bytes
   uint64_t* empty_bar = bars + PAIR_STAGES;
   uint64_t* tfull_bar = bars + 2 * PAIR_STAGES;           // [2]
@@ -240,8 +267,10 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       }
     }
   } else if (warp == 1) {
-    if (even && lane == 0) {
+    if (even) {
       const uint32_t id = idesc(p.bf16, p.a_mn, p.b_mn, 256, 256);
+      const uint32_t a0 = desc_lo(smem_u32(smem), p.a_mn), b0 = desc_lo(smem_u32(smem) + TILE, p.b_mn);
+      const uint32_t a_step = desc_step(p.a_mn), b_step = desc_step(p.b_mn);
       int stage = 0;
       uint32_t phase = 0, chunks = 0;
       bool ok = true;
@@ -258,24 +287,28 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           }
           if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t a = smem_u32(smem + stage * PAIR_STAGE), b = a + TILE;
+          const uint32_t at = (uint32_t)(stage * (PAIR_STAGE >> 4));
           const uint32_t d = tmem + (uint32_t)(buf * ACC_COLS);
+          const bool last = in_chunk + 1 == p.chunk || it == steps - 1;
+          if (elect_one()) {
 #pragma unroll
-          for (int s = 0; s < BK / 16; ++s)
-            mma_f16_pair(d, desc(a, p.a_mn, s), desc(b, p.b_mn, s), id, (in_chunk | s) ? 1u : 0u);
-          tc_commit_pair(cluster_addr(&empty_bar[stage], 0));
-          tc_commit_pair(cluster_addr(&empty_bar[stage], 1));
+            for (int s = 0; s < BK / 16; ++s)
+              mma_f16_pair(d, desc(a0 + at + s * a_step), desc(b0 + at + s * b_step), id,
+                           (in_chunk | s) ? 1u : 0u);
+            commit_both(&empty_bar[stage]);
+            if (last) commit_both(&tfull_bar[buf]);
+          }
+          __syncwarp();
           if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
-          if (++in_chunk == p.chunk || it == steps - 1) {
-            tc_commit_pair(cluster_addr(&tfull_bar[buf], 0));
-            tc_commit_pair(cluster_addr(&tfull_bar[buf], 1));
+          ++in_chunk;
+          if (last) {
             ++chunks;
             in_chunk = 0;
           }
         }
       }
       if (!ok) raise_abort();
-      tc_commit_pair(cluster_addr(drain_bar, 0));
+      if (elect_one()) tc_commit_pair(cluster_addr(drain_bar, 0));
       const uint64_t t0 = global_ns();
       while (!mbar_try_wait(drain_bar, 0) && global_ns() - t0 < kWaitLimitNs) {
       }
@@ -286,12 +319,13 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t tempty[2] = {cluster_addr(&tempty_bar[0], 0), cluster_addr(&tempty_bar[1], 0)};
     const int nchunks = (steps + p.chunk - 1) / p.chunk;
+    const uint32_t block = smem_u32(smem + PAIR_STAGES * PAIR_STAGE + (warp - 2) * BLOCK_SMEM);
     uint32_t chunks = 0;
     bool ok = true;
     for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
       int64_t tm, tn;
       tile_at(tile, num_m, num_n, p.group_m, tm, tn);
-      const int64_t row = tm * 256 + (int64_t)rank * 128 + quarter * 32 + lane;
+      const int64_t row = tm * 256 + (int64_t)rank * 128 + quarter * 32;
       const int64_t col = tn * 256 + half * 128;
       if (CHUNKED) {
         float acc[128];
@@ -317,13 +351,16 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           ++chunks;
         }
         if (!ok) break;
-#pragma unroll
+        // One copy of the epilogue's code for the four blocks: the block's sums are
+        // selected, since registers have no index.
+#pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           if (col + q * 32 < p.N) {
             float v[32];
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = acc[q * 32 + j];
-            epilogue<T, MODE, 32>(p.e, row, col + q * 32, v);
+            for (int j = 0; j < 32; ++j)
+              v[j] = q & 2 ? (q & 1 ? acc[96 + j] : acc[64 + j]) : (q & 1 ? acc[32 + j] : acc[j]);
+            block_epilogue<T, MODE>(p.e, row, col + q * 32, v, block, lane);
           }
         }
       } else {
@@ -338,7 +375,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           if (col + q * 32 < p.N) {
             float v[32];
             tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
-            epilogue<T, MODE, 32>(p.e, row, col + q * 32, v);
+            block_epilogue<T, MODE>(p.e, row, col + q * 32, v, block, lane);
           }
         }
         tc_fence_before();
@@ -457,8 +494,10 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
       }
     }
   } else if (warp == 1) {
-    if (lane == 0) {
+    {
       const uint32_t id = idesc(p.bf16, p.b_mn, p.a_mn, NT, 128);
+      const uint32_t a0 = desc_lo(smem_u32(smem), p.b_mn), b0 = desc_lo(smem_u32(smem) + TILE, p.a_mn);
+      const uint32_t a_step = desc_step(p.b_mn), b_step = desc_step(p.a_mn);
       int stage = 0, in_chunk = 0;
       uint32_t phase = 0, chunks = 0;
       for (int it = begin; it < end; ++it) {
@@ -469,20 +508,25 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
         }
         if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) break;
         tc_fence_after();
-        const uint32_t a = smem_u32(smem + stage * STAGE), b = a + TILE;
+        const uint32_t at = (uint32_t)(stage * (STAGE >> 4));
+        const bool last = in_chunk + 1 == p.chunk || it == end - 1;
+        if (elect_one()) {
 #pragma unroll
-        for (int s = 0; s < BK / 16; ++s)
-          mma_f16(tmem + (uint32_t)(buf * NT), desc(a, p.b_mn, s), desc(b, p.a_mn, s), id,
-                  (in_chunk | s) ? 1u : 0u);
-        tc_commit(&empty_bar[stage]);
+          for (int s = 0; s < BK / 16; ++s)
+            mma_f16(tmem + (uint32_t)(buf * NT), desc(a0 + at + s * a_step), desc(b0 + at + s * b_step), id,
+                    (in_chunk | s) ? 1u : 0u);
+          tc_commit(&empty_bar[stage]);
+          if (last) tc_commit(&tfull_bar[buf]);
+        }
+        __syncwarp();
         if (++stage == STAGES) { stage = 0; phase ^= 1u; }
-        if (++in_chunk == p.chunk || it == end - 1) {
-          tc_commit(&tfull_bar[buf]);
+        ++in_chunk;
+        if (last) {
           ++chunks;
           in_chunk = 0;
         }
       }
-      tc_commit(drain_bar);
+      if (elect_one()) tc_commit(drain_bar);
       const uint64_t t0 = global_ns();
       while (!mbar_try_wait(drain_bar, 0) && global_ns() - t0 < kWaitLimitNs) {
       }
