@@ -99,70 +99,91 @@ tile_kernel(int64_t M, int64_t N, int64_t K, Operand A, Operand B, Epilogue e) {
 }
 
 // ---------------------------------------------------------------- column sums
-// db: rows [r0, r1) of a block summed per column in F32, 8 columns a thread and
-// 8 row lanes joined in order; row blocks joined in order by sum_parts, so the
-// result does not depend on timing.
-constexpr int CS_COLS = 256;
+// db: 128 columns per cluster of up to 8 CTAs that take a part of the rows each;
+// 16 lanes of 8 columns by 16 rows a CTA, F32 sums per lane, joined over the rows'
+// lanes and then, through the cluster's shared memory, over the CTAs, always in
+// the same order.  One pass over dy, bound by HBM: 8 rows in flight per lane.
+constexpr int CS_COLS = 128, CS_ROWS = 16, CS_RANKS = 8;
 
-template <typename T>
+template <typename T, typename G>
 __global__ void __launch_bounds__(256)
-colsum_kernel(const T* __restrict__ x, int64_t m, int64_t n, int64_t rows, int vec,
-              float* __restrict__ part) {
-  __shared__ float s[8][CS_COLS + 8];
-  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
-  const int64_t col = (int64_t)blockIdx.x * CS_COLS + tx * 8;
+colsum_kernel(const T* __restrict__ x, int64_t m, int64_t n, int ranks, int64_t rows, int vec,
+              G* __restrict__ out) {
+  __shared__ float s[CS_ROWS][CS_COLS + 8];
+  __shared__ float part[CS_COLS];
+  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const uint32_t rank = cluster_ctarank();
+  const int64_t col0 = (int64_t)(blockIdx.x / ranks) * CS_COLS, col = col0 + tx * 8;
   const int valid = col >= n ? 0 : (n - col < 8 ? (int)(n - col) : 8);
-  const int64_t r0 = (int64_t)blockIdx.y * rows, r1 = std::min<int64_t>(m, r0 + rows);
+  const bool whole = vec && valid == 8;
+  const int64_t r1 = std::min<int64_t>(m, (rank + 1) * rows);
   float acc[8] = {};
-  if (valid > 0)
-#pragma unroll 4
-    for (int64_t r = r0 + ty; r < r1; r += 8) {
+  if (valid > 0) {
+    int64_t r = rank * rows + ty;
+    for (; r + 7 * CS_ROWS < r1; r += 8 * CS_ROWS) {
+      float v[8][8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) load_row<T, 8>(x + (r + u * CS_ROWS) * n + col, valid, whole, v[u]);
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) acc[i] += v[u][i];
+    }
+    for (; r < r1; r += CS_ROWS) {
       float v[8];
-      load_row<T, 8>(x + r * n + col, valid, vec && valid == 8, v);
+      load_row<T, 8>(x + r * n + col, valid, whole, v);
 #pragma unroll
       for (int i = 0; i < 8; ++i) acc[i] += v[i];
     }
+  }
 #pragma unroll
   for (int i = 0; i < 8; ++i) s[ty][tx * 8 + i] = acc[i];
   __syncthreads();
-  const int64_t c = (int64_t)blockIdx.x * CS_COLS + threadIdx.x;
-  if (c >= n) return;
-  float t = 0.0f;
+  if (threadIdx.x < CS_COLS) {
+    float t = 0.0f;
 #pragma unroll
-  for (int y = 0; y < 8; ++y) t += s[y][threadIdx.x];
-  part[(int64_t)blockIdx.y * n + c] = t;
+    for (int y = 0; y < CS_ROWS; ++y) t += s[y][threadIdx.x];
+    part[threadIdx.x] = t;
+  }
+  cluster_sync_all();
+  if (rank == 0 && threadIdx.x < CS_COLS && col0 + threadIdx.x < n) {
+    float t = 0.0f;
+    for (uint32_t r = 0; r < (uint32_t)ranks; ++r) {
+      float v;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(part + threadIdx.x, r)) : "memory");
+      t += v;
+    }
+    out[col0 + threadIdx.x] = from_f32<G>(t);
+  }
+  cluster_sync_all();   // no CTA leaves while its part may still be read
 }
 
-template <typename G>
-__global__ void __launch_bounds__(256)
-sum_parts_kernel(const float* __restrict__ part, int64_t n, int parts, G* __restrict__ out) {
-  const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (c >= n) return;
-  float t = 0.0f;
-  for (int p = 0; p < parts; ++p) t += part[(int64_t)p * n + c];
-  out[c] = from_f32<G>(t);
+template <typename T, typename G>
+static orca_status colsum_launch(orca_ctx* ctx, const T* x, int64_t m, int64_t n, G* out) {
+  if (n <= 0) return ORCA_OK;
+  const int ranks = m <= 64 ? 1 : CS_RANKS;
+  const int64_t rows = std::max<int64_t>(1, cdiv(m, ranks));
+  const int vec = byte_alignment(x, n * (int64_t)sizeof(T)) == 16;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ranks;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.blockDim = dim3(256);
+  cfg.stream = ctx->stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3((unsigned)(cdiv(n, CS_COLS) * ranks));
+  ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, colsum_kernel<T, G>, x, m, n, ranks, rows, vec, out));
+  count_launch(ctx);
+  return ORCA_OK;
 }
 
 template <typename T>
 static orca_status colsum(orca_ctx* ctx, const T* x, int64_t m, int64_t n, const orca_span* out) {
-  if (n <= 0) return ORCA_OK;
-  const int64_t bx = cdiv(n, CS_COLS);
-  int64_t parts = std::max<int64_t>(1, std::min<int64_t>(cdiv(m, 64), (int64_t)ctx->sm_count * 4 / bx));
-  const int64_t rows = std::max<int64_t>(1, cdiv(m, parts));
-  parts = std::max<int64_t>(1, cdiv(m, rows));
-  Scratch part(ctx);
-  ORCA_TRY(part.get((size_t)(parts * n) * 4));
-  const bool vec = byte_alignment(x, n * (int64_t)sizeof(T)) == 16;
-  colsum_kernel<T><<<dim3((unsigned)bx, (unsigned)parts), 256, 0, ctx->stream>>>(
-      x, m, n, rows, vec ? 1 : 0, (float*)part.p);
-  const unsigned g = (unsigned)cdiv(n, 256);
-  if (out->dtype == ORCA_F32)
-    sum_parts_kernel<<<g, 256, 0, ctx->stream>>>((const float*)part.p, n, (int)parts, (float*)out->data);
-  else
-    sum_parts_kernel<<<g, 256, 0, ctx->stream>>>((const float*)part.p, n, (int)parts, (T*)out->data);
-  count_launch(ctx, 2);
-  ORCA_CUDA_TRY(cudaGetLastError());
-  return ORCA_OK;
+  if (out->dtype == ORCA_F32) return colsum_launch(ctx, x, m, n, (float*)out->data);
+  return colsum_launch(ctx, x, m, n, (T*)out->data);
 }
 
 // ---------------------------------------------------------------- products
@@ -173,7 +194,7 @@ static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   e.rows = M;
   e.cols = N;
   int al = 16;
-  for (const void* p : {(const void*)e.out, e.residual, (const void*)e.z, e.x})
+  for (const void* p : {(const void*)e.out, e.residual, (const void*)e.z, e.x, (const void*)e.a})
     if (p) al = std::min(al, byte_alignment(p, N * (int64_t)sizeof(T)));
   if (e.bias) al = std::min(al, byte_alignment(e.bias, 0));
   e.vec = al == 16;
@@ -205,6 +226,15 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
                             int64_t n, int act, const orca_span* dx, const orca_span* dw,
                             const orca_span* db) {
   const bool packed = x && x->dtype == ORCA_U8;
+  // dW's operand a = act(x): x itself, or a matrix that the epilogue of the dX
+  // product writes on the way (it reads x for the slope anyway), or a pass of its own.
+  Scratch act_x(ctx);
+  const void* a_operand = x ? x->data : nullptr;
+  if (dw && m * k > 0 && (packed || act != ORCA_ACT_NONE)) {
+    ORCA_TRY(act_x.get((size_t)(m * k) * sizeof(T)));
+    a_operand = act_x.p;
+  }
+  const bool emit = act_x.p && dx && n > 0;
   if (dx) {
     Operand a, b;
     a.p = dy->data; a.ld = n;
@@ -213,7 +243,7 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
     e.act = act;
     e.out = dx->data;
     if (residual) e.residual = residual->data;
-    if (act != ORCA_ACT_NONE) {
+    if (act != ORCA_ACT_NONE || emit) {
       if (packed) {
         e.codes = (uint8_t*)x->data;
         e.exps = e.codes + ckpt_exps_at(m, k);
@@ -221,22 +251,18 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
         e.x = x->data;
       }
     }
+    if (emit) e.a = act_x.p;
     ORCA_TRY((product<T, DX>(ctx, m, k, n, a, b, e)));
   }
   if (dw) {
-    Scratch act_x(ctx);
-    Operand a, b;
-    a.ld = k; a.mn_major = 1;
-    if (!packed && act == ORCA_ACT_NONE) {
-      a.p = x ? x->data : nullptr;
-    } else if (m * k > 0) {
-      ORCA_TRY(act_x.get((size_t)(m * k) * sizeof(T)));
+    if (act_x.p && !emit) {
       if (packed)
-        ORCA_TRY(ckpt8_unpack_launch(ctx, (const uint8_t*)x->data, m, k, act, act_x.p, w ? w->dtype : dy->dtype));
+        ORCA_TRY(ckpt8_unpack_launch(ctx, (const uint8_t*)x->data, m, k, act, act_x.p, dy->dtype));
       else
         ORCA_TRY(act_launch(ctx, x->data, x->dtype, m * k, act, act_x.p));
-      a.p = act_x.p;
     }
+    Operand a, b;
+    a.p = a_operand; a.ld = k; a.mn_major = 1;
     b.p = dy->data; b.ld = n; b.mn_major = 1;
     Epilogue e;
     e.out = dw->data;

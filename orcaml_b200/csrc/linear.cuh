@@ -307,6 +307,7 @@ struct Epilogue {
   uint8_t* codes = nullptr;           // FWD: kept in 8 bits; DX: x in 8 bits
   uint8_t* exps = nullptr;
   const void* x = nullptr;            // DX: x in T (with an activation only)
+  void* a = nullptr;                  // DX: act(x) in T, the operand of dW, is written here
 };
 
 // V consecutive columns of one row per thread, 32 / V adjacent lanes on
@@ -336,10 +337,14 @@ __device__ __forceinline__ void epilogue(const Epilogue& e, int64_t row, int64_t
     apply_act<V>(e.act, v);
   } else {
     if (valid <= 0) return;
-    if (e.act != ORCA_ACT_NONE) {
+    if (e.codes || e.x) {
       if (e.codes) ckpt_load<V>(e.codes, e.exps, row, e.cols, col, valid, e.ckpt_align, t);
       else load_row<T, V>((const T*)e.x + at, valid, vec, t);
       mul_slope<V>(e.act, t, v);
+      if (e.a) {
+        apply_act<V>(e.act, t);
+        store_row<T, V>((T*)e.a + at, valid, vec, t);
+      }
     }
   }
   if (e.residual) {
@@ -464,7 +469,7 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       block_store<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
     }
     apply_act<32>(e.act, v);
-  } else if (e.act != ORCA_ACT_NONE) {
+  } else if (packed || e.x) {
     if (packed) {
       const float down = lane < rows ? ckpt_down(e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP]) : 0.0f;
       union { uint4 q[2]; uint32_t w[8]; } u;
@@ -475,6 +480,10 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       block_load_f32<T>((const T*)e.x + at, e.cols, rows, t, smem, lane);
     }
     mul_slope<32>(e.act, t, v);
+    if (e.a) {
+      apply_act<32>(e.act, t);
+      block_store_f32<T>((T*)e.a + at, e.cols, rows, t, smem, lane);
+    }
   }
   if (e.residual) {
     block_load_f32<T>((const T*)e.residual + at, e.cols, rows, t, smem, lane);

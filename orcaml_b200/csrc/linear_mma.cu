@@ -32,8 +32,16 @@ constexpr int TILE = ROWS * BK * 2;          // 16 KB
 constexpr uint32_t PAIR_A = 0x001102u, PAIR_B = 0x010120u;   // pair p: (x >> 4 * p) & 15
 constexpr int F32_PAIRS = 6;
 
-// Steps (of four MMAs) per accumulation chunk of an F32 result.
-constexpr int CHUNK = 16;
+// What sharing a tile among clusters costs, in steps of the whole grid.
+constexpr int SHARE_STEPS = 24;
+
+// Steps (of four MMAs) per accumulation chunk of an F32 result.  The tensor core
+// adds with a few bits less than F32; a chain of L MMAs over random data is off by
+// about 9e-10 * L^1.5 of the result's norm.  F32 operands: 64 MMAs, 5e-7, what an
+// F32 chain of FMAs gives.  F32 gradients of 16-bit operands: 256 MMAs, 4e-6
+// against the operands' own 2^-9; emptying the accumulator every 32 MMAs
+// instead cost 13 % of the product's time.
+constexpr int CHUNK_F32 = 16, CHUNK_DW = 64;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -99,6 +107,22 @@ __device__ __forceinline__ void commit_both(uint64_t* bar) {
       : "memory");
 }
 
+// 32 lanes x 32 columns from registers, the layout of tmem_ld_32x32b_x32.
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const float* v) {
+  uint32_t r[32];
+#pragma unroll
+  for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::"r"(r[0]),
+      "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
+      "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]),
+      "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31]), "r"(taddr)
+      : "memory");
+}
+
 struct Params {
   int64_t M, N, K;
   int a_mn, b_mn;
@@ -106,6 +130,10 @@ struct Params {
   int pairs;               // plane pairs: 1, or F32_PAIRS
   int chunk;               // steps per accumulation chunk
   int group_m;             // tile rows per raster group
+  int64_t full;            // pair_kernel: tiles [0, full) are whole, one cluster each
+  int tail;                // ... the rest is shared by the first `tail` clusters (0: no rest)
+  float* parts;            // ... their partial sums and arrival counters
+  int* arrived;
   int* dev_err;
   Epilogue e;
 };
@@ -142,14 +170,51 @@ __device__ __forceinline__ void tile_at(int64_t tile, int64_t num_m, int64_t num
   tn = r / gm;
 }
 
+// The pieces of work of one cluster of pair_kernel, in order: whole tiles, then its
+// equal share of the steps of the tiles that do not fill a last round, which
+// may end one tile, cover some and begin another.
+struct Work {
+  int64_t cluster, nclusters, full, next, pos, end;
+  int steps;
+  __device__ Work(const Params& p, int64_t c, int64_t n, int64_t tiles, int steps_)
+      : cluster(c), nclusters(n), full(p.full), next(c), pos(0), end(0), steps(steps_) {
+    if (p.tail && c < p.tail) {
+      const int64_t total = (tiles - full) * steps;
+      pos = total * c / p.tail;
+      end = total * (c + 1) / p.tail;
+    }
+  }
+  __device__ bool get(int64_t& tile, int& begin, int& stop) {
+    if (next < full) {
+      tile = next;
+      next += nclusters;
+      begin = 0;
+      stop = steps;
+      return true;
+    }
+    if (pos >= end) return false;
+    const int64_t t = pos / steps;
+    begin = (int)(pos - t * steps);
+    stop = end - pos < steps - begin ? begin + (int)(end - pos) : steps;
+    tile = full + t;
+    pos += stop - begin;
+    return true;
+  }
+};
+
 // ---------------------------------------------------------------- CTA pairs
+// Tiles beyond whole rounds of the resident clusters are cut along the sum, so
+// that all clusters finish together (4096 x 4096 outputs are 3.46 rounds of 74
+// clusters).  A cluster leaves the sums of a piece in memory and counts itself in;
+// the last to arrive at a tile adds the pieces in their order -- the same bits
+// whoever is last -- and finishes it.  Nobody waits for anybody.  Each epilogue
+// warp does this for its own 32 x 128 part.
+//
 // Roles: warp 0 loads, warp 1 (of the even CTA) issues the MMAs, warps 2-9
 // drain one of two 256-column accumulators while the MMAs fill the other.  The
 // even CTA's full barrier counts both CTAs' bytes; the MMA's commits free the
-// stage and publish the accumulator in both.  CHUNKED (F32 results): the
-// accumulator is emptied every `chunk` steps into F32 registers, because the
-// tensor core adds with a few bits less than F32 and one long chain would lose
-// them.  Every wait is bounded; a role that gives up raises the abort flag of
+// stage and publish the accumulator in both.  For F32 results the accumulator
+// is emptied every `chunk` steps into F32 registers.  Every wait is bounded; a role that gives up raises the abort flag of
 // both CTAs, and both pass the same two cluster barriers in every case.
 constexpr int EPI_WARPS = 8;
 constexpr int PAIR_THREADS = 64 + 32 * EPI_WARPS;
@@ -158,8 +223,10 @@ constexpr int PAIR_STAGE = 2 * TILE;                     // A and B, this CTA's 
 constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + EPI_WARPS * BLOCK_SMEM + 1024 + 256;
 static_assert(PAIR_SMEM <= 232448, "shared memory of one CTA");
 constexpr int ACC_COLS = 256;
+constexpr int64_t PART_FLOATS = 256 * 256;               // one piece: two CTAs of 128 x 256
+constexpr int ARRIVALS = 2 * EPI_WARPS;                  // counters of a tile
 
-template <typename T, int MODE, bool CHUNKED>
+template <typename T, int MODE>
 __global__ void __launch_bounds__(PAIR_THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ Params p) {
@@ -221,13 +288,16 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       for (int s = 0; s < PAIR_STAGES; ++s) issued[s] = -1;
       uint64_t last_issue = 0;
       bool ok = true;
-      for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
+      Work work(p, cluster, nclusters, tiles, steps);
+      int64_t tile;
+      int begin, stop;
+      while (ok && work.get(tile, begin, stop)) {
         int64_t tm, tn;
         tile_at(tile, num_m, num_n, p.group_m, tm, tn);
         const int64_t row = tm * 256 + (int64_t)rank * 128, col = tn * 256 + (int64_t)rank * 128;
-        int pair = 0;
-        int64_t k0 = 0;
-        for (int it = 0; it < steps; ++it) {
+        int pair = begin % p.pairs;
+        int64_t k0 = (int64_t)(begin / p.pairs) * BK;
+        for (int it = begin; it < stop; ++it) {
           const int pa = p.pairs == 1 ? 0 : (int)(PAIR_A >> (4 * pair)) & 15;
           const int pb = p.pairs == 1 ? 0 : (int)(PAIR_B >> (4 * pair)) & 15;
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.dev_err)) {
@@ -274,9 +344,12 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       int stage = 0;
       uint32_t phase = 0, chunks = 0;
       bool ok = true;
-      for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
+      Work work(p, cluster, nclusters, tiles, steps);
+      int64_t tile;
+      int begin, stop;
+      while (ok && work.get(tile, begin, stop)) {
         int in_chunk = 0;
-        for (int it = 0; it < steps; ++it) {
+        for (int it = begin; it < stop; ++it) {
           const int buf = (int)(chunks & 1u);
           if (in_chunk == 0) {
             if (!mbar_wait(&tempty_bar[buf], ((chunks >> 1) & 1u) ^ 1u, abort_flag, p.dev_err)) {
@@ -289,7 +362,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           tc_fence_after();
           const uint32_t at = (uint32_t)(stage * (PAIR_STAGE >> 4));
           const uint32_t d = tmem + (uint32_t)(buf * ACC_COLS);
-          const bool last = in_chunk + 1 == p.chunk || it == steps - 1;
+          const bool last = in_chunk + 1 == p.chunk || it == stop - 1;
           if (elect_one()) {
 #pragma unroll
             for (int s = 0; s < BK / 16; ++s)
@@ -318,26 +391,40 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     const int quarter = warp & 3, half = (warp - 2) / 4;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
     const uint32_t tempty[2] = {cluster_addr(&tempty_bar[0], 0), cluster_addr(&tempty_bar[1], 0)};
-    const int nchunks = (steps + p.chunk - 1) / p.chunk;
     const uint32_t block = smem_u32(smem + PAIR_STAGES * PAIR_STAGE + (warp - 2) * BLOCK_SMEM);
     uint32_t chunks = 0;
     bool ok = true;
-    for (int64_t tile = cluster; tile < tiles && ok; tile += nclusters) {
+    Work work(p, cluster, nclusters, tiles, steps);
+    int64_t tile;
+    int begin, stop;
+    while (ok && work.get(tile, begin, stop)) {
       int64_t tm, tn;
       tile_at(tile, num_m, num_n, p.group_m, tm, tn);
       const int64_t row = tm * 256 + (int64_t)rank * 128 + quarter * 32;
       const int64_t col = tn * 256 + half * 128;
-      if (CHUNKED) {
+      const bool piece = stop - begin < steps;
+      // This warp's part of a piece: blocks of 32 columns, column by column.
+      const int64_t my_part = (int64_t)((rank * EPI_WARPS + warp - 2) * 4) * 1024 + lane;
+      float* mine = p.parts + (cluster * 2 + (begin == 0)) * PART_FLOATS + my_part;
+      const int nchunks = (stop - begin + p.chunk - 1) / p.chunk;
+      auto release = [&](int buf) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_remote(tempty[buf]);
+      };
+      int buf = (int)(chunks & 1u);
+      ok = mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64);
+      tc_fence_after();
+      ++chunks;
+      if (ok && nchunks > 1) {
+        // The sums go back to the last chunk's accumulator, where the epilogue finds
+        // them block by block as it finds those of a single chunk: holding 128 sums
+        // in registers through the epilogue spilled them, and with this much
+        // shared memory in use the spills went to L2.
         float acc[128];
 #pragma unroll
         for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
-        for (int c = 0; c < nchunks; ++c) {
-          const int buf = (int)(chunks & 1u);
-          if (!mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64)) {
-            ok = false;
-            break;
-          }
-          tc_fence_after();
+        for (int c = 0;; ++c) {
 #pragma unroll
           for (int q = 0; q < 8; ++q) {
             float v[16];
@@ -345,44 +432,65 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
             for (int j = 0; j < 16; ++j) acc[q * 16 + j] = __fadd_rn(acc[q * 16 + j], v[j]);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_remote(tempty[buf]);
+          if (c == nchunks - 1) break;
+          release(buf);
+          buf = (int)(chunks & 1u);
+          ok = mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64);
+          if (!ok) break;
+          tc_fence_after();
           ++chunks;
         }
-        if (!ok) break;
-        // One copy of the epilogue's code for the four blocks: the block's sums are
-        // selected, since registers have no index.
-#pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
-          if (col + q * 32 < p.N) {
-            float v[32];
+        if (ok) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j)
-              v[j] = q & 2 ? (q & 1 ? acc[96 + j] : acc[64 + j]) : (q & 1 ? acc[32 + j] : acc[j]);
-            block_epilogue<T, MODE>(p.e, row, col + q * 32, v, block, lane);
-          }
+          for (int q = 0; q < 4; ++q) tmem_st_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), acc + q * 32);
+          asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
-      } else {
-        const int buf = (int)(chunks & 1u);
-        if (!mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
+      }
+      if (!ok) break;
+      int64_t first = 0, count = 0;
+      if (piece) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
-          if (col + q * 32 < p.N) {
-            float v[32];
-            tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
-            block_epilogue<T, MODE>(p.e, row, col + q * 32, v, block, lane);
-          }
+          float v[32];
+          tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
+#pragma unroll
+          for (int j = 0; j < 32; ++j) __stcg(mine + (q * 32 + j) * 32, v[j]);
         }
-        tc_fence_before();
+        release(buf);
+        // Clusters first .. first + count - 1 share this tile.
+        const int64_t t = tile - p.full, total = (tiles - p.full) * steps;
+        first = t * steps * p.tail / total;
+        while (total * (first + 1) / p.tail <= t * steps) ++first;
+        while (total * first / p.tail > t * steps) --first;
+        int64_t lastc = first;
+        while (total * (lastc + 1) / p.tail < (t + 1) * steps) ++lastc;
+        count = lastc - first + 1;
+        __threadfence();
         __syncwarp();
-        if (lane == 0) mbar_arrive_remote(tempty[buf]);
-        ++chunks;
+        int before = 0;
+        if (lane == 0) before = atomicAdd(p.arrived + t * ARRIVALS + rank * EPI_WARPS + warp - 2, 1);
+        before = __shfl_sync(0xffffffffu, before, 0);
+        if (before != (int)count - 1) continue;
+        __threadfence();
       }
+#pragma unroll 1
+      for (int q = 0; q < 4; ++q) {
+        if (col + q * 32 >= p.N) break;
+        float v[32];
+        if (piece) {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          for (int64_t c = 0; c < count; ++c) {
+            const float* part = p.parts + ((first + c) * 2 + (c == 0)) * PART_FLOATS + my_part;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], __ldcg(part + (q * 32 + j) * 32));
+          }
+        } else {
+          tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
+        }
+        block_epilogue<T, MODE>(p.e, row, col + q * 32, v, block, lane);
+      }
+      if (!piece) release(buf);
     }
     if (!ok) raise_abort();
   }
@@ -679,9 +787,9 @@ static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int b
 }
 
 // ---------------------------------------------------------------- launches
-template <typename T, int MODE, bool CHUNKED>
-static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, const Params& p) {
-  const auto kernel = pair_kernel<T, MODE, CHUNKED>;
+template <typename T, int MODE>
+static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, Params p) {
+  const auto kernel = pair_kernel<T, MODE>;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -703,8 +811,27 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
     if (n < 1) return fail(ORCA_CUDA_ERROR, "no cluster of two CTAs fits on the device");
     fit.store(n);
   }
-  const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256);
-  cfg.gridDim = dim3((unsigned)(2 * std::min<int64_t>(tiles, fit.load())));
+  const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256), n = fit.load();
+  const int64_t steps = cdiv(p.K, BK) * p.pairs, rest = tiles % n;
+  // Sharing the last tiles saves the part of a round that would be idle and costs
+  // a pass over the pieces, about SHARE_STEPS steps.  At most 4 clusters a tile:
+  // its last one reads all their pieces.
+  const int64_t tail = std::min(n, rest * 4);
+  p.full = tiles;
+  p.tail = 0;
+  p.parts = nullptr;
+  p.arrived = nullptr;
+  Scratch scratch(ctx);
+  if (rest && steps - cdiv(rest * steps, tail) > SHARE_STEPS) {
+    p.full = tiles - rest;
+    p.tail = (int)tail;
+    const size_t parts = (size_t)(tail * 2 * PART_FLOATS) * 4, counters = (size_t)(rest * ARRIVALS) * 4;
+    ORCA_TRY(scratch.get(parts + counters));
+    p.parts = (float*)scratch.p;
+    p.arrived = (int*)((uint8_t*)scratch.p + parts);
+    ORCA_CUDA_TRY(cudaMemsetAsync(p.arrived, 0, counters, ctx->stream));
+  }
+  cfg.gridDim = dim3((unsigned)(2 * (p.tail ? n : std::min(tiles, n))));
   ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, ma, mb, p));
   count_launch(ctx);
   return ORCA_OK;
@@ -746,8 +873,10 @@ struct Plan {
   int ranks;
 };
 static Plan choose(orca_ctx* ctx, const Params& p, int64_t steps, bool q_mn) {
-  const int64_t pair_waves = cdiv(cdiv(p.M, 256) * cdiv(p.N, 256), ctx->sm_count / 2);
-  double best = (double)pair_waves * ((double)steps * 512 + 3000) + 8000;
+  const int64_t pair_tiles = cdiv(p.M, 256) * cdiv(p.N, 256), clusters = ctx->sm_count / 2;
+  const int64_t rest = pair_tiles % clusters;
+  const int64_t last = rest ? std::min(steps, cdiv(rest * steps, std::min(clusters, rest * 4)) + SHARE_STEPS) : 0;
+  double best = (double)(pair_tiles / clusters * steps + last) * 512 + 8000;
   Plan plan{0, 1};
   int nt = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
   if (q_mn && nt < 64) nt = 64;
@@ -766,8 +895,7 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   const int planes = dtype == ORCA_F32 ? 3 : 1;
   const int64_t steps = cdiv(p.K, BK) * p.pairs;
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
-  const bool f32_out = dtype == ORCA_F32 || (MODE == DW && p.e.out_f32);
-  p.chunk = f32_out ? CHUNK : (int)steps;
+  p.chunk = dtype == ORCA_F32 ? CHUNK_F32 : (MODE == DW && p.e.out_f32 ? CHUNK_DW : (int)steps);
   const Plan plan = choose(ctx, p, steps, p.a_mn != 0);
   CUtensorMap ma, mb;
   ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : (plan.nt ? plan.nt : ROWS)));
@@ -778,14 +906,7 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   }
   if (plan.nt == 64) return launch_split<T, MODE, 64>(ctx, mb, ma, p, plan.ranks);
   if (plan.nt == 128) return launch_split<T, MODE, 128>(ctx, mb, ma, p, plan.ranks);
-  if constexpr (std::is_same<T, float>::value) {
-    return launch_pair<T, MODE, true>(ctx, ma, mb, p);
-  } else {
-    if constexpr (MODE == DW) {
-      if (f32_out) return launch_pair<T, MODE, true>(ctx, ma, mb, p);
-    }
-    return launch_pair<T, MODE, false>(ctx, ma, mb, p);
-  }
+  return launch_pair<T, MODE>(ctx, ma, mb, p);
 }
 
 }  // namespace lin
@@ -803,7 +924,11 @@ orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, in
   p.b_mn = B.mn_major;
   p.bf16 = dtype != ORCA_F16;
   p.pairs = dtype == ORCA_F32 ? F32_PAIRS : 1;
-  p.group_m = 8;
+  // Raster: 8 tile rows by 9 columns are about what runs at once.  Where all of A
+  // stays in L2 (48 MB of 126), all its rows form one group and B is read once
+  // (4096 x 4096 x 16384: 404 us against 416).
+  const int64_t a_bytes = M * K * 2 * (dtype == ORCA_F32 ? 3 : 1);
+  p.group_m = a_bytes <= (int64_t)48 << 20 ? (int)cdiv(M, 256) : 8;
   p.dev_err = ctx->dev_err;
   p.e = e;
 #define ORCA_MODE(MODE)                                                            \
