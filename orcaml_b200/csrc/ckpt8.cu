@@ -15,9 +15,87 @@ namespace lin {
 
 constexpr int THREADS = 256;
 
-// A block covers `lanes_x` lanes of V columns and THREADS / lanes_x rows; it
-// walks the rows with the grid's stride.  Row ends are ragged: lanes past the
-// last column stay for the shuffles.
+// Rows of whole groups, 16-byte aligned: the matrix, its codes and its exponents
+// are three contiguous arrays.  A lane takes 8 values (pack) or 16 (unpack), with
+// all its loads in flight before the first is used: HBM needs ~44 KB in flight
+// per SM.
+constexpr int PACK_STEPS = 4, UNPACK_STEPS = 4;
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+pack_flat_kernel(const T* __restrict__ x, int64_t vecs, uint8_t* __restrict__ codes,
+                 uint8_t* __restrict__ exps) {
+  constexpr int P = (int)sizeof(T) / 2;              // 16-byte pieces of 8 values
+  const int64_t base = (int64_t)blockIdx.x * (THREADS * PACK_STEPS) + threadIdx.x;
+  union { uint4 q[P]; T e[8]; } in[PACK_STEPS];
+#pragma unroll
+  for (int s = 0; s < PACK_STEPS; ++s) {
+    const int64_t i = base + s * THREADS;
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+      in[s].q[p] = i < vecs ? __ldcs(reinterpret_cast<const uint4*>(x) + i * P + p) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
+  for (int s = 0; s < PACK_STEPS; ++s) {
+    const int64_t i = base + s * THREADS;
+    float v[8];
+    uint32_t amax = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = to_f32(in[s].e[j]);
+      const uint32_t a = __float_as_uint(v[j]) & 0x7fffffffu;
+      amax = a > amax ? a : amax;
+    }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {                // a group is 4 lanes (vecs is a multiple of 4)
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, amax, o);
+      amax = other > amax ? other : amax;
+    }
+    if (i >= vecs) continue;
+    const uint32_t e = ckpt_exponent(amax);
+    const float up = ckpt_up(e);
+    reinterpret_cast<uint2*>(codes)[i] = make_uint2(ckpt_word(v, up), ckpt_word(v + 4, up));
+    if (i % 4 == 0) exps[i / 4] = (uint8_t)e;
+  }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(THREADS)
+unpack_flat_kernel(const uint8_t* __restrict__ codes, const uint8_t* __restrict__ exps, int64_t vecs,
+                   int act, T* __restrict__ out) {
+  const int64_t base = (int64_t)blockIdx.x * (THREADS * UNPACK_STEPS) + threadIdx.x;
+  uint4 in[UNPACK_STEPS];
+  uint32_t e[UNPACK_STEPS];
+#pragma unroll
+  for (int s = 0; s < UNPACK_STEPS; ++s) {
+    const int64_t i = base + s * THREADS;
+    in[s] = i < vecs ? __ldcs(reinterpret_cast<const uint4*>(codes) + i) : make_uint4(0, 0, 0, 0);
+    e[s] = i < vecs ? __ldg(exps + i / 2) : 1u;
+  }
+#pragma unroll 1
+  for (int s = 0; s < UNPACK_STEPS; ++s) {
+    const int64_t i = base + s * THREADS;
+    // (the loads' registers have no index: select)
+    uint4 q = in[0];
+    uint32_t x = e[0];
+#pragma unroll
+    for (int t = 1; t < UNPACK_STEPS; ++t)
+      if (s == t) { q = in[t]; x = e[t]; }
+    if (i >= vecs) break;
+    const float down = ckpt_down(x);
+    float v[16];
+    ckpt_values(q.x, down, v);
+    ckpt_values(q.y, down, v + 4);
+    ckpt_values(q.z, down, v + 8);
+    ckpt_values(q.w, down, v + 12);
+    apply_act<16>(act, v);
+    store_row<T, 16>(out + i * 16, 16, true, v);
+  }
+}
+
+// Any other matrix.  A block covers `lanes_x` lanes of V columns and THREADS /
+// lanes_x rows and walks the rows with the grid's stride.  Row ends are ragged:
+// lanes past the last column stay for the shuffles.
 template <typename T, int V>
 __global__ void __launch_bounds__(THREADS)
 pack_kernel(const T* __restrict__ x, int64_t m, int64_t n, uint8_t* __restrict__ codes,
@@ -86,6 +164,11 @@ static void pack(orca_ctx* ctx, const T* x, int64_t m, int64_t n, uint8_t* ckpt)
   uint8_t* exps = ckpt + ckpt_exps_at(m, n);
   const int align = byte_alignment(ckpt, n);
   const bool vec = byte_alignment(x, n * (int64_t)sizeof(T)) == 16;
+  if (vec && align == 16 && n % GROUP == 0) {
+    const int64_t vecs = m * n / 8;
+    pack_flat_kernel<T><<<(unsigned)cdiv(vecs, THREADS * PACK_STEPS), THREADS, 0, ctx->stream>>>(x, vecs, ckpt, exps);
+    return;
+  }
   int lx;
   // 8 columns a lane where their 16-byte (F32: 32-byte) loads are aligned; 4 in
   // single elements otherwise.
@@ -103,6 +186,12 @@ static void unpack(orca_ctx* ctx, const uint8_t* ckpt, int64_t m, int64_t n, int
   const uint8_t* exps = ckpt + ckpt_exps_at(m, n);
   const int align = byte_alignment(ckpt, n);
   const bool vec = byte_alignment(out, n * (int64_t)sizeof(T)) == 16;
+  if (vec && align == 16 && n % GROUP == 0) {
+    const int64_t vecs = m * n / 16;
+    unpack_flat_kernel<T><<<(unsigned)cdiv(vecs, THREADS * UNPACK_STEPS), THREADS, 0, ctx->stream>>>(
+        ckpt, exps, vecs, act, out);
+    return;
+  }
   int lx;
   if (vec) {
     const dim3 g = walk_grid(ctx, m, n, 8, &lx);

@@ -52,58 +52,24 @@ orca_status need_apart(const orca_span* out, const orca_span* other, const char*
 
 namespace lin {
 
-// ---------------------------------------------------------------- FFMA tiles
-// 64 x 64 tiles of F32 sums, each a sequential FMA chain over the sum's
-// index, 4 x 4 per thread; operands in any orientation and alignment.
-constexpr int SM = 64, SN = 64, SK = 16;
-
+// ---------------------------------------------------------------- empty sums
+// K = 0: the epilogue of zeros, 4 columns a lane.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256)
-tile_kernel(int64_t M, int64_t N, int64_t K, Operand A, Operand B, Epilogue e) {
-  __shared__ float As[SK][SM + 4];
-  __shared__ float Bs[SK][SN + 4];
-  const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-  const int64_t num_n = cdiv(N, SN);
-  const int64_t m0 = blockIdx.x / num_n * SM, n0 = blockIdx.x % num_n * SN;
-  const T* a = (const T*)A.p;
-  const T* b = (const T*)B.p;
-  float acc[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += SK) {
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int el = tid + r * 256;
-      const int mm = A.mn_major ? el % SM : el / SK, ka = A.mn_major ? el / SM : el % SK;
-      const int64_t gm = m0 + mm, gk = k0 + ka;
-      As[ka][mm] = gm < M && gk < K ? to_f32(a[A.mn_major ? gk * A.ld + gm : gm * A.ld + gk]) : 0.0f;
-      const int nn = B.mn_major ? el % SN : el / SK, kb = B.mn_major ? el / SN : el % SK;
-      const int64_t gn = n0 + nn, gj = k0 + kb;
-      Bs[kb][nn] = gn < N && gj < K ? to_f32(b[B.mn_major ? gj * B.ld + gn : gn * B.ld + gj]) : 0.0f;
-    }
-    __syncthreads();
-#pragma unroll
-    for (int kk = 0; kk < SK; ++kk) {
-      float av[4], bv[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) av[i] = As[kk][ty * 4 + i];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) bv[j] = Bs[kk][tx * 4 + j];
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(av[i], bv[j], acc[i][j]);
-    }
-    __syncthreads();
+zero_kernel(Epilogue e) {
+  const int64_t vecs = cdiv(e.cols, 128) * 32;       // whole warps per row (groups of columns)
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < e.rows * vecs; i += (int64_t)gridDim.x * 256) {
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    epilogue<T, MODE, 4>(e, i / vecs, i % vecs * 4, v);
   }
-#pragma unroll
-  for (int i = 0; i < 4; ++i) epilogue<T, MODE, 4>(e, m0 + ty * 4 + i, n0 + tx * 4, acc[i]);
 }
 
 // ---------------------------------------------------------------- column sums
-// db: 128 columns per cluster of up to 8 CTAs that take a part of the rows each;
-// 16 lanes of 8 columns by 16 rows a CTA, F32 sums per lane, joined over the rows'
+// db: 256 columns per cluster of up to 8 CTAs that take a part of the rows each;
+// 32 lanes of 8 columns by 8 rows a CTA, F32 sums per lane, joined over the rows'
 // lanes and then, through the cluster's shared memory, over the CTAs, always in
 // the same order.  One pass over dy, bound by HBM: 8 rows in flight per lane.
-constexpr int CS_COLS = 128, CS_ROWS = 16, CS_RANKS = 8;
+constexpr int CS_COLS = 256, CS_ROWS = 8, CS_RANKS = 8;
 
 template <typename T, typename G>
 __global__ void __launch_bounds__(256)
@@ -111,7 +77,7 @@ colsum_kernel(const T* __restrict__ x, int64_t m, int64_t n, int ranks, int64_t 
               G* __restrict__ out) {
   __shared__ float s[CS_ROWS][CS_COLS + 8];
   __shared__ float part[CS_COLS];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
+  const int tx = threadIdx.x % 32, ty = threadIdx.x / 32;
   const uint32_t rank = cluster_ctarank();
   const int64_t col0 = (int64_t)(blockIdx.x / ranks) * CS_COLS, col = col0 + tx * 8;
   const int valid = col >= n ? 0 : (n - col < 8 ? (int)(n - col) : 8);
@@ -187,9 +153,13 @@ static orca_status colsum(orca_ctx* ctx, const T* x, int64_t m, int64_t n, const
 }
 
 // ---------------------------------------------------------------- products
+template <typename T> constexpr orca_dtype dtype_of() {
+  return std::is_same<T, float>::value ? ORCA_F32 : (std::is_same<T, __half>::value ? ORCA_F16 : ORCA_BF16);
+}
+
 template <typename T, int MODE>
-static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const Operand& A,
-                           const Operand& B, Epilogue e) {
+static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const Planes& A, int a_mn,
+                           const Planes& B, int b_mn, Epilogue e) {
   if (M <= 0 || N <= 0) return ORCA_OK;
   e.rows = M;
   e.cols = N;
@@ -199,13 +169,9 @@ static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   if (e.bias) al = std::min(al, byte_alignment(e.bias, 0));
   e.vec = al == 16;
   if (e.codes) e.ckpt_align = byte_alignment(e.codes, N);
-  if (K > 0) {
-    const orca_dtype t = std::is_same<T, float>::value ? ORCA_F32 : (std::is_same<T, __half>::value ? ORCA_F16 : ORCA_BF16);
-    return mma_product(ctx, MODE, t, M, N, K, A, B, e);
-  }
-  const int64_t tiles = cdiv(M, SM) * cdiv(N, SN);
-  if (tiles > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
-  tile_kernel<T, MODE><<<(unsigned)tiles, 256, 0, ctx->stream>>>(M, N, K, A, B, e);
+  if (K > 0) return mma_product(ctx, MODE, dtype_of<T>(), M, N, K, A, a_mn, B, b_mn, e);
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(M * cdiv(N, 128) * 32, 256), (int64_t)ctx->sm_count * 16);
+  zero_kernel<T, MODE><<<grid, 256, 0, ctx->stream>>>(e);
   count_launch(ctx);
   ORCA_CUDA_TRY(cudaGetLastError());
   return ORCA_OK;
@@ -214,10 +180,12 @@ static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const
 template <typename T>
 static orca_status forward(orca_ctx* ctx, const orca_span* x, const orca_span* w, int64_t m,
                            int64_t k, int64_t n, const Epilogue& e) {
-  Operand a, b;
-  a.p = x->data; a.ld = k;
-  b.p = w->data; b.ld = n; b.mn_major = 1;
-  return product<T, FWD>(ctx, m, n, k, a, b, e);
+  if (m <= 0 || n <= 0) return ORCA_OK;
+  Scratch sx(ctx), sw(ctx);
+  Planes px, pw;
+  ORCA_TRY(mma_prepare(ctx, dtype_of<T>(), x->data, m, k, sx, &px));
+  ORCA_TRY(mma_prepare(ctx, dtype_of<T>(), w->data, k, n, sw, &pw));
+  return product<T, FWD>(ctx, m, n, k, px, 0, pw, 1, e);
 }
 
 template <typename T>
@@ -225,20 +193,20 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
                             const orca_span* dy, const orca_span* residual, int64_t m, int64_t k,
                             int64_t n, int act, const orca_span* dx, const orca_span* dw,
                             const orca_span* db) {
+  constexpr orca_dtype dtype = dtype_of<T>();
   const bool packed = x && x->dtype == ORCA_U8;
   // dW's operand a = act(x): x itself, or a matrix that the epilogue of the dX
   // product writes on the way (it reads x for the slope anyway), or a pass of its own.
-  Scratch act_x(ctx);
-  const void* a_operand = x ? x->data : nullptr;
+  Scratch act_x(ctx), sdy(ctx);
+  const void* a = x ? x->data : nullptr;
   if (dw && m * k > 0 && (packed || act != ORCA_ACT_NONE)) {
     ORCA_TRY(act_x.get((size_t)(m * k) * sizeof(T)));
-    a_operand = act_x.p;
+    a = act_x.p;
   }
   const bool emit = act_x.p && dx && n > 0;
+  Planes pdy;
+  if ((dx || dw) && k > 0) ORCA_TRY(mma_prepare(ctx, dtype, dy->data, m, n, sdy, &pdy));
   if (dx) {
-    Operand a, b;
-    a.p = dy->data; a.ld = n;
-    b.p = w->data; b.ld = n;
     Epilogue e;
     e.act = act;
     e.out = dx->data;
@@ -252,22 +220,25 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
       }
     }
     if (emit) e.a = act_x.p;
-    ORCA_TRY((product<T, DX>(ctx, m, k, n, a, b, e)));
+    Scratch sw(ctx);
+    Planes pw;
+    ORCA_TRY(mma_prepare(ctx, dtype, w->data, k, n, sw, &pw));
+    ORCA_TRY((product<T, DX>(ctx, m, k, n, pdy, 0, pw, 0, e)));
   }
   if (dw) {
     if (act_x.p && !emit) {
       if (packed)
-        ORCA_TRY(ckpt8_unpack_launch(ctx, (const uint8_t*)x->data, m, k, act, act_x.p, dy->dtype));
+        ORCA_TRY(ckpt8_unpack_launch(ctx, (const uint8_t*)x->data, m, k, act, act_x.p, dtype));
       else
-        ORCA_TRY(act_launch(ctx, x->data, x->dtype, m * k, act, act_x.p));
+        ORCA_TRY(act_launch(ctx, x->data, dtype, m * k, act, act_x.p));
     }
-    Operand a, b;
-    a.p = a_operand; a.ld = k; a.mn_major = 1;
-    b.p = dy->data; b.ld = n; b.mn_major = 1;
     Epilogue e;
     e.out = dw->data;
     e.out_f32 = dw->dtype == ORCA_F32;
-    ORCA_TRY((product<T, DW>(ctx, k, n, m, a, b, e)));
+    Scratch sa(ctx);
+    Planes pa;
+    ORCA_TRY(mma_prepare(ctx, dtype, a, m, k, sa, &pa));
+    ORCA_TRY((product<T, DW>(ctx, k, n, m, pa, 1, pdy, 1, e)));
   }
   if (db) ORCA_TRY(colsum<T>(ctx, (const T*)dy->data, m, n, db));
   return ORCA_OK;

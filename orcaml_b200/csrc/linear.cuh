@@ -201,6 +201,16 @@ __device__ __forceinline__ uint32_t ckpt_word(const float* v, float up) {
   return up == 0.0f ? 0u : __byte_perm(a, b, 0x5410);
 }
 
+// Values of the four codes of a word: a code plus 128 as the low mantissa byte of
+// 2^23, less 2^23 + 128 (exact; again no conversion instruction).
+__device__ __forceinline__ void ckpt_values(uint32_t word, float down, float* v) {
+  const uint32_t w = word ^ 0x80808080u;
+  v[0] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)) - 8388736.0f) * down;
+  v[1] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)) - 8388736.0f) * down;
+  v[2] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)) - 8388736.0f) * down;
+  v[3] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)) - 8388736.0f) * down;
+}
+
 // Codes the V values of one lane, 32 / V adjacent lanes sharing a group (all
 // of them call this), and stores codes and exponent.  Columns from `valid` on
 // are outside.  `words`: 4-byte (V >= 4) stores are aligned; `quads`: 16-byte.
@@ -275,8 +285,7 @@ __device__ __forceinline__ void ckpt_load(const uint8_t* codes, const uint8_t* e
       for (int i = 0; i < V / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
     }
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      v[i] = (float)(int8_t)(w[i / 4] >> (8 * (i % 4))) * down;
+    for (int i = 0; i < V / 4; ++i) ckpt_values(w[i], down, v + 4 * i);
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i) v[i] = i < valid ? (float)(int8_t)p[i] * down : 0.0f;
@@ -475,7 +484,7 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       union { uint4 q[2]; uint32_t w[8]; } u;
       block_load<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
 #pragma unroll
-      for (int i = 0; i < 32; ++i) t[i] = (float)(int8_t)(u.w[i / 4] >> (8 * (i % 4))) * down;
+      for (int i = 0; i < 8; ++i) ckpt_values(u.w[i], down, t + 4 * i);
     } else {
       block_load_f32<T>((const T*)e.x + at, e.cols, rows, t, smem, lane);
     }
@@ -504,12 +513,13 @@ orca_status ckpt8_unpack_launch(orca_ctx* ctx, const uint8_t* ckpt, int64_t m, i
 orca_status act_launch(orca_ctx* ctx, const void* x, orca_dtype dtype, int64_t len, int act, void* out);
 
 namespace lin {
-// Element (i, c) of an operand, i along the output and c along the sum: at
-// c * ld + i when mn_major, else at i * ld + c.
-struct Operand {
+// A matrix as the tensor cores take it: rows of `cols` contiguous 16-bit elements
+// with 16-byte aligned row starts, in 1 plane (BF16, F16) or 3 (F32).  ld and
+// plane count elements.
+struct Planes {
   const void* p = nullptr;
-  int64_t ld = 0;
-  int mn_major = 0;
+  int64_t ld = 0, plane = 0;
+  int64_t rows = 0, cols = 0;
 };
 
 // Stream-ordered scratch of one call; in a captured graph it becomes the
@@ -528,10 +538,15 @@ struct Scratch {
 };
 }  // namespace lin
 
-// linear_mma.cu: D[M, N] = A @ B on the tensor cores, through the epilogue.
-// K > 0; operands of element type `dtype`, any alignment.
+// linear_mma.cu.  mma_prepare: the planes of a contiguous [rows, cols] matrix of
+// any alignment, in `scratch` unless the matrix itself will do.  mma_product:
+// D[M, N] = A @ B through the epilogue, K > 0; an operand's matrix has the sum
+// along its rows' elements, or with *_mn along its rows.
+orca_status mma_prepare(orca_ctx* ctx, orca_dtype dtype, const void* p, int64_t rows, int64_t cols,
+                        lin::Scratch& scratch, lin::Planes* out);
 orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, int64_t N, int64_t K,
-                        const lin::Operand& A, const lin::Operand& B, const lin::Epilogue& e);
+                        const lin::Planes& a, int a_mn, const lin::Planes& b, int b_mn,
+                        const lin::Epilogue& e);
 
 // Checks of spans (linear.cu).
 orca_status need_span(orca_ctx* ctx, const orca_span* s, int64_t len, const char* what);

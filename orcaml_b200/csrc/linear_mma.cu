@@ -515,9 +515,11 @@ template <int NT> constexpr int split_stage() { return TILE + NT * BK * 2; }
 template <int NT> constexpr int split_stages() { return 196608 / split_stage<NT>() < 12 ? 196608 / split_stage<NT>() : 12; }
 template <int NT> constexpr int split_smem() { return split_stages<NT>() * split_stage<NT>() + 1024 + 256; }
 
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(addr));
   return v;
 }
 
@@ -666,19 +668,30 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   if (warp == 1) tmem_dealloc(tmem, COLS);
-  const int lane_col = (warp & 3) * 32 + lane;
   if (warp >= 2) {
 #pragma unroll
-    for (int j = 0; j < NT; ++j) part[j * 128 + lane_col] = acc[j];
+    for (int j = 0; j < NT; ++j) part[j * 128 + (warp & 3) * 32 + lane] = acc[j];
   }
   cluster_sync_all();
-  if (warp >= 2 && !*abort_flag) {
+  if (!*abort_flag) {
+    // A warp per row, 4 columns per lane; the parts of a row are all in flight at once.
     const int j1 = NT * (rank + 1) / ranks;
-    for (int j = NT * rank / ranks; j < j1 && row0 + j < p.M; ++j) {
-      float v[1] = {0.0f};
-      for (int r = 0; r < ranks; ++r)
-        v[0] = __fadd_rn(v[0], ld_cluster_f32(cluster_addr(part + j * 128 + lane_col, (uint32_t)r)));
-      epilogue<T, MODE, 1>(p.e, row0 + j, col0 + lane_col, v);
+    for (int j = NT * rank / ranks + warp; j < j1 && row0 + j < p.M; j += SPLIT_THREADS / 32) {
+      float4 u[8];
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ranks) u[r] = ld_cluster_f32x4(cluster_addr(part + j * 128 + lane * 4, (uint32_t)r));
+      float v[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+#pragma unroll
+      for (int r = 1; r < 8; ++r) {
+        if (r < ranks) {
+          v[0] = __fadd_rn(v[0], u[r].x);
+          v[1] = __fadd_rn(v[1], u[r].y);
+          v[2] = __fadd_rn(v[2], u[r].z);
+          v[3] = __fadd_rn(v[3], u[r].w);
+        }
+      }
+      epilogue<T, MODE, 4>(p.e, row0 + j, col0 + lane * 4, v);
     }
   }
   __syncwarp();
@@ -724,38 +737,33 @@ prepare_kernel(const S* __restrict__ x, int64_t rows, int64_t cols, int64_t ld, 
   }
 }
 
-// An operand as the tensor maps take it: 16-bit planes, rows 16-byte aligned.
-struct Planes {
-  const void* p;
-  int64_t ld, plane;      // elements
-  int64_t rows, cols;     // rows of cols contiguous elements
-};
+}  // namespace lin
 
-static orca_status prepare(orca_ctx* ctx, orca_dtype dtype, const Operand& op, int64_t mn, int64_t k,
-                           Scratch& scratch, Planes* out) {
-  out->rows = op.mn_major ? k : mn;
-  out->cols = op.mn_major ? mn : k;
-  out->ld = op.ld;
-  out->plane = out->rows * out->ld;
-  out->p = op.p;
-  if (dtype != ORCA_F32 && byte_alignment(op.p, op.ld * 2) == 16) return ORCA_OK;
-  out->ld = cdiv(out->cols, 8) * 8;
-  out->plane = out->rows * out->ld;
+orca_status mma_prepare(orca_ctx* ctx, orca_dtype dtype, const void* p, int64_t rows, int64_t cols,
+                        lin::Scratch& scratch, lin::Planes* out) {
+  using namespace lin;
+  *out = Planes{p, cols, rows * cols, rows, cols};
+  if (rows <= 0 || cols <= 0) return ORCA_OK;
+  if (dtype != ORCA_F32 && byte_alignment(p, cols * 2) == 16) return ORCA_OK;
+  out->ld = cdiv(cols, 8) * 8;
+  out->plane = rows * out->ld;
   const int planes = dtype == ORCA_F32 ? 3 : 1;
   ORCA_TRY(scratch.get((size_t)(planes * out->plane) * 2));
   out->p = scratch.p;
   const int64_t vecs = out->plane / 8;
   const unsigned grid = (unsigned)std::min<int64_t>(cdiv(vecs, 256), (int64_t)ctx->sm_count * 16);
   if (dtype == ORCA_F32)
-    prepare_kernel<float><<<grid, 256, 0, ctx->stream>>>((const float*)op.p, out->rows, out->cols, op.ld,
+    prepare_kernel<float><<<grid, 256, 0, ctx->stream>>>((const float*)p, rows, cols, cols,
                                                          (uint16_t*)scratch.p, out->ld);
   else
-    prepare_kernel<__half><<<grid, 256, 0, ctx->stream>>>((const __half*)op.p, out->rows, out->cols, op.ld,
+    prepare_kernel<__half><<<grid, 256, 0, ctx->stream>>>((const __half*)p, rows, cols, cols,
                                                           (uint16_t*)scratch.p, out->ld);
   count_launch(ctx);
   ORCA_CUDA_TRY(cudaGetLastError());
   return ORCA_OK;
 }
+
+namespace lin {
 
 // ---------------------------------------------------------------- tensor maps
 static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -912,16 +920,13 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
 }  // namespace lin
 
 orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, int64_t N, int64_t K,
-                        const lin::Operand& A, const lin::Operand& B, const lin::Epilogue& e) {
+                        const lin::Planes& a, int a_mn, const lin::Planes& b, int b_mn,
+                        const lin::Epilogue& e) {
   using namespace lin;
-  Scratch sa(ctx), sb(ctx);
-  Planes a, b;
-  ORCA_TRY(prepare(ctx, dtype, A, M, K, sa, &a));
-  ORCA_TRY(prepare(ctx, dtype, B, N, K, sb, &b));
   Params p;
   p.M = M; p.N = N; p.K = K;
-  p.a_mn = A.mn_major;
-  p.b_mn = B.mn_major;
+  p.a_mn = a_mn;
+  p.b_mn = b_mn;
   p.bf16 = dtype != ORCA_F16;
   p.pairs = dtype == ORCA_F32 ? F32_PAIRS : 1;
   // Raster: 8 tile rows by 9 columns are about what runs at once.  Where all of A
