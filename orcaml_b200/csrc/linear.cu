@@ -177,14 +177,22 @@ static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   return ORCA_OK;
 }
 
+static Planes matrix(const void* p, int64_t rows, int64_t cols) {
+  Planes x;
+  x.p = p;
+  x.rows = rows;
+  x.cols = cols;
+  return x;
+}
+
 template <typename T>
 static orca_status forward(orca_ctx* ctx, const orca_span* x, const orca_span* w, int64_t m,
                            int64_t k, int64_t n, const Epilogue& e) {
   if (m <= 0 || n <= 0) return ORCA_OK;
-  Scratch sx(ctx), sw(ctx);
-  Planes px, pw;
-  ORCA_TRY(mma_prepare(ctx, dtype_of<T>(), x->data, m, k, sx, &px));
-  ORCA_TRY(mma_prepare(ctx, dtype_of<T>(), w->data, k, n, sw, &pw));
+  Scratch scratch(ctx);
+  Planes px = matrix(x->data, m, k), pw = matrix(w->data, k, n);
+  Planes* const both[] = {&px, &pw};
+  ORCA_TRY(mma_prepare(ctx, dtype_of<T>(), both, 2, scratch));
   return product<T, FWD>(ctx, m, n, k, px, 0, pw, 1, e);
 }
 
@@ -197,15 +205,17 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
   const bool packed = x && x->dtype == ORCA_U8;
   // dW's operand a = act(x): x itself, or a matrix that the epilogue of the dX
   // product writes on the way (it reads x for the slope anyway), or a pass of its own.
-  Scratch act_x(ctx), sdy(ctx);
+  Scratch act_x(ctx), scratch(ctx), scratch_a(ctx);
   const void* a = x ? x->data : nullptr;
   if (dw && m * k > 0 && (packed || act != ORCA_ACT_NONE)) {
     ORCA_TRY(act_x.get((size_t)(m * k) * sizeof(T)));
     a = act_x.p;
   }
   const bool emit = act_x.p && dx && n > 0;
-  Planes pdy;
-  if ((dx || dw) && k > 0) ORCA_TRY(mma_prepare(ctx, dtype, dy->data, m, n, sdy, &pdy));
+  Planes pdy = matrix(dy->data, m, n), pw, pa;
+  if (dx) pw = matrix(w->data, k, n);
+  Planes* const first[] = {&pdy, &pw};
+  if ((dx || dw) && k > 0) ORCA_TRY(mma_prepare(ctx, dtype, first, 2, scratch));
   if (dx) {
     Epilogue e;
     e.act = act;
@@ -220,9 +230,6 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
       }
     }
     if (emit) e.a = act_x.p;
-    Scratch sw(ctx);
-    Planes pw;
-    ORCA_TRY(mma_prepare(ctx, dtype, w->data, k, n, sw, &pw));
     ORCA_TRY((product<T, DX>(ctx, m, k, n, pdy, 0, pw, 0, e)));
   }
   if (dw) {
@@ -235,9 +242,9 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
     Epilogue e;
     e.out = dw->data;
     e.out_f32 = dw->dtype == ORCA_F32;
-    Scratch sa(ctx);
-    Planes pa;
-    ORCA_TRY(mma_prepare(ctx, dtype, a, m, k, sa, &pa));
+    pa = matrix(a, m, k);
+    Planes* const second[] = {&pa};
+    ORCA_TRY(mma_prepare(ctx, dtype, second, 1, scratch_a));
     ORCA_TRY((product<T, DW>(ctx, k, n, m, pa, 1, pdy, 1, e)));
   }
   if (db) ORCA_TRY(colsum<T>(ctx, (const T*)dy->data, m, n, db));

@@ -538,12 +538,14 @@ struct Scratch {
 };
 }  // namespace lin
 
-// linear_mma.cu.  mma_prepare: the planes of a contiguous [rows, cols] matrix of
-// any alignment, in `scratch` unless the matrix itself will do.  mma_product:
-// D[M, N] = A @ B through the epilogue, K > 0; an operand's matrix has the sum
-// along its rows' elements, or with *_mn along its rows.
-orca_status mma_prepare(orca_ctx* ctx, orca_dtype dtype, const void* p, int64_t rows, int64_t cols,
-                        lin::Scratch& scratch, lin::Planes* out);
+// linear_mma.cu.  mma_prepare: takes contiguous [rows, cols] matrices of any
+// alignment (p, rows, cols set) and makes planes of them, in `scratch` where the
+// matrix itself will not do.  mma_product: D[M, N] = A @ B through the epilogue,
+// K > 0; an operand's matrix has the sum along its rows' elements, or with *_mn
+// along its rows.
+constexpr int MAX_OPERANDS = 2;
+orca_status mma_prepare(orca_ctx* ctx, orca_dtype dtype, lin::Planes* const* x, int count,
+                        lin::Scratch& scratch);
 orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, int64_t N, int64_t K,
                         const lin::Planes& a, int a_mn, const lin::Planes& b, int b_mn,
                         const lin::Epilogue& e);

@@ -32,9 +32,6 @@ constexpr int TILE = ROWS * BK * 2;          // 16 KB
 constexpr uint32_t PAIR_A = 0x001102u, PAIR_B = 0x010120u;   // pair p: (x >> 4 * p) & 15
 constexpr int F32_PAIRS = 6;
 
-// What sharing a tile among clusters costs, in steps of the whole grid.
-constexpr int SHARE_STEPS = 24;
-
 // Steps (of four MMAs) per accumulation chunk of an F32 result.  The tensor core
 // adds with a few bits less than F32; a chain of L MMAs over random data is off by
 // about 9e-10 * L^1.5 of the result's norm.  F32 operands: 64 MMAs, 5e-7, what an
@@ -403,8 +400,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       const int64_t row = tm * 256 + (int64_t)rank * 128 + quarter * 32;
       const int64_t col = tn * 256 + half * 128;
       const bool piece = stop - begin < steps;
-      // This warp's part of a piece: blocks of 32 columns, column by column.
-      const int64_t my_part = (int64_t)((rank * EPI_WARPS + warp - 2) * 4) * 1024 + lane;
+      // This warp's part of a piece: blocks of 32 columns, four columns of each lane
+      // side by side.
+      const int64_t my_part = (int64_t)((rank * EPI_WARPS + warp - 2) * 4) * 1024 + lane * 4;
       float* mine = p.parts + (cluster * 2 + (begin == 0)) * PART_FLOATS + my_part;
       const int nchunks = (stop - begin + p.chunk - 1) / p.chunk;
       auto release = [&](int buf) {
@@ -447,14 +445,17 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
       }
       if (!ok) break;
-      int64_t first = 0, count = 0;
+      int64_t first = 0;
+      int count = 0;
       if (piece) {
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           float v[32];
           tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
 #pragma unroll
-          for (int j = 0; j < 32; ++j) __stcg(mine + (q * 32 + j) * 32, v[j]);
+          for (int j = 0; j < 8; ++j)
+            __stcg(reinterpret_cast<float4*>(mine + (q * 8 + j) * 128),
+                   make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
         }
         release(buf);
         // Clusters first .. first + count - 1 share this tile.
@@ -464,13 +465,13 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         while (total * first / p.tail > t * steps) --first;
         int64_t lastc = first;
         while (total * (lastc + 1) / p.tail < (t + 1) * steps) ++lastc;
-        count = lastc - first + 1;
+        count = (int)(lastc - first) + 1;
         __threadfence();
         __syncwarp();
         int before = 0;
         if (lane == 0) before = atomicAdd(p.arrived + t * ARRIVALS + rank * EPI_WARPS + warp - 2, 1);
         before = __shfl_sync(0xffffffffu, before, 0);
-        if (before != (int)count - 1) continue;
+        if (before != count - 1) continue;
         __threadfence();
       }
 #pragma unroll 1
@@ -478,12 +479,41 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         if (col + q * 32 >= p.N) break;
         float v[32];
         if (piece) {
+          // Two pieces' loads in flight; added in the pieces' order.
+          const float* part = p.parts + (first * 2 + 1) * PART_FLOATS + my_part + q * 1024;
+          const float* next = p.parts + (first + 1) * 2 * PART_FLOATS + my_part + q * 1024;
+          float4 x[8], y[8];
 #pragma unroll
-          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
-          for (int64_t c = 0; c < count; ++c) {
-            const float* part = p.parts + ((first + c) * 2 + (c == 0)) * PART_FLOATS + my_part;
+          for (int j = 0; j < 8; ++j) x[j] = __ldcg(reinterpret_cast<const float4*>(part + j * 128));
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] = __fadd_rn(v[j], __ldcg(part + (q * 32 + j) * 32));
+          for (int j = 0; j < 8; ++j) {
+            v[4 * j] = x[j].x; v[4 * j + 1] = x[j].y; v[4 * j + 2] = x[j].z; v[4 * j + 3] = x[j].w;
+          }
+          for (int c = 1; c < count; c += 2) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x[j] = __ldcg(reinterpret_cast<const float4*>(next + j * 128));
+            next += 2 * PART_FLOATS;
+            if (c + 1 < count) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) y[j] = __ldcg(reinterpret_cast<const float4*>(next + j * 128));
+              next += 2 * PART_FLOATS;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              v[4 * j] = __fadd_rn(v[4 * j], x[j].x);
+              v[4 * j + 1] = __fadd_rn(v[4 * j + 1], x[j].y);
+              v[4 * j + 2] = __fadd_rn(v[4 * j + 2], x[j].z);
+              v[4 * j + 3] = __fadd_rn(v[4 * j + 3], x[j].w);
+            }
+            if (c + 1 < count) {
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                v[4 * j] = __fadd_rn(v[4 * j], y[j].x);
+                v[4 * j + 1] = __fadd_rn(v[4 * j + 1], y[j].y);
+                v[4 * j + 2] = __fadd_rn(v[4 * j + 2], y[j].z);
+                v[4 * j + 3] = __fadd_rn(v[4 * j + 3], y[j].w);
+              }
+            }
           }
         } else {
           tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
@@ -509,10 +539,12 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 // adds, in rank order, and stores a share of the rows.  Warp 0 loads, warp 1
 // issues the MMAs, warps 2-5 (one TMEM lane quarter each) hold a column per
 // thread.  With few rows the weights' bytes are all the work, and the stages
-// keep ~190 KB of them in flight per SM.
+// keep 100 to 190 KB of them in flight per SM.
 constexpr int SPLIT_THREADS = 192;
 template <int NT> constexpr int split_stage() { return TILE + NT * BK * 2; }
-template <int NT> constexpr int split_stages() { return 196608 / split_stage<NT>() < 12 ? 196608 / split_stage<NT>() : 12; }
+// With 16 rows two CTAs share an SM (108 KB each): one starts while the other ends
+// (16384 columns of 4096: 23.9 us against 26.0 with one CTA of 10 stages).
+template <int NT> constexpr int split_stages() { return NT == 16 ? 6 : 196608 / split_stage<NT>(); }
 template <int NT> constexpr int split_smem() { return split_stages<NT>() * split_stage<NT>() + 1024 + 256; }
 
 __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
@@ -699,65 +731,94 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
 }
 
 // ---------------------------------------------------------------- operand preparation
-// [rows, cols] (row stride ld) -> planes of BF16 / F16 with row stride ldp (a
+// Contiguous [rows, cols] matrices -> planes of BF16 / F16 with row stride ldp (a
 // multiple of 8): F32 is split, 16-bit types are copied.  The padding is outside
-// the tensor map and not written.
-template <typename S>
+// the tensor map.  One launch for all operands of a call; bound by HBM (F32: 10
+// bytes an element).
+struct Prepare {
+  const void* x[MAX_OPERANDS];
+  uint16_t* out[MAX_OPERANDS];
+  int64_t rows[MAX_OPERANDS], cols[MAX_OPERANDS], ldp[MAX_OPERANDS];
+  int64_t end[MAX_OPERANDS];      // of each matrix's 8-element pieces, counted through
+  int count;
+};
+
+template <bool F32>
 __global__ void __launch_bounds__(256)
-prepare_kernel(const S* __restrict__ x, int64_t rows, int64_t cols, int64_t ld, uint16_t* __restrict__ out,
-               int64_t ldp) {
-  const int64_t plane = rows * ldp, per_row = ldp / 8, vecs = rows * per_row;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < vecs; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / per_row, c = (i - r * per_row) * 8;
-    const S* p = x + r * ld + c;
+prepare_kernel(const __grid_constant__ Prepare job) {
+  const int64_t total = job.end[job.count - 1];
+  for (int64_t g = (int64_t)blockIdx.x * 256 + threadIdx.x; g < total; g += (int64_t)gridDim.x * 256) {
+    int o = 0;
+    while (g >= job.end[o]) ++o;
+    const int64_t i = g - (o ? job.end[o - 1] : 0), cols = job.cols[o], ldp = job.ldp[o];
+    const int64_t per_row = ldp / 8, plane = job.rows[o] * ldp;
+    const int64_t r = total <= INT32_MAX ? (int64_t)((uint32_t)i / (uint32_t)per_row) : i / per_row;
+    const int64_t c = (i - r * per_row) * 8;
     union { uint4 q; uint16_t e[8]; } u[3];
+    if (F32) {
+      const float* p = (const float*)job.x[o] + r * cols + c;
+      const bool whole = (reinterpret_cast<uintptr_t>(p) & 15) == 0 && c + 8 <= cols;
+      float v[8];
+      load_row<float, 8>(p, cols - c < 8 ? (int)(cols - c) : 8, whole, v);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      if (sizeof(S) == 4) {
-        const float v = c + j < cols ? (float)to_f32(p[j]) : 0.0f;
-        const uint32_t b0 = __float_as_uint(v) & 0xffff0000u;
-        const float r1 = v - __uint_as_float(b0);
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t b0 = __float_as_uint(v[j]) & 0xffff0000u;
+        const float r1 = v[j] - __uint_as_float(b0);
         const uint32_t b1 = __float_as_uint(r1) & 0xffff0000u;
         const float r2 = r1 - __uint_as_float(b1);
         // An infinity or a NaN has no remainder: its first plane carries it.
         const bool fine = (b0 & 0x7f800000u) != 0x7f800000u;
-        u[0].e[j] = (uint16_t)((fine ? b0 : (__float_as_uint(v) | (v != v ? 0x400000u : 0u))) >> 16);
+        u[0].e[j] = (uint16_t)((fine ? b0 : (__float_as_uint(v[j]) | (v[j] != v[j] ? 0x400000u : 0u))) >> 16);
         u[1].e[j] = fine ? (uint16_t)(b1 >> 16) : (uint16_t)0;
         u[2].e[j] = fine ? (uint16_t)(__float_as_uint(r2) >> 16) : (uint16_t)0;
-      } else {
-        u[0].e[j] = c + j < cols ? reinterpret_cast<const uint16_t*>(p)[j] : (uint16_t)0;
       }
+    } else {
+      const uint16_t* p = (const uint16_t*)job.x[o] + r * cols + c;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) u[0].e[j] = c + j < cols ? p[j] : (uint16_t)0;
     }
-    uint4* o = reinterpret_cast<uint4*>(out + r * ldp + c);
-    o[0] = u[0].q;
-    if (sizeof(S) == 4) {
-      *reinterpret_cast<uint4*>(out + plane + r * ldp + c) = u[1].q;
-      *reinterpret_cast<uint4*>(out + 2 * plane + r * ldp + c) = u[2].q;
+    uint4* out = reinterpret_cast<uint4*>(job.out[o] + r * ldp + c);
+    out[0] = u[0].q;
+    if (F32) {
+      out[plane / 8] = u[1].q;
+      out[plane / 4] = u[2].q;
     }
   }
 }
-
 }  // namespace lin
 
-orca_status mma_prepare(orca_ctx* ctx, orca_dtype dtype, const void* p, int64_t rows, int64_t cols,
-                        lin::Scratch& scratch, lin::Planes* out) {
+orca_status mma_prepare(orca_ctx* ctx, orca_dtype dtype, lin::Planes* const* x, int count,
+                        lin::Scratch& scratch) {
   using namespace lin;
-  *out = Planes{p, cols, rows * cols, rows, cols};
-  if (rows <= 0 || cols <= 0) return ORCA_OK;
-  if (dtype != ORCA_F32 && byte_alignment(p, cols * 2) == 16) return ORCA_OK;
-  out->ld = cdiv(cols, 8) * 8;
-  out->plane = rows * out->ld;
+  Prepare job = {};
   const int planes = dtype == ORCA_F32 ? 3 : 1;
-  ORCA_TRY(scratch.get((size_t)(planes * out->plane) * 2));
-  out->p = scratch.p;
-  const int64_t vecs = out->plane / 8;
-  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(vecs, 256), (int64_t)ctx->sm_count * 16);
-  if (dtype == ORCA_F32)
-    prepare_kernel<float><<<grid, 256, 0, ctx->stream>>>((const float*)p, rows, cols, cols,
-                                                         (uint16_t*)scratch.p, out->ld);
-  else
-    prepare_kernel<__half><<<grid, 256, 0, ctx->stream>>>((const __half*)p, rows, cols, cols,
-                                                          (uint16_t*)scratch.p, out->ld);
+  size_t bytes = 0, at[MAX_OPERANDS];
+  Planes* which[MAX_OPERANDS];
+  for (int i = 0; i < count; ++i) {
+    Planes& p = *x[i];
+    p.ld = p.cols;
+    p.plane = p.rows * p.cols;
+    if (p.plane <= 0 || (dtype != ORCA_F32 && byte_alignment(p.p, p.cols * 2) == 16)) continue;
+    const int o = job.count++;
+    which[o] = &p;
+    job.x[o] = p.p;
+    job.rows[o] = p.rows;
+    job.cols[o] = p.cols;
+    p.ld = job.ldp[o] = cdiv(p.cols, 8) * 8;
+    p.plane = p.rows * p.ld;
+    job.end[o] = p.plane / 8 + (o ? job.end[o - 1] : 0);
+    at[o] = bytes;
+    bytes += (size_t)(planes * p.plane) * 2;      // a multiple of 16
+  }
+  if (!job.count) return ORCA_OK;
+  ORCA_TRY(scratch.get(bytes));
+  for (int o = 0; o < job.count; ++o) {
+    job.out[o] = (uint16_t*)((uint8_t*)scratch.p + at[o]);
+    which[o]->p = job.out[o];
+  }
+  const unsigned grid = (unsigned)std::min<int64_t>(cdiv(job.end[job.count - 1], 256), (int64_t)ctx->sm_count * 16);
+  if (dtype == ORCA_F32) prepare_kernel<true><<<grid, 256, 0, ctx->stream>>>(job);
+  else prepare_kernel<false><<<grid, 256, 0, ctx->stream>>>(job);
   count_launch(ctx);
   ORCA_CUDA_TRY(cudaGetLastError());
   return ORCA_OK;
@@ -794,6 +855,39 @@ static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int b
   return ORCA_OK;
 }
 
+// ---------------------------------------------------------------- plans
+// Times in microseconds that the choices below compare, measured at 1.9 GHz: a
+// pair step; and what sharing a tile among `parts` clusters costs (each leaves its
+// sums in L2, the last one adds them).
+constexpr double PAIR_STEP = 0.42;
+static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
+
+// The tiles beyond whole rounds of n clusters: how many clusters share them (0:
+// none do, they are a last round of their own), and the steps that round takes.
+struct Tail {
+  int64_t clusters, steps;
+};
+static Tail share(int64_t rest, int64_t steps, int64_t n, double* us) {
+  Tail best{0, rest ? steps : 0};
+  *us = rest ? (double)steps * PAIR_STEP : 0.0;
+  // An equal number of clusters per tile, or all of them with ranges that cross tiles.
+  for (int64_t parts = 2; rest && parts <= 5; ++parts) {
+    int64_t c = rest * parts, pieces = parts;
+    if (c > n) {
+      c = n;
+      pieces = cdiv(n, rest) + 1;
+    }
+    const int64_t s = cdiv(rest * steps, c);
+    const double t = (double)s * PAIR_STEP + share_cost(pieces);
+    if (t < *us) {
+      *us = t;
+      best = Tail{c, s};
+    }
+    if (c == n) break;
+  }
+  return best;
+}
+
 // ---------------------------------------------------------------- launches
 template <typename T, int MODE>
 static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, Params p) {
@@ -821,19 +915,17 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   }
   const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256), n = fit.load();
   const int64_t steps = cdiv(p.K, BK) * p.pairs, rest = tiles % n;
-  // Sharing the last tiles saves the part of a round that would be idle and costs
-  // a pass over the pieces, about SHARE_STEPS steps.  At most 4 clusters a tile:
-  // its last one reads all their pieces.
-  const int64_t tail = std::min(n, rest * 4);
+  double us;
+  const Tail tail = share(rest, steps, n, &us);
   p.full = tiles;
   p.tail = 0;
   p.parts = nullptr;
   p.arrived = nullptr;
   Scratch scratch(ctx);
-  if (rest && steps - cdiv(rest * steps, tail) > SHARE_STEPS) {
+  if (tail.clusters) {
     p.full = tiles - rest;
-    p.tail = (int)tail;
-    const size_t parts = (size_t)(tail * 2 * PART_FLOATS) * 4, counters = (size_t)(rest * ARRIVALS) * 4;
+    p.tail = (int)tail.clusters;
+    const size_t parts = (size_t)(tail.clusters * 2 * PART_FLOATS) * 4, counters = (size_t)(rest * ARRIVALS) * 4;
     ORCA_TRY(scratch.get(parts + counters));
     p.parts = (float*)scratch.p;
     p.arrived = (int*)((uint8_t*)scratch.p + parts);
@@ -845,15 +937,43 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   return ORCA_OK;
 }
 
+// Clusters of 2^i CTAs of a split_kernel that are resident at once (asked once per
+// device: clusters of 8 do not fill every GPC).
 template <typename T, int MODE, int NT>
-static orca_status launch_split(orca_ctx* ctx, const CUtensorMap& mp, const CUtensorMap& mq, const Params& p,
-                                int ranks) {
+static orca_status split_fits(orca_ctx* ctx, int (&fits)[4]) {
+  static std::atomic<int> known[64][4];
   const auto kernel = split_kernel<T, MODE, NT>;
-  static std::atomic<bool> ready[64];
-  if (!ready[ctx->device & 63].load()) {
-    ORCA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem<NT>()));
-    ready[ctx->device & 63].store(true);
+  for (int i = 3; i >= 0; --i) {
+    std::atomic<int>& fit = known[ctx->device & 63][i];
+    if (fit.load() == 0) {
+      if (i == 3)
+        ORCA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, split_smem<NT>()));
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1u << i;
+      attr[0].val.clusterDim.y = 1;
+      attr[0].val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1024);
+      cfg.blockDim = dim3(SPLIT_THREADS);
+      cfg.dynamicSmemBytes = split_smem<NT>();
+      cfg.attrs = attr;
+      cfg.numAttrs = 1;
+      int n = 0;
+      ORCA_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+      fit.store(std::max(n, 1));
+    }
+    fits[i] = fit.load();
   }
+  return ORCA_OK;
+}
+
+template <typename T, int MODE, int NT>
+static orca_status launch_split(orca_ctx* ctx, const Planes& a, const Planes& b, int planes, const Params& p,
+                                int ranks) {
+  CUtensorMap ma, mb;
+  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : NT));
+  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ranks;
@@ -868,34 +988,48 @@ static orca_status launch_split(orca_ctx* ctx, const CUtensorMap& mp, const CUte
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, mp, mq, p, ranks));
+  ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, split_kernel<T, MODE, NT>, mb, ma, p, ranks));
   count_launch(ctx);
   return ORCA_OK;
 }
 
-// Which kernel, by an estimate of its time in clocks.  A pair step (256 x 256 x
-// 64 on two SMs) takes 512 clocks of the tensor pipe; a split step 2 * NT, or
-// its bytes at what an SM gets from L2 when all of them load (about 40 a clock).
 struct Plan {
-  int nt;       // 0: pair_kernel
-  int ranks;
+  int nt = 0;       // 0: pair_kernel
+  int ranks = 1;
+  double us = 0;
 };
-static Plan choose(orca_ctx* ctx, const Params& p, int64_t steps, bool q_mn) {
-  const int64_t pair_tiles = cdiv(p.M, 256) * cdiv(p.N, 256), clusters = ctx->sm_count / 2;
-  const int64_t rest = pair_tiles % clusters;
-  const int64_t last = rest ? std::min(steps, cdiv(rest * steps, std::min(clusters, rest * 4)) + SHARE_STEPS) : 0;
-  double best = (double)(pair_tiles / clusters * steps + last) * 512 + 8000;
-  Plan plan{0, 1};
-  int nt = p.M <= 16 ? 16 : (p.M <= 32 ? 32 : (p.M <= 64 ? 64 : 128));
-  if (q_mn && nt < 64) nt = 64;
-  const int64_t tiles = cdiv(p.N, 128) * cdiv(p.M, nt);
-  const double step = std::max(2.0 * nt, (TILE + nt * 128) / 40.0);
-  for (int ranks = 1; ranks <= 8 && ranks <= steps; ranks *= 2) {
-    const double waves = (double)cdiv(tiles * ranks, ctx->sm_count);
-    const double t = waves * ((double)cdiv(steps, ranks) * step + 4000 + (ranks > 1 ? 2000 + 16 * nt : 0)) + 4000;
-    if (t < best) { best = t; plan = {nt, ranks}; }
+
+// split_kernel with NT rows: as many CTAs per tile as still run at once, and the
+// time that takes, fitted to 48..1024 rows through 512 x 784 to 16384 x 4096.
+template <typename T, int MODE, int NT>
+static orca_status consider(orca_ctx* ctx, const Params& p, int64_t steps, Plan* best) {
+  int fits[4];
+  ORCA_TRY((split_fits<T, MODE, NT>(ctx, fits)));
+  constexpr double STEP = NT == 16 ? 0.27 : (NT == 32 ? 0.28 : (NT == 64 ? 0.29 : 0.31));
+  const int64_t tiles = cdiv(p.N, 128) * cdiv(p.M, NT);
+  const double hbm = (p.pairs == 1 ? 2.0 : 6.0) * ((double)p.M + (double)p.N) * (double)p.K / 5.5e6 + 3.0;
+  for (int i = 0; i < 4 && (1 << i) <= steps; ++i) {
+    const int ranks = 1 << i;
+    // With 16 rows two CTAs fit an SM; that hides their ends, it does not add bandwidth.
+    const int64_t at_once = std::min<int64_t>(fits[i], std::max(1, ctx->sm_count / ranks));
+    const double us = std::max(
+        hbm, (double)cdiv(tiles, at_once) * ((double)cdiv(steps, ranks) * STEP + (NT == 128 ? 3.0 : 1.0)) + 6.3 + 0.05 * ranks);
+    if (us < best->us) *best = Plan{NT, ranks, us};
   }
-  return plan;
+  return ORCA_OK;
+}
+
+template <typename T, int MODE>
+static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, Plan* plan) {
+  const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256), n = ctx->sm_count / 2;
+  share(tiles % n, steps, n, &plan->us);
+  plan->us += (double)(tiles / n * steps) * PAIR_STEP + 8.0;
+  if constexpr (MODE != DW) {
+    if (p.M <= 16) return consider<T, MODE, 16>(ctx, p, steps, plan);
+    if (p.M <= 32) return consider<T, MODE, 32>(ctx, p, steps, plan);
+  }
+  ORCA_TRY((consider<T, MODE, 64>(ctx, p, steps, plan)));
+  return p.M > 64 ? consider<T, MODE, 128>(ctx, p, steps, plan) : ORCA_OK;
 }
 
 template <typename T, int MODE>
@@ -904,16 +1038,17 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   const int64_t steps = cdiv(p.K, BK) * p.pairs;
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
   p.chunk = dtype == ORCA_F32 ? CHUNK_F32 : (MODE == DW && p.e.out_f32 ? CHUNK_DW : (int)steps);
-  const Plan plan = choose(ctx, p, steps, p.a_mn != 0);
-  CUtensorMap ma, mb;
-  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : (plan.nt ? plan.nt : ROWS)));
-  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
+  Plan plan;
+  ORCA_TRY((choose<T, MODE>(ctx, p, steps, &plan)));
   if constexpr (MODE != DW) {
-    if (plan.nt == 16) return launch_split<T, MODE, 16>(ctx, mb, ma, p, plan.ranks);
-    if (plan.nt == 32) return launch_split<T, MODE, 32>(ctx, mb, ma, p, plan.ranks);
+    if (plan.nt == 16) return launch_split<T, MODE, 16>(ctx, a, b, planes, p, plan.ranks);
+    if (plan.nt == 32) return launch_split<T, MODE, 32>(ctx, a, b, planes, p, plan.ranks);
   }
-  if (plan.nt == 64) return launch_split<T, MODE, 64>(ctx, mb, ma, p, plan.ranks);
-  if (plan.nt == 128) return launch_split<T, MODE, 128>(ctx, mb, ma, p, plan.ranks);
+  if (plan.nt == 64) return launch_split<T, MODE, 64>(ctx, a, b, planes, p, plan.ranks);
+  if (plan.nt == 128) return launch_split<T, MODE, 128>(ctx, a, b, planes, p, plan.ranks);
+  CUtensorMap ma, mb;
+  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : ROWS));
+  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
   return launch_pair<T, MODE>(ctx, ma, mb, p);
 }
 
