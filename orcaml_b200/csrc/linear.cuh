@@ -6,6 +6,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace orca {
@@ -370,7 +372,7 @@ __device__ __forceinline__ void epilogue(const Epilogue& e, int64_t row, int64_t
 // that the 16-byte accesses of a warp cover whole rows of the block (64 or 128
 // bytes, full sectors) instead of one piece in each of 32 rows.  16-byte pieces
 // are placed at (piece ^ f(row)), free of bank conflicts both ways.
-constexpr int BLOCK_SMEM = 32 * 32 * 4;
+constexpr int BLOCK_SMEM = 32 * 32 * 4;       // 16-bit types need half
 
 __device__ __forceinline__ uint4 lds_v4(uint32_t a) {
   uint4 v;
@@ -434,6 +436,58 @@ __device__ __forceinline__ void block_load_f32(const T* p, int64_t ld, int rows,
   for (int i = 0; i < 32; ++i) v[i] = to_f32(u.e[i]);
 }
 
+// Elements as 32-bit words: 4 columns of T in 2 words (F32: 4).
+template <typename T> __device__ __forceinline__ void words_to_f32(const uint32_t* w, float (&v)[4]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(w[j]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __half2float(__ushort_as_half((unsigned short)(w[j / 2] >> (16 * (j % 2)))));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(j % 2 ? w[j / 2] & 0xffff0000u : w[j / 2] << 16);
+  }
+}
+template <typename T> __device__ __forceinline__ void f32_to_words(const float (&v)[4], uint32_t* w) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __float_as_uint(v[j]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      w[j] = (uint32_t)__half_as_ushort(__float2half_rn(v[2 * j])) |
+             (uint32_t)__half_as_ushort(__float2half_rn(v[2 * j + 1])) << 16;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      w[j] = (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v[2 * j])) |
+             (uint32_t)__bfloat16_as_ushort(__float2bfloat16_rn(v[2 * j + 1])) << 16;
+  }
+}
+// v *= act'(x) and x = act(x) in T, four columns at a time: x comes as codes or as
+// the words of T, and is never 32 registers more.
+template <typename T, int ACT>
+__device__ __forceinline__ void slope_block(const uint32_t (&codes)[8], bool packed, float down,
+                                            uint32_t (&x)[8 * sizeof(T)], float (&v)[32]) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float z[4];
+    if (packed) ckpt_values(codes[i], down, z);
+    else words_to_f32<T>(x + i * (int)sizeof(T), z);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[4 * i + j] *= act_slope<ACT>(z[j]);
+      z[j] = act_value<ACT>(z[j]);
+    }
+    f32_to_words<T>(z, x + i * (int)sizeof(T));
+  }
+}
+template <int P> __device__ __forceinline__ void pieces_to_words(const uint4 (&q)[P], uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) { w[4 * i] = q[i].x; w[4 * i + 1] = q[i].y; w[4 * i + 2] = q[i].z; w[4 * i + 3] = q[i].w; }
+}
+
 // The epilogue of one block: rows row0 + lane, columns col .. col + 32.  Blocks
 // that reach past the last column or whose memory is not 16-byte aligned take
 // the row-per-lane form.
@@ -449,13 +503,23 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
   const int rows = e.rows - row0 < 32 ? (int)(e.rows - row0) : 32;
   const int64_t at = row0 * e.cols + col;
   if (MODE == DW) {
-    if (e.out_f32) block_store_f32<float>((float*)e.out + at, e.cols, rows, v, smem, lane);
-    else block_store_f32<T>((T*)e.out + at, e.cols, rows, v, smem, lane);
+    if (e.out_f32) {
+      // 16 columns at a time: 2 KB of shared memory, as the 16-bit types have.
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        union { uint4 q[4]; float f[16]; } u;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) u.f[i] = v[16 * h + i];
+        block_store<4>(reinterpret_cast<uint8_t*>((float*)e.out + at + 16 * h), e.cols * 4, rows, u.q, smem, lane);
+      }
+    } else {
+      block_store_f32<T>((T*)e.out + at, e.cols, rows, v, smem, lane);
+    }
     return;
   }
-  float t[32];
   if (MODE == FWD) {
     if (e.bias) {
+      float t[32];
       load_row<T, 32>((const T*)e.bias + col, 32, true, t);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += t[i];
@@ -479,22 +543,35 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
     }
     apply_act<32>(e.act, v);
   } else if (packed || e.x) {
+    constexpr int P = 2 * (int)sizeof(T);
+    uint32_t codes[8], x[4 * P];
+    float down = 0.0f;
     if (packed) {
-      const float down = lane < rows ? ckpt_down(e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP]) : 0.0f;
-      union { uint4 q[2]; uint32_t w[8]; } u;
-      block_load<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) ckpt_values(u.w[i], down, t + 4 * i);
+      if (lane < rows) down = ckpt_down(e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP]);
+      uint4 q[2];
+      block_load<2>(e.codes + at, e.cols, rows, q, smem, lane);
+      pieces_to_words<2>(q, codes);
     } else {
-      block_load_f32<T>((const T*)e.x + at, e.cols, rows, t, smem, lane);
+      uint4 q[P];
+      block_load<P>(reinterpret_cast<const uint8_t*>((const T*)e.x + at), e.cols * (int64_t)sizeof(T), rows, q, smem, lane);
+      pieces_to_words<P>(q, x);
     }
-    mul_slope<32>(e.act, t, v);
+    switch (e.act) {
+      case ORCA_ACT_RELU: slope_block<T, ORCA_ACT_RELU>(codes, packed, down, x, v); break;
+      case ORCA_ACT_GELU: slope_block<T, ORCA_ACT_GELU>(codes, packed, down, x, v); break;
+      case ORCA_ACT_GELU_TANH: slope_block<T, ORCA_ACT_GELU_TANH>(codes, packed, down, x, v); break;
+      case ORCA_ACT_SILU: slope_block<T, ORCA_ACT_SILU>(codes, packed, down, x, v); break;
+      default: slope_block<T, ORCA_ACT_NONE>(codes, packed, down, x, v);
+    }
     if (e.a) {
-      apply_act<32>(e.act, t);
-      block_store_f32<T>((T*)e.a + at, e.cols, rows, t, smem, lane);
+      uint4 q[P];
+#pragma unroll
+      for (int i = 0; i < P; ++i) q[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+      block_store<P>(reinterpret_cast<uint8_t*>((T*)e.a + at), e.cols * (int64_t)sizeof(T), rows, q, smem, lane);
     }
   }
   if (e.residual) {
+    float t[32];
     block_load_f32<T>((const T*)e.residual + at, e.cols, rows, t, smem, lane);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] += t[i];

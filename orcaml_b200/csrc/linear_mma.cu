@@ -127,8 +127,9 @@ struct Params {
   int pairs;               // plane pairs: 1, or F32_PAIRS
   int chunk;               // steps per accumulation chunk
   int group_m;             // tile rows per raster group
-  int64_t full;            // pair_kernel: tiles [0, full) are whole, one cluster each
+  int full;                // pair_kernel: tiles [0, full) are whole, one cluster each
   int tail;                // ... the rest is shared by the first `tail` clusters (0: no rest)
+  uint32_t shared;         // ... its steps, all tiles together
   float* parts;            // ... their partial sums and arrival counters
   int* arrived;
   int* dev_err;
@@ -157,12 +158,11 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
   }
 }
 
-__device__ __forceinline__ void tile_at(int64_t tile, int64_t num_m, int64_t num_n, int group_m,
-                                        int64_t& tm, int64_t& tn) {
-  const int64_t size = (int64_t)group_m * num_n;
-  const int64_t first = tile / size * group_m;
-  const int64_t gm = num_m - first < group_m ? num_m - first : group_m;
-  const int64_t r = tile % size;
+__device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int group_m, int& tm, int& tn) {
+  const int size = group_m * num_n;           // at most the tiles: below 2^31
+  const int first = tile / size * group_m;
+  const int gm = num_m - first < group_m ? num_m - first : group_m;
+  const int r = tile % size;
   tm = first + r % gm;
   tn = r / gm;
 }
@@ -171,17 +171,19 @@ __device__ __forceinline__ void tile_at(int64_t tile, int64_t num_m, int64_t num
 // equal share of the steps of the tiles that do not fill a last round, which
 // may end one tile, cover some and begin another.
 struct Work {
-  int64_t cluster, nclusters, full, next, pos, end;
-  int steps;
-  __device__ Work(const Params& p, int64_t c, int64_t n, int64_t tiles, int steps_)
-      : cluster(c), nclusters(n), full(p.full), next(c), pos(0), end(0), steps(steps_) {
-    if (p.tail && c < p.tail) {
-      const int64_t total = (tiles - full) * steps;
-      pos = total * c / p.tail;
-      end = total * (c + 1) / p.tail;
+  int next, nclusters, full, steps;
+  uint32_t pos, end;              // of the shared steps, counted through the tiles
+  __device__ Work(const Params& p, int c, int n, int steps_)
+      : next(c), nclusters(n), full(p.full), steps(steps_), pos(0), end(0) {
+    if (c < p.tail) {
+      pos = first_step(p, c);
+      end = first_step(p, c + 1);
     }
   }
-  __device__ bool get(int64_t& tile, int& begin, int& stop) {
+  static __device__ uint32_t first_step(const Params& p, int c) {
+    return (uint32_t)((uint64_t)p.shared * (uint32_t)c / (uint32_t)p.tail);
+  }
+  __device__ bool get(int& tile, int& begin, int& stop) {
     if (next < full) {
       tile = next;
       next += nclusters;
@@ -190,11 +192,11 @@ struct Work {
       return true;
     }
     if (pos >= end) return false;
-    const int64_t t = pos / steps;
-    begin = (int)(pos - t * steps);
-    stop = end - pos < steps - begin ? begin + (int)(end - pos) : steps;
-    tile = full + t;
-    pos += stop - begin;
+    const uint32_t t = pos / (uint32_t)steps;
+    begin = (int)(pos - t * (uint32_t)steps);
+    stop = end - pos < (uint32_t)(steps - begin) ? begin + (int)(end - pos) : steps;
+    tile = full + (int)t;
+    pos += (uint32_t)(stop - begin);
     return true;
   }
 };
@@ -207,53 +209,72 @@ struct Work {
 // whoever is last -- and finishes it.  Nobody waits for anybody.  Each epilogue
 // warp does this for its own 32 x 128 part.
 //
-// Roles: warp 0 loads, warp 1 (of the even CTA) issues the MMAs, warps 2-9
-// drain one of two 256-column accumulators while the MMAs fill the other.  The
-// even CTA's full barrier counts both CTAs' bytes; the MMA's commits free the
-// stage and publish the accumulator in both.  For F32 results the accumulator
-// is emptied every `chunk` steps into F32 registers.  Every wait is bounded; a role that gives up raises the abort flag of
-// both CTAs, and both pass the same two cluster barriers in every case.
-constexpr int EPI_WARPS = 8;
-constexpr int PAIR_THREADS = 64 + 32 * EPI_WARPS;
-constexpr int PAIR_STAGES = 6;
-constexpr int PAIR_STAGE = 2 * TILE;                     // A and B, this CTA's halves
-constexpr int PAIR_SMEM = PAIR_STAGES * PAIR_STAGE + EPI_WARPS * BLOCK_SMEM + 1024 + 256;
-static_assert(PAIR_SMEM <= 232448, "shared memory of one CTA");
+// Roles: warp 0 loads, warp 1 (of the even CTA) issues the MMAs, the other warps
+// drain the accumulators.  The even CTA's full barrier counts both CTAs' bytes;
+// the MMA's commits free the stage and publish the accumulator in both.  Every
+// wait is bounded; a role that gives up raises the abort flag of both CTAs, and
+// both pass the same two cluster barriers in every case.
+//
+// HALVES = 1: 256 x 256 tiles, two accumulators of 256 columns, one filled while 8
+// warps drain the other; for F32 results it is emptied every `chunk` steps into
+// F32 registers.
+// HALVES = 2: 512 x 256 tiles, both accumulators filled together from one tile of
+// B: a quarter fewer bytes from L2 and through shared memory per product, which
+// under the power limit are what is left to save.  The drain is not hidden, so 16
+// warps do it, each half being refilled as soon as it is empty.
+template <int HALVES> struct Shape {
+  static constexpr int EPI_WARPS = 8 * HALVES;
+  static constexpr int THREADS = 64 + 32 * EPI_WARPS;
+  static constexpr int STAGES = HALVES == 1 ? 6 : 4;
+  static constexpr int STAGE = (HALVES + 1) * TILE;         // A tiles, B tile: this CTA's rows
+  static constexpr int BLOCK = BLOCK_SMEM / HALVES;
+  static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * BLOCK + 1024 + 256;
+  static constexpr int M = 256 * HALVES;
+  static constexpr int BLOCKS = 4 / HALVES;                 // 32-column blocks of a half per warp
+  static constexpr int64_t PART_FLOATS = M * 256;           // one piece of a tile
+  static constexpr int ARRIVALS = 2 * EPI_WARPS;            // counters of a tile
+  static_assert(SMEM <= 232448, "shared memory of one CTA");
+};
 constexpr int ACC_COLS = 256;
-constexpr int64_t PART_FLOATS = 256 * 256;               // one piece: two CTAs of 128 x 256
-constexpr int ARRIVALS = 2 * EPI_WARPS;                  // counters of a tile
 
-template <typename T, int MODE>
-__global__ void __launch_bounds__(PAIR_THREADS, 1)
+// mbar_wait by a whole warp: one answer for all lanes.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* dev_err,
+                                          unsigned sleep_ns = 0) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, dev_err, sleep_ns));
+}
+
+template <typename T, int MODE, int HALVES>
+__global__ void __launch_bounds__(Shape<HALVES>::THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ Params p) {
+  using S = Shape<HALVES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + PAIR_STAGES * PAIR_STAGE + EPI_WARPS * BLOCK_SMEM);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::STAGES * S::STAGE + S::EPI_WARPS * S::BLOCK);
   uint64_t* full_bar = bars;                              // (even) both CTAs' bytes
-  uint64_t* empty_bar = bars + PAIR_STAGES;
-  uint64_t* tfull_bar = bars + 2 * PAIR_STAGES;           // [2]
-  uint64_t* tempty_bar = bars + 2 * PAIR_STAGES + 2;      // [2] (even)
-  uint64_t* drain_bar = bars + 2 * PAIR_STAGES + 4;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * PAIR_STAGES + 5);
+  uint64_t* empty_bar = bars + S::STAGES;
+  uint64_t* tfull_bar = bars + 2 * S::STAGES;           // [2]
+  uint64_t* tempty_bar = bars + 2 * S::STAGES + 2;      // [2] (even)
+  uint64_t* drain_bar = bars + 2 * S::STAGES + 4;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * S::STAGES + 5);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const uint32_t rank = cluster_ctarank();
   const bool even = rank == 0;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int64_t num_m = cdiv(p.M, 256), num_n = cdiv(p.N, 256), tiles = num_m * num_n;
-  const int64_t cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
+  const int num_m = (int)cdiv(p.M, S::M), num_n = (int)cdiv(p.N, 256);
+  const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   const int steps = (int)cdiv(p.K, BK) * p.pairs;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < PAIR_STAGES; ++s) {
+    for (int s = 0; s < S::STAGES; ++s) {
       mbar_init(&full_bar[s], 1);
       mbar_init(&empty_bar[s], 1);
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&tfull_bar[a], 1);
-      mbar_init(&tempty_bar[a], 2 * EPI_WARPS);
+      mbar_init(&tempty_bar[a], 2 * S::EPI_WARPS);
     }
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
@@ -281,19 +302,19 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
-      int issued[PAIR_STAGES];
-      for (int s = 0; s < PAIR_STAGES; ++s) issued[s] = -1;
+      int issued[S::STAGES];
+      for (int s = 0; s < S::STAGES; ++s) issued[s] = -1;
       uint64_t last_issue = 0;
       bool ok = true;
-      Work work(p, cluster, nclusters, tiles, steps);
-      int64_t tile;
+      Work work(p, cluster, nclusters, steps);
+      int tile;
       int begin, stop;
       while (ok && work.get(tile, begin, stop)) {
-        int64_t tm, tn;
+        int tm, tn;
         tile_at(tile, num_m, num_n, p.group_m, tm, tn);
-        const int64_t row = tm * 256 + (int64_t)rank * 128, col = tn * 256 + (int64_t)rank * 128;
+        const int row = tm * S::M + (int)rank * 128, col = tn * 256 + (int)rank * 128;
         int pair = begin % p.pairs;
-        int64_t k0 = (int64_t)(begin / p.pairs) * BK;
+        int k0 = begin / p.pairs * BK;
         for (int it = begin; it < stop; ++it) {
           const int pa = p.pairs == 1 ? 0 : (int)(PAIR_A >> (4 * pair)) & 15;
           const int pb = p.pairs == 1 ? 0 : (int)(PAIR_B >> (4 * pair)) & 15;
@@ -301,19 +322,23 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             ok = false;
             break;
           }
-          uint8_t* a_dst = smem + stage * PAIR_STAGE;
+          uint8_t* a_dst = smem + stage * S::STAGE;
           if (even) {
-            mbar_arrive_expect_tx(&full_bar[stage], 2 * PAIR_STAGE);
-            load_tile(a_dst, &map_a, &full_bar[stage], p.a_mn, ROWS, row, k0, pa);
-            load_tile(a_dst + TILE, &map_b, &full_bar[stage], p.b_mn, ROWS, col, k0, pb);
+            mbar_arrive_expect_tx(&full_bar[stage], 2 * S::STAGE);
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+              load_tile(a_dst + h * TILE, &map_a, &full_bar[stage], p.a_mn, ROWS, row + h * 256, k0, pa);
+            load_tile(a_dst + HALVES * TILE, &map_b, &full_bar[stage], p.b_mn, ROWS, col, k0, pb);
             issued[stage] = (int)phase;
           } else {
             const uint32_t bar = cluster_addr(&full_bar[stage], 0);
-            load_tile_pair(a_dst, &map_a, bar, p.a_mn, ROWS, row, k0, pa);
-            load_tile_pair(a_dst + TILE, &map_b, bar, p.b_mn, ROWS, col, k0, pb);
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+              load_tile_pair(a_dst + h * TILE, &map_a, bar, p.a_mn, ROWS, row + h * 256, k0, pa);
+            load_tile_pair(a_dst + HALVES * TILE, &map_b, bar, p.b_mn, ROWS, col, k0, pb);
             last_issue = global_ns();
           }
-          if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
+          if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
           if (++pair == p.pairs) { pair = 0; k0 += BK; }
         }
       }
@@ -326,7 +351,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           }
       }
       // Never leave with copies in flight into this CTA's shared memory.
-      for (int s = 0; s < PAIR_STAGES; ++s) {
+      for (int s = 0; s < S::STAGES; ++s) {
         if (issued[s] < 0) continue;
         const uint64_t t0 = global_ns();
         while (!mbar_try_wait(&full_bar[s], (uint32_t)issued[s]) && global_ns() - t0 < kWaitLimitNs) {
@@ -336,40 +361,48 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   } else if (warp == 1) {
     if (even) {
       const uint32_t id = idesc(p.bf16, p.a_mn, p.b_mn, 256, 256);
-      const uint32_t a0 = desc_lo(smem_u32(smem), p.a_mn), b0 = desc_lo(smem_u32(smem) + TILE, p.b_mn);
+      const uint32_t a0 = desc_lo(smem_u32(smem), p.a_mn), b0 = desc_lo(smem_u32(smem) + HALVES * TILE, p.b_mn);
       const uint32_t a_step = desc_step(p.a_mn), b_step = desc_step(p.b_mn);
       int stage = 0;
       uint32_t phase = 0, chunks = 0;
       bool ok = true;
-      Work work(p, cluster, nclusters, tiles, steps);
-      int64_t tile;
+      Work work(p, cluster, nclusters, steps);
+      int tile;
       int begin, stop;
       while (ok && work.get(tile, begin, stop)) {
         int in_chunk = 0;
         for (int it = begin; it < stop; ++it) {
-          const int buf = (int)(chunks & 1u);
+          // HALVES = 1: this chunk's accumulator; HALVES = 2: both, chunk = tile.
+          const int buf = HALVES == 1 ? (int)(chunks & 1u) : 0;
+          const uint32_t use = HALVES == 1 ? chunks >> 1 : chunks;
           if (in_chunk == 0) {
-            if (!mbar_wait(&tempty_bar[buf], ((chunks >> 1) & 1u) ^ 1u, abort_flag, p.dev_err)) {
-              ok = false;
-              break;
-            }
+            if (!warp_wait(&tempty_bar[buf], (use & 1u) ^ 1u, abort_flag, p.dev_err)) { ok = false; break; }
             tc_fence_after();
           }
-          if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) { ok = false; break; }
+          if (!warp_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) { ok = false; break; }
           tc_fence_after();
-          const uint32_t at = (uint32_t)(stage * (PAIR_STAGE >> 4));
-          const uint32_t d = tmem + (uint32_t)(buf * ACC_COLS);
+          const uint32_t at = (uint32_t)(stage * (S::STAGE >> 4));
           const bool last = in_chunk + 1 == p.chunk || it == stop - 1;
-          if (elect_one()) {
 #pragma unroll
-            for (int s = 0; s < BK / 16; ++s)
-              mma_f16_pair(d, desc(a0 + at + s * a_step), desc(b0 + at + s * b_step), id,
-                           (in_chunk | s) ? 1u : 0u);
-            commit_both(&empty_bar[stage]);
-            if (last) commit_both(&tfull_bar[buf]);
+          for (int h = 0; h < HALVES; ++h) {
+            if (h == 1 && in_chunk == 0) {
+              if (!warp_wait(&tempty_bar[1], (use & 1u) ^ 1u, abort_flag, p.dev_err)) { ok = false; break; }
+              tc_fence_after();
+            }
+            const uint32_t d = tmem + (uint32_t)((buf + h) * ACC_COLS), ah = a0 + at + h * (TILE >> 4);
+            if (elect_one()) {
+#pragma unroll
+              for (int s = 0; s < BK / 16; ++s)
+                mma_f16_pair(d, desc(ah + s * a_step), desc(b0 + at + s * b_step), id, (in_chunk | s) ? 1u : 0u);
+              if (h == HALVES - 1) {
+                commit_both(&empty_bar[stage]);
+                if (last) commit_both(&tfull_bar[buf]);
+              }
+            }
+            __syncwarp();
           }
-          __syncwarp();
-          if (++stage == PAIR_STAGES) { stage = 0; phase ^= 1u; }
+          if (!ok) break;
+          if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
           ++in_chunk;
           if (last) {
             ++chunks;
@@ -384,37 +417,34 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       }
     }
   } else {
-    // Warp w reads TMEM lanes [32 * (w % 4), +32) and columns [128 * half, +128).
-    const int quarter = warp & 3, half = (warp - 2) / 4;
-    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)(half * 128);
+    // Warp w reads TMEM lanes [32 * (w % 4), +32) and, of each half, the columns
+    // [32 * BLOCKS * ((w - 2) / 4), +32 * BLOCKS).
+    const int quarter = warp & 3, first_col = (warp - 2) / 4 * (32 * S::BLOCKS);
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)first_col;
     const uint32_t tempty[2] = {cluster_addr(&tempty_bar[0], 0), cluster_addr(&tempty_bar[1], 0)};
-    const uint32_t block = smem_u32(smem + PAIR_STAGES * PAIR_STAGE + (warp - 2) * BLOCK_SMEM);
+    const uint32_t block = smem_u32(smem + S::STAGES * S::STAGE + (warp - 2) * S::BLOCK);
     uint32_t chunks = 0;
     bool ok = true;
-    Work work(p, cluster, nclusters, tiles, steps);
-    int64_t tile;
+    Work work(p, cluster, nclusters, steps);
+    int tile;
     int begin, stop;
     while (ok && work.get(tile, begin, stop)) {
-      int64_t tm, tn;
+      int tm, tn;
       tile_at(tile, num_m, num_n, p.group_m, tm, tn);
-      const int64_t row = tm * 256 + (int64_t)rank * 128 + quarter * 32;
-      const int64_t col = tn * 256 + half * 128;
+      const int row = tm * S::M + (int)rank * 128 + quarter * 32;
+      const int col = tn * 256 + first_col;
       const bool piece = stop - begin < steps;
-      // This warp's part of a piece: blocks of 32 columns, four columns of each lane
-      // side by side.
-      const int64_t my_part = (int64_t)((rank * EPI_WARPS + warp - 2) * 4) * 1024 + lane * 4;
-      float* mine = p.parts + (cluster * 2 + (begin == 0)) * PART_FLOATS + my_part;
       const int nchunks = (stop - begin + p.chunk - 1) / p.chunk;
       auto release = [&](int buf) {
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_remote(tempty[buf]);
       };
-      int buf = (int)(chunks & 1u);
-      ok = mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64);
+      int buf = HALVES == 1 ? (int)(chunks & 1u) : 0;
+      ok = warp_wait(&tfull_bar[buf], (HALVES == 1 ? chunks >> 1 : chunks) & 1u, abort_flag, p.dev_err, 64);
       tc_fence_after();
       ++chunks;
-      if (ok && nchunks > 1) {
+      if (HALVES == 1 && ok && nchunks > 1) {
         // The sums go back to the last chunk's accumulator, where the epilogue finds
         // them block by block as it finds those of a single chunk: holding 128 sums
         // in registers through the epilogue spilled them, and with this much
@@ -433,7 +463,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           if (c == nchunks - 1) break;
           release(buf);
           buf = (int)(chunks & 1u);
-          ok = mbar_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64);
+          ok = warp_wait(&tfull_bar[buf], (chunks >> 1) & 1u, abort_flag, p.dev_err, 64);
           if (!ok) break;
           tc_fence_after();
           ++chunks;
@@ -445,82 +475,72 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
       }
       if (!ok) break;
-      int64_t first = 0;
-      int count = 0;
+      int first = 0, count = 0;
+      // This warp's part of a piece: blocks of 32 columns, four columns of each lane
+      // side by side.
+      const int my_part = (int)((rank * S::EPI_WARPS + warp - 2) * 4) * 1024 + lane * 4;
       if (piece) {
+        float* mine = p.parts + (int64_t)(cluster * 2 + (begin == 0)) * S::PART_FLOATS + my_part;
 #pragma unroll 1
         for (int q = 0; q < 4; ++q) {
           float v[32];
-          tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
+          tmem_ld_32x32b_x32(lanes + (uint32_t)((buf + q / S::BLOCKS) * ACC_COLS + q % S::BLOCKS * 32), v);
 #pragma unroll
           for (int j = 0; j < 8; ++j)
             __stcg(reinterpret_cast<float4*>(mine + (q * 8 + j) * 128),
                    make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
         }
         release(buf);
+        if (HALVES == 2) release(1);
         // Clusters first .. first + count - 1 share this tile.
-        const int64_t t = tile - p.full, total = (tiles - p.full) * steps;
-        first = t * steps * p.tail / total;
-        while (total * (first + 1) / p.tail <= t * steps) ++first;
-        while (total * first / p.tail > t * steps) --first;
-        int64_t lastc = first;
-        while (total * (lastc + 1) / p.tail < (t + 1) * steps) ++lastc;
-        count = (int)(lastc - first) + 1;
+        const int t = tile - p.full;
+        const uint32_t t0 = (uint32_t)t * (uint32_t)steps, t1 = t0 + (uint32_t)steps;
+        first = (int)((uint64_t)t0 * (uint32_t)p.tail / p.shared);
+        while (Work::first_step(p, first + 1) <= t0) ++first;
+        while (Work::first_step(p, first) > t0) --first;
+        count = 1;
+        while (Work::first_step(p, first + count) < t1) ++count;
         __threadfence();
         __syncwarp();
         int before = 0;
-        if (lane == 0) before = atomicAdd(p.arrived + t * ARRIVALS + rank * EPI_WARPS + warp - 2, 1);
+        if (lane == 0) before = atomicAdd(p.arrived + t * S::ARRIVALS + rank * S::EPI_WARPS + warp - 2, 1);
         before = __shfl_sync(0xffffffffu, before, 0);
         if (before != count - 1) continue;
         __threadfence();
       }
 #pragma unroll 1
       for (int q = 0; q < 4; ++q) {
-        if (col + q * 32 >= p.N) break;
+        // Blocks of half 0, then of half 1.
+        const int h = q / S::BLOCKS;
+        const int c0 = col + q % S::BLOCKS * 32;
         float v[32];
         if (piece) {
-          // Two pieces' loads in flight; added in the pieces' order.
-          const float* part = p.parts + (first * 2 + 1) * PART_FLOATS + my_part + q * 1024;
-          const float* next = p.parts + (first + 1) * 2 * PART_FLOATS + my_part + q * 1024;
-          float4 x[8], y[8];
+          // The pieces in their order, the next one's loads behind this one's adds.
+          const float* part = p.parts + (int64_t)(first * 2 + 1) * S::PART_FLOATS + my_part + q * 1024;
+          float4 x[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = __ldcg(reinterpret_cast<const float4*>(part + j * 128));
 #pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            v[4 * j] = x[j].x; v[4 * j + 1] = x[j].y; v[4 * j + 2] = x[j].z; v[4 * j + 3] = x[j].w;
-          }
-          for (int c = 1; c < count; c += 2) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) x[j] = __ldcg(reinterpret_cast<const float4*>(next + j * 128));
-            next += 2 * PART_FLOATS;
-            if (c + 1 < count) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) y[j] = __ldcg(reinterpret_cast<const float4*>(next + j * 128));
-              next += 2 * PART_FLOATS;
-            }
+          for (int j = 0; j < 32; ++j) v[j] = 0.0f;
+          part += S::PART_FLOATS;             // (first + 1, 0), then every second
+          for (int c = 1;; ++c) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               v[4 * j] = __fadd_rn(v[4 * j], x[j].x);
               v[4 * j + 1] = __fadd_rn(v[4 * j + 1], x[j].y);
               v[4 * j + 2] = __fadd_rn(v[4 * j + 2], x[j].z);
               v[4 * j + 3] = __fadd_rn(v[4 * j + 3], x[j].w);
+              if (c < count) x[j] = __ldcg(reinterpret_cast<const float4*>(part + j * 128));
             }
-            if (c + 1 < count) {
-#pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                v[4 * j] = __fadd_rn(v[4 * j], y[j].x);
-                v[4 * j + 1] = __fadd_rn(v[4 * j + 1], y[j].y);
-                v[4 * j + 2] = __fadd_rn(v[4 * j + 2], y[j].z);
-                v[4 * j + 3] = __fadd_rn(v[4 * j + 3], y[j].w);
-              }
-            }
+            if (c == count) break;
+            part += 2 * S::PART_FLOATS;
           }
         } else {
-          tmem_ld_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), v);
+          tmem_ld_32x32b_x32(lanes + (uint32_t)((buf + h) * ACC_COLS + q % S::BLOCKS * 32), v);
+          if (q % S::BLOCKS == S::BLOCKS - 1) release(buf + h);     // read out: refill it
         }
-        block_epilogue<T, MODE>(p.e, row, col + q * 32, v, block, lane);
+        if (c0 < p.N) block_epilogue<T, MODE>(p.e, row + h * 256, c0, v, block, lane);
       }
-      if (!piece) release(buf);
     }
     if (!ok) raise_abort();
   }
@@ -645,10 +665,10 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
       for (int it = begin; it < end; ++it) {
         const int buf = (int)(chunks & 1u);
         if (in_chunk == 0) {
-          if (!mbar_wait(&tempty_bar[buf], ((chunks >> 1) & 1u) ^ 1u, abort_flag, p.dev_err)) break;
+          if (!warp_wait(&tempty_bar[buf], ((chunks >> 1) & 1u) ^ 1u, abort_flag, p.dev_err)) break;
           tc_fence_after();
         }
-        if (!mbar_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) break;
+        if (!warp_wait(&full_bar[stage], phase, abort_flag, p.dev_err)) break;
         tc_fence_after();
         const uint32_t at = (uint32_t)(stage * (STAGE >> 4));
         const bool last = in_chunk + 1 == p.chunk || it == end - 1;
@@ -680,7 +700,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
     for (int j = 0; j < NT; ++j) acc[j] = 0.0f;
     for (int c = 0; c < nchunks; ++c) {
       const int buf = c & 1;
-      if (!mbar_wait(&tfull_bar[buf], (uint32_t)(c >> 1) & 1u, abort_flag, p.dev_err)) break;
+      if (!warp_wait(&tfull_bar[buf], (uint32_t)(c >> 1) & 1u, abort_flag, p.dev_err)) break;
       tc_fence_after();
 #pragma unroll
       for (int q = 0; q < NT / 16; ++q) {
@@ -856,10 +876,12 @@ static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int b
 }
 
 // ---------------------------------------------------------------- plans
-// Times in microseconds that the choices below compare, measured at 1.9 GHz: a
-// pair step; and what sharing a tile among `parts` clusters costs (each leaves its
+// Times in microseconds that the choices below compare, measured: a step of a
+// tile of 256 or 512 rows (the second saves bytes: 8192 x 8192 x 8192 took 793 us
+// against 834), the drain that 512 rows do not hide, and what sharing a tile among `parts` clusters costs (each leaves its
 // sums in L2, the last one adds them).
-constexpr double PAIR_STEP = 0.42;
+static double pair_step(int halves) { return halves == 1 ? 0.44 : 0.82; }
+static double drain_cost(int mode) { return mode == DW ? 2.0 : (mode == FWD ? 5.0 : 9.0); }
 static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
 
 // The tiles beyond whole rounds of n clusters: how many clusters share them (0:
@@ -867,9 +889,10 @@ static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
 struct Tail {
   int64_t clusters, steps;
 };
-static Tail share(int64_t rest, int64_t steps, int64_t n, double* us) {
+static Tail share(int64_t rest, int64_t steps, int64_t n, int halves, double* us) {
+  const double step = pair_step(halves);
   Tail best{0, rest ? steps : 0};
-  *us = rest ? (double)steps * PAIR_STEP : 0.0;
+  *us = rest ? (double)steps * step : 0.0;
   // An equal number of clusters per tile, or all of them with ranges that cross tiles.
   for (int64_t parts = 2; rest && parts <= 5; ++parts) {
     int64_t c = rest * parts, pieces = parts;
@@ -878,7 +901,7 @@ static Tail share(int64_t rest, int64_t steps, int64_t n, double* us) {
       pieces = cdiv(n, rest) + 1;
     }
     const int64_t s = cdiv(rest * steps, c);
-    const double t = (double)s * PAIR_STEP + share_cost(pieces);
+    const double t = (double)s * step + halves * share_cost(pieces);
     if (t < *us) {
       *us = t;
       best = Tail{c, s};
@@ -889,9 +912,10 @@ static Tail share(int64_t rest, int64_t steps, int64_t n, double* us) {
 }
 
 // ---------------------------------------------------------------- launches
-template <typename T, int MODE>
+template <typename T, int MODE, int HALVES>
 static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, Params p) {
-  const auto kernel = pair_kernel<T, MODE>;
+  using S = Shape<HALVES>;
+  const auto kernel = pair_kernel<T, MODE, HALVES>;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -899,33 +923,41 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   attr[0].val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(ctx->sm_count / 2 * 2));
-  cfg.blockDim = dim3(PAIR_THREADS);
-  cfg.dynamicSmemBytes = PAIR_SMEM;
+  cfg.blockDim = dim3(S::THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   static std::atomic<int> fits[64];      // clusters that are resident at once, per device
   std::atomic<int>& fit = fits[ctx->device & 63];
   if (fit.load() == 0) {
-    ORCA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PAIR_SMEM));
+    ORCA_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     int n = 0;
     ORCA_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
     if (n < 1) return fail(ORCA_CUDA_ERROR, "no cluster of two CTAs fits on the device");
     fit.store(n);
   }
-  const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256), n = fit.load();
+  // Raster: 2048 rows by 9 tile columns are about what runs at once.  Where all of A
+  // stays in L2 (48 MB of 126), all its rows form one group and B is read once
+  // (4096 x 4096 x 16384: 404 us against 416).
+  const int64_t a_bytes = p.M * p.K * 2 * (p.pairs == 1 ? 1 : 3);
+  p.group_m = a_bytes <= (int64_t)48 << 20 ? (int)cdiv(p.M, S::M) : 2048 / S::M;
+  const int64_t tiles = cdiv(p.M, S::M) * cdiv(p.N, 256), n = fit.load();
   const int64_t steps = cdiv(p.K, BK) * p.pairs, rest = tiles % n;
   double us;
-  const Tail tail = share(rest, steps, n, &us);
-  p.full = tiles;
+  const Tail tail = share(rest, steps, n, HALVES, &us);
+  if (tiles > INT32_MAX - 4096) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
+  p.full = (int)tiles;
   p.tail = 0;
+  p.shared = 0;
   p.parts = nullptr;
   p.arrived = nullptr;
   Scratch scratch(ctx);
-  if (tail.clusters) {
-    p.full = tiles - rest;
+  if (tail.clusters && rest * steps <= INT32_MAX) {
+    p.full = (int)(tiles - rest);
+    p.shared = (uint32_t)(rest * steps);
     p.tail = (int)tail.clusters;
-    const size_t parts = (size_t)(tail.clusters * 2 * PART_FLOATS) * 4, counters = (size_t)(rest * ARRIVALS) * 4;
+    const size_t parts = (size_t)(tail.clusters * 2 * S::PART_FLOATS) * 4, counters = (size_t)(rest * S::ARRIVALS) * 4;
     ORCA_TRY(scratch.get(parts + counters));
     p.parts = (float*)scratch.p;
     p.arrived = (int*)((uint8_t*)scratch.p + parts);
@@ -995,6 +1027,7 @@ static orca_status launch_split(orca_ctx* ctx, const Planes& a, const Planes& b,
 
 struct Plan {
   int nt = 0;       // 0: pair_kernel
+  int halves = 1;   // ... with 256 or 512 rows a tile
   int ranks = 1;
   double us = 0;
 };
@@ -1014,16 +1047,24 @@ static orca_status consider(orca_ctx* ctx, const Params& p, int64_t steps, Plan*
     const int64_t at_once = std::min<int64_t>(fits[i], std::max(1, ctx->sm_count / ranks));
     const double us = std::max(
         hbm, (double)cdiv(tiles, at_once) * ((double)cdiv(steps, ranks) * STEP + (NT == 128 ? 3.0 : 1.0)) + 6.3 + 0.05 * ranks);
-    if (us < best->us) *best = Plan{NT, ranks, us};
+    if (us < best->us) *best = Plan{NT, 1, ranks, us};
   }
   return ORCA_OK;
 }
 
 template <typename T, int MODE>
 static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, Plan* plan) {
-  const int64_t tiles = cdiv(p.M, 256) * cdiv(p.N, 256), n = ctx->sm_count / 2;
-  share(tiles % n, steps, n, &plan->us);
-  plan->us += (double)(tiles / n * steps) * PAIR_STEP + 8.0;
+  const int64_t n = ctx->sm_count / 2;
+  plan->us = 1e30;
+  for (int halves = 1; halves <= 2; ++halves) {
+    // The two-accumulator tile has no F32 chunks.
+    if (halves == 2 && (std::is_same<T, float>::value || p.chunk < steps)) break;
+    const int64_t tiles = cdiv(p.M, 256 * halves) * cdiv(p.N, 256);
+    double us;
+    share(tiles % n, steps, n, halves, &us);
+    us += (double)(tiles / n * steps) * pair_step(halves) + (double)cdiv(tiles, n) * (halves == 2 ? drain_cost(MODE) : 0.0) + 8.0;
+    if (us < plan->us) *plan = Plan{0, halves, 1, us};
+  }
   if constexpr (MODE != DW) {
     if (p.M <= 16) return consider<T, MODE, 16>(ctx, p, steps, plan);
     if (p.M <= 32) return consider<T, MODE, 32>(ctx, p, steps, plan);
@@ -1049,7 +1090,10 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   CUtensorMap ma, mb;
   ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : ROWS));
   ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
-  return launch_pair<T, MODE>(ctx, ma, mb, p);
+  if constexpr (!std::is_same<T, float>::value) {
+    if (plan.halves == 2) return launch_pair<T, MODE, 2>(ctx, ma, mb, p);
+  }
+  return launch_pair<T, MODE, 1>(ctx, ma, mb, p);
 }
 
 }  // namespace lin
@@ -1064,11 +1108,6 @@ orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, in
   p.b_mn = b_mn;
   p.bf16 = dtype != ORCA_F16;
   p.pairs = dtype == ORCA_F32 ? F32_PAIRS : 1;
-  // Raster: 8 tile rows by 9 columns are about what runs at once.  Where all of A
-  // stays in L2 (48 MB of 126), all its rows form one group and B is read once
-  // (4096 x 4096 x 16384: 404 us against 416).
-  const int64_t a_bytes = M * K * 2 * (dtype == ORCA_F32 ? 3 : 1);
-  p.group_m = a_bytes <= (int64_t)48 << 20 ? (int)cdiv(M, 256) : 8;
   p.dev_err = ctx->dev_err;
   p.e = e;
 #define ORCA_MODE(MODE)                                                            \

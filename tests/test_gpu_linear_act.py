@@ -279,6 +279,22 @@ def test_forward(be, kind, m, k, n):
     fwd_case(be, TYPES[kind], m, k, n, acts[(i + 2) % 5], i % 2 == 1, keeps[(i + 1) % 3], bias=i % 3 != 0)
 
 
+# Sizes that reach every tiling: several rounds of 256- and of 512-row tiles, a
+# last round shared along the sum by two to five clusters, long sums of few
+# tiles, borders inside the tiles.
+LARGE = [(4096, 8192, 4608), (2320, 4104, 2312), (1100, 8200, 1096), (300, 16384, 520), (4100, 264, 5000),
+         (8192, 8192, 8192)]
+
+
+@pytest.mark.parametrize("m,k,n", LARGE)
+def test_forward_large(be, m, k, n):
+    i = LARGE.index((m, k, n))
+    fwd_case(be, torch.bfloat16, m, k, n, "gelu" if i % 2 else "none", i % 3 == 0, [None, "ckpt8", "z"][i % 3])
+    if m * k * n < 2 ** 36:
+        fwd_case(be, torch.float16, m, k, n, "silu", True, None)
+        fwd_case(be, torch.float32, m, k, n, "gelu_tanh", True, "z")
+
+
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
 @pytest.mark.parametrize("kind", list(TYPES))
 def test_forward_every_activation_and_keep(be, kind, act):
@@ -420,6 +436,25 @@ def test_backward(be, kind, m, k, n):
     acts = ["none", "relu", "gelu", "gelu_tanh", "silu"]
     for j, packed in enumerate((False, True)):
         bwd_case(be, TYPES[kind], m, k, n, acts[(i + j) % 5], packed, (i + j) % 2 == 0, "f32" if (i + j) % 3 else "same")
+
+
+@pytest.mark.parametrize("m,k,n", [(n, m, k) for m, k, n in LARGE])
+def test_backward_large(be, m, k, n):
+    bwd_case(be, torch.bfloat16, m, k, n, "gelu", True, True, "same")
+    bwd_case(be, torch.bfloat16, m, k, n, "none", (m + k) % 3 == 0, False, "f32")
+    if m * k * n < 2 ** 36:
+        bwd_case(be, torch.float16, m, k, n, "silu", False, True, "f32")
+        bwd_case(be, torch.float32, m, k, n, "gelu_tanh", True, True, "same")
+
+
+def test_sums_shared_by_clusters_repeat_their_bits(be):
+    t, (m, k, n) = torch.bfloat16, (1100, 8200, 1096)
+    g = gen_of(40)
+    x, w = rand(g, m, k, t=t), rand(g, k, n, scale=0.01, t=t)
+    outs = [torch.empty(m, n, dtype=t, device="cuda") for _ in range(12)]
+    for o in outs:
+        be.linear_act_fwd(sp(be, x), sp(be, w), None, m, k, n, act="gelu", out=sp(be, o))
+    assert all(torch.equal(o, outs[0]) for o in outs)
 
 
 @pytest.mark.parametrize("act", ["none", "relu", "gelu", "gelu_tanh", "silu"])
