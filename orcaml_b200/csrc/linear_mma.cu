@@ -626,6 +626,11 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  // Up to here the kernel may run beside the end of the one before it in the stream;
+  // it touches memory only once that one is complete.  Its own successor may set up
+  // from here on.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   float acc[NT];
 
   if (warp == 0) {
@@ -881,7 +886,7 @@ static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int b
 // against 834), the drain that 512 rows do not hide, and what sharing a tile among `parts` clusters costs (each leaves its
 // sums in L2, the last one adds them).
 static double pair_step(int halves) { return halves == 1 ? 0.44 : 0.82; }
-static double drain_cost(int mode) { return mode == DW ? 2.0 : (mode == FWD ? 5.0 : 9.0); }
+static double drain_cost(int mode) { return mode == DW ? 2.0 : (mode == FWD ? 7.0 : 9.0); }
 static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
 
 // The tiles beyond whole rounds of n clusters: how many clusters share them (0:
@@ -1006,11 +1011,13 @@ static orca_status launch_split(orca_ctx* ctx, const Planes& a, const Planes& b,
   CUtensorMap ma, mb;
   ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : NT));
   ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ranks;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
   const int64_t blocks = cdiv(p.N, 128) * cdiv(p.M, NT) * ranks;
   if (blocks > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
@@ -1019,7 +1026,7 @@ static orca_status launch_split(orca_ctx* ctx, const Planes& a, const Planes& b,
   cfg.dynamicSmemBytes = split_smem<NT>();
   cfg.stream = ctx->stream;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = 2;
   ORCA_CUDA_TRY(cudaLaunchKernelEx(&cfg, split_kernel<T, MODE, NT>, mb, ma, p, ranks));
   count_launch(ctx);
   return ORCA_OK;
