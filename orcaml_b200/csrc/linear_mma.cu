@@ -34,11 +34,11 @@ constexpr int F32_PAIRS = 6;
 
 // Steps (of four MMAs) per accumulation chunk of an F32 result.  The tensor core
 // adds with a few bits less than F32; a chain of L MMAs over random data is off by
-// about 9e-10 * L^1.5 of the result's norm.  F32 operands: 64 MMAs, 5e-7, what an
-// F32 chain of FMAs gives.  F32 gradients of 16-bit operands: 256 MMAs, 4e-6
+// about 9e-10 * L^1.5 of the result's norm.  F32 operands: 72 MMAs (3 blocks of 6 plane
+// products), 5e-7, what an F32 chain of FMAs gives.  F32 gradients of 16-bit operands: 256 MMAs, 4e-6
 // against the operands' own 2^-9; emptying the accumulator every 32 MMAs
 // instead cost 13 % of the product's time.
-constexpr int CHUNK_F32 = 16, CHUNK_DW = 64;
+constexpr int CHUNK_F32 = 18, CHUNK_DW = 64;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -218,15 +218,17 @@ struct Work {
 // HALVES = 1: 256 x 256 tiles, two accumulators of 256 columns, one filled while 8
 // warps drain the other; for F32 results it is emptied every `chunk` steps into
 // F32 registers.
+// F32 operands: a stage holds the three planes of both operands for a 64-deep step
+// and feeds the six plane products, so that each byte is fetched once, not twice.
 // HALVES = 2: 512 x 256 tiles, both accumulators filled together from one tile of
 // B: a quarter fewer bytes from L2 and through shared memory per product, which
 // under the power limit are what is left to save.  The drain is not hidden, so 16
 // warps do it, each half being refilled as soon as it is empty.
-template <int HALVES> struct Shape {
+template <int HALVES, int PLANES> struct Shape {
   static constexpr int EPI_WARPS = 8 * HALVES;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGES = HALVES == 1 ? 6 : 4;
-  static constexpr int STAGE = (HALVES + 1) * TILE;         // A tiles, B tile: this CTA's rows
+  static constexpr int STAGES = PLANES == 3 ? 2 : (HALVES == 1 ? 6 : 4);
+  static constexpr int STAGE = (HALVES + 1) * PLANES * TILE;   // A tiles, B tile: this CTA's rows
   static constexpr int BLOCK = BLOCK_SMEM / HALVES;
   static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * BLOCK + 1024 + 256;
   static constexpr int M = 256 * HALVES;
@@ -243,11 +245,14 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, dev_err, sleep_ns));
 }
 
+template <typename T> constexpr int plane_count() { return std::is_same<T, float>::value ? 3 : 1; }
+
 template <typename T, int MODE, int HALVES>
-__global__ void __launch_bounds__(Shape<HALVES>::THREADS, 1)
+__global__ void __launch_bounds__(Shape<HALVES, plane_count<T>()>::THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ Params p) {
-  using S = Shape<HALVES>;
+  constexpr int PLANES = plane_count<T>();
+  using S = Shape<HALVES, PLANES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -265,7 +270,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int num_m = (int)cdiv(p.M, S::M), num_n = (int)cdiv(p.N, 256);
   const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
-  const int steps = (int)cdiv(p.K, BK) * p.pairs;
+  const int steps = (int)cdiv(p.K, BK);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < S::STAGES; ++s) {
@@ -313,11 +318,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         int tm, tn;
         tile_at(tile, num_m, num_n, p.group_m, tm, tn);
         const int row = tm * S::M + (int)rank * 128, col = tn * 256 + (int)rank * 128;
-        int pair = begin % p.pairs;
-        int k0 = begin / p.pairs * BK;
         for (int it = begin; it < stop; ++it) {
-          const int pa = p.pairs == 1 ? 0 : (int)(PAIR_A >> (4 * pair)) & 15;
-          const int pb = p.pairs == 1 ? 0 : (int)(PAIR_B >> (4 * pair)) & 15;
+          const int k0 = it * BK;
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.dev_err)) {
             ok = false;
             break;
@@ -326,20 +328,25 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           if (even) {
             mbar_arrive_expect_tx(&full_bar[stage], 2 * S::STAGE);
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-              load_tile(a_dst + h * TILE, &map_a, &full_bar[stage], p.a_mn, ROWS, row + h * 256, k0, pa);
-            load_tile(a_dst + HALVES * TILE, &map_b, &full_bar[stage], p.b_mn, ROWS, col, k0, pb);
+            for (int l = 0; l < PLANES; ++l) {
+#pragma unroll
+              for (int h = 0; h < HALVES; ++h)
+                load_tile(a_dst + (l * HALVES + h) * TILE, &map_a, &full_bar[stage], p.a_mn, ROWS, row + h * 256, k0, l);
+              load_tile(a_dst + (PLANES * HALVES + l) * TILE, &map_b, &full_bar[stage], p.b_mn, ROWS, col, k0, l);
+            }
             issued[stage] = (int)phase;
           } else {
             const uint32_t bar = cluster_addr(&full_bar[stage], 0);
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-              load_tile_pair(a_dst + h * TILE, &map_a, bar, p.a_mn, ROWS, row + h * 256, k0, pa);
-            load_tile_pair(a_dst + HALVES * TILE, &map_b, bar, p.b_mn, ROWS, col, k0, pb);
+            for (int l = 0; l < PLANES; ++l) {
+#pragma unroll
+              for (int h = 0; h < HALVES; ++h)
+                load_tile_pair(a_dst + (l * HALVES + h) * TILE, &map_a, bar, p.a_mn, ROWS, row + h * 256, k0, l);
+              load_tile_pair(a_dst + (PLANES * HALVES + l) * TILE, &map_b, bar, p.b_mn, ROWS, col, k0, l);
+            }
             last_issue = global_ns();
           }
           if (++stage == S::STAGES) { stage = 0; phase ^= 1u; }
-          if (++pair == p.pairs) { pair = 0; k0 += BK; }
         }
       }
       if (!ok) {
@@ -361,7 +368,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   } else if (warp == 1) {
     if (even) {
       const uint32_t id = idesc(p.bf16, p.a_mn, p.b_mn, 256, 256);
-      const uint32_t a0 = desc_lo(smem_u32(smem), p.a_mn), b0 = desc_lo(smem_u32(smem) + HALVES * TILE, p.b_mn);
+      const uint32_t a0 = desc_lo(smem_u32(smem), p.a_mn), b0 = desc_lo(smem_u32(smem) + PLANES * HALVES * TILE, p.b_mn);
       const uint32_t a_step = desc_step(p.a_mn), b_step = desc_step(p.b_mn);
       int stage = 0;
       uint32_t phase = 0, chunks = 0;
@@ -392,8 +399,13 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             const uint32_t d = tmem + (uint32_t)((buf + h) * ACC_COLS), ah = a0 + at + h * (TILE >> 4);
             if (elect_one()) {
 #pragma unroll
-              for (int s = 0; s < BK / 16; ++s)
-                mma_f16_pair(d, desc(ah + s * a_step), desc(b0 + at + s * b_step), id, (in_chunk | s) ? 1u : 0u);
+              for (int l = 0; l < (PLANES == 3 ? F32_PAIRS : 1); ++l) {
+                const uint32_t pa = PLANES == 3 ? (PAIR_A >> (4 * l)) & 15u : 0u, pb = PLANES == 3 ? (PAIR_B >> (4 * l)) & 15u : 0u;
+#pragma unroll
+                for (int s = 0; s < BK / 16; ++s)
+                  mma_f16_pair(d, desc(ah + pa * (HALVES * TILE >> 4) + s * a_step),
+                               desc(b0 + at + pb * (TILE >> 4) + s * b_step), id, (in_chunk | l | s) ? 1u : 0u);
+              }
               if (h == HALVES - 1) {
                 commit_both(&empty_bar[stage]);
                 if (last) commit_both(&tfull_bar[buf]);
@@ -885,7 +897,9 @@ static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int b
 // tile of 256 or 512 rows (the second saves bytes: 8192 x 8192 x 8192 took 793 us
 // against 834), the drain that 512 rows do not hide, and what sharing a tile among `parts` clusters costs (each leaves its
 // sums in L2, the last one adds them).
-static double pair_step(int halves) { return halves == 1 ? 0.44 : 0.82; }
+static double pair_step(int halves, int planes) {
+  return planes == 3 ? 0.44 * F32_PAIRS : (halves == 1 ? 0.44 : 0.82);
+}
 static double drain_cost(int mode) { return mode == DW ? 2.0 : (mode == FWD ? 7.0 : 9.0); }
 static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
 
@@ -894,8 +908,7 @@ static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
 struct Tail {
   int64_t clusters, steps;
 };
-static Tail share(int64_t rest, int64_t steps, int64_t n, int halves, double* us) {
-  const double step = pair_step(halves);
+static Tail share(int64_t rest, int64_t steps, int64_t n, double step, int halves, double* us) {
   Tail best{0, rest ? steps : 0};
   *us = rest ? (double)steps * step : 0.0;
   // An equal number of clusters per tile, or all of them with ranges that cross tiles.
@@ -919,7 +932,8 @@ static Tail share(int64_t rest, int64_t steps, int64_t n, int halves, double* us
 // ---------------------------------------------------------------- launches
 template <typename T, int MODE, int HALVES>
 static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, Params p) {
-  using S = Shape<HALVES>;
+  constexpr int PLANES = plane_count<T>();
+  using S = Shape<HALVES, PLANES>;
   const auto kernel = pair_kernel<T, MODE, HALVES>;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -948,9 +962,10 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   const int64_t a_bytes = p.M * p.K * 2 * (p.pairs == 1 ? 1 : 3);
   p.group_m = a_bytes <= (int64_t)48 << 20 ? (int)cdiv(p.M, S::M) : 2048 / S::M;
   const int64_t tiles = cdiv(p.M, S::M) * cdiv(p.N, 256), n = fit.load();
-  const int64_t steps = cdiv(p.K, BK) * p.pairs, rest = tiles % n;
+  const int64_t steps = cdiv(p.K, BK), rest = tiles % n;
   double us;
-  const Tail tail = share(rest, steps, n, HALVES, &us);
+  const Tail tail = share(rest, steps, n, pair_step(HALVES, PLANES), HALVES, &us);
+  if (PLANES == 3) p.chunk = CHUNK_F32 / F32_PAIRS;
   if (tiles > INT32_MAX - 4096) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
   p.full = (int)tiles;
   p.tail = 0;
@@ -1061,15 +1076,16 @@ static orca_status consider(orca_ctx* ctx, const Params& p, int64_t steps, Plan*
 
 template <typename T, int MODE>
 static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, Plan* plan) {
-  const int64_t n = ctx->sm_count / 2;
+  const int64_t n = ctx->sm_count / 2, blocks = cdiv(p.K, BK);
   plan->us = 1e30;
   for (int halves = 1; halves <= 2; ++halves) {
     // The two-accumulator tile has no F32 chunks.
     if (halves == 2 && (std::is_same<T, float>::value || p.chunk < steps)) break;
     const int64_t tiles = cdiv(p.M, 256 * halves) * cdiv(p.N, 256);
     double us;
-    share(tiles % n, steps, n, halves, &us);
-    us += (double)(tiles / n * steps) * pair_step(halves) + (double)cdiv(tiles, n) * (halves == 2 ? drain_cost(MODE) : 0.0) + 8.0;
+    const double step = pair_step(halves, plane_count<T>());
+    share(tiles % n, blocks, n, step, halves, &us);
+    us += (double)(tiles / n * blocks) * step + (double)cdiv(tiles, n) * (halves == 2 ? drain_cost(MODE) : 0.0) + 8.0;
     if (us < plan->us) *plan = Plan{0, halves, 1, us};
   }
   if constexpr (MODE != DW) {

@@ -5,9 +5,11 @@ Tolerances, all derived from the number formats:
   * a result rounded once to type t is off by at most u_t = finfo(t).eps / 2 of
     its value;
   * the F32 sums over K products are off by at most g(K) * sum |a||b|.  An
-    accumulator step of the tensor core (16 products) loses at most 2^-22 of the
-    magnitudes summed so far, so g = 2^-22 * (K / 16 + 16) covers one chain;
-    F32 operands are summed in chains of at most 32 steps that are joined in F32;
+    accumulator step of the tensor core (16 products) loses less than 2^-22 of
+    the magnitudes summed so far, so g = 2^-22 * (K / 16 + 16) covers one chain;
+    F32 operands are summed in chains of at most 72 steps that are joined in F32,
+    the magnitudes growing evenly along a chain: 72 / 2 steps of the whole at
+    the 2^-23 that an F32 accumulator loses by truncation, 18 * 2^-22 and the joins;
   * activations have slopes of at most 1.13 (GELU's maximum is 1.129), slopes
     change by at most 0.81 per unit (GELU's second derivative at 0 is 0.798),
     and F32 evaluations are off by a few units of 2^-24.
@@ -118,7 +120,7 @@ def decode(buf, m, n):
 
 
 def sum_error(k, t):
-    if t == torch.float32:   # chains of 32 steps, joined in F32; six products each
+    if t == torch.float32:   # chains joined in F32; six products each
         return 2.0 ** -22 * 32 + 2.0 ** -24 * (6 * k / 64 / 8 + 8)
     return 2.0 ** -22 * (k / 16 + 16)
 
