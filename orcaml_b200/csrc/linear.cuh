@@ -67,12 +67,36 @@ __device__ __forceinline__ void store_row(T* p, int valid, bool vec, const float
 
 // ---------------------------------------------------------------- activations
 // f(z) and f'(z) in f32, off by about 2^-22 of |z|.  They run in epilogues and
-// in passes bound by HBM, so they are built from the fast exponential and
-// reciprocal and have no branches.  ReLU is z > 0 ? z : 0, as the F32 path's.
-//
-// Normal upper tail Q(|z|) = erfc(|z| / sqrt 2) / 2 by formula 7.1.26 of
-// Abramowitz and Stegun (|error| of erf <= 1.5e-7): a polynomial in
-// t = 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2.  *e = e^(-z^2 / 2).
+// in passes bound by HBM, so they take two values at a time (packed f32 arithmetic
+// issues once for both), are built from the fast exponential and reciprocal and
+// have no branches.  ReLU is z > 0 ? z : 0, as the F32 path's.
+struct F2 {
+  uint64_t u;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.u) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ void split(F2 x, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(x.u));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
 __device__ __forceinline__ float rcp(float x) {
   float r;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
@@ -83,84 +107,107 @@ __device__ __forceinline__ float exp2_fast(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
   return r;
 }
+template <typename F> __device__ __forceinline__ F2 each(F2 x, F f) {
+  float a, b;
+  split(x, a, b);
+  return f2(f(a), f(b));
+}
+__device__ __forceinline__ F2 rcp2(F2 x) { return each(x, [](float v) { return rcp(v); }); }
+__device__ __forceinline__ F2 exp2_2(F2 x) { return each(x, [](float v) { return exp2_fast(v); }); }
 constexpr float LOG2_E = 1.44269504f;
-__device__ __forceinline__ float normal_tail(float z, float* e) {
-  const float x = fabsf(z);
-  const float t = rcp(fmaf(0.3275911f * 0.70710678f, x, 1.0f));
-  float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
-  q = fmaf(t, q, 0.5f * 1.421413741f);
-  q = fmaf(t, q, 0.5f * -0.284496736f);
-  q = fmaf(t, q, 0.5f * 0.254829592f);
-  *e = exp2_fast((-0.5f * LOG2_E) * x * x);
-  return q * t * *e;
+
+// Normal upper tail Q(|z|) = erfc(|z| / sqrt 2) / 2 by formula 7.1.26 of
+// Abramowitz and Stegun (|error| of erf <= 1.5e-7): a polynomial in
+// t = 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2.  e = e^(-z^2 / 2).
+__device__ __forceinline__ F2 normal_tail(F2 z, F2& e) {
+  const F2 x = each(z, [](float v) { return fabsf(v); });
+  const F2 t = rcp2(fma2(f2(0.3275911f * 0.70710678f), x, f2(1.0f)));
+  F2 q = fma2(t, f2(0.5f * 1.061405429f), f2(0.5f * -1.453152027f));
+  q = fma2(t, q, f2(0.5f * 1.421413741f));
+  q = fma2(t, q, f2(0.5f * -0.284496736f));
+  q = fma2(t, q, f2(0.5f * 0.254829592f));
+  e = exp2_2(mul2(mul2(z, z), f2(-0.5f * LOG2_E)));
+  return mul2(mul2(q, t), e);
 }
 // 1 / (1 + e^-x); 0 below about -88, where e^-x is infinite.
-__device__ __forceinline__ float sigmoid(float x) { return rcp(1.0f + exp2_fast(-LOG2_E * x)); }
+__device__ __forceinline__ F2 sigmoid2(F2 x) {
+  return rcp2(add2(exp2_2(mul2(x, f2(-LOG2_E))), f2(1.0f)));
+}
 // 2 sqrt(2 / pi) (z + 0.044715 z^3): (1 + tanh(half of it)) / 2 is its sigmoid.
-__device__ __forceinline__ float tanh_arg(float z) {
-  return z * fmaf(0.0713548163f * z, z, 1.59576912f);
+__device__ __forceinline__ F2 tanh_arg(F2 z) {
+  return mul2(z, fma2(mul2(z, z), f2(0.0713548163f), f2(1.59576912f)));
 }
 
-template <int ACT> __device__ __forceinline__ float act_value(float z) {
-  if (ACT == ORCA_ACT_RELU) return z > 0.0f ? z : 0.0f;
+template <int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
+  if (ACT == ORCA_ACT_RELU) return each(z, [](float v) { return v > 0.0f ? v : 0.0f; });
   if (ACT == ORCA_ACT_GELU) {
-    float e;
-    const float q = normal_tail(z, &e);
-    return z * (z < 0.0f ? q : 1.0f - q);
+    // z (1 - Q) above 0, z Q below: z or 0 less |z| Q.  |z| is bounded there so
+    // that an infinity times 0 is not a NaN.
+    F2 e;
+    const F2 q = normal_tail(z, e);
+    float a, b, qa, qb;
+    split(z, a, b);
+    split(q, qa, qb);
+    return f2(fmaf(-fminf(fabsf(a), 1e38f), qa, a < 0.0f ? 0.0f : a),
+              fmaf(-fminf(fabsf(b), 1e38f), qb, b < 0.0f ? 0.0f : b));
   }
-  if (ACT == ORCA_ACT_GELU_TANH) return z * sigmoid(tanh_arg(z));
-  if (ACT == ORCA_ACT_SILU) return z * sigmoid(z);
+  if (ACT == ORCA_ACT_GELU_TANH) return mul2(z, sigmoid2(tanh_arg(z)));
+  if (ACT == ORCA_ACT_SILU) return mul2(z, sigmoid2(z));
   return z;
 }
-template <int ACT> __device__ __forceinline__ float act_slope(float z) {
-  if (ACT == ORCA_ACT_RELU) return z > 0.0f ? 1.0f : 0.0f;
+template <int ACT> __device__ __forceinline__ F2 act_slope(F2 z) {
+  if (ACT == ORCA_ACT_RELU) return each(z, [](float v) { return v > 0.0f ? 1.0f : 0.0f; });
   if (ACT == ORCA_ACT_GELU) {
-    float e;
-    const float q = normal_tail(z, &e);
-    return fmaf(z * 0.39894228f, e, z < 0.0f ? q : 1.0f - q);
+    F2 e;
+    const F2 q = normal_tail(z, e);
+    float a, b, qa, qb;
+    split(z, a, b);
+    split(q, qa, qb);
+    return fma2(mul2(z, f2(0.39894228f)), e, f2(a < 0.0f ? qa : 1.0f - qa, b < 0.0f ? qb : 1.0f - qb));
   }
   if (ACT == ORCA_ACT_GELU_TANH) {
     // Beyond |z| = 10 the sigmoid is 0 or 1 in f32 and the second term 0; the
     // bound keeps z * z finite there.  A NaN stays one through z - z.
-    const float y = fminf(fmaxf(z, -10.0f), 10.0f);
-    const float s = sigmoid(tanh_arg(y));
-    return fmaf(y * s * (1.0f - s), fmaf(0.2140644489f * y, y, 1.59576912f), s) + (z - z);
+    const F2 y = each(z, [](float v) { return fminf(fmaxf(v, -10.0f), 10.0f); });
+    const F2 s = sigmoid2(tanh_arg(y));
+    const F2 up = fma2(mul2(y, y), f2(0.2140644489f), f2(1.59576912f));
+    const F2 r = fma2(mul2(mul2(y, s), fma2(s, f2(-1.0f), f2(1.0f))), up, s);
+    return add2(r, fma2(z, f2(-1.0f), z));
   }
   if (ACT == ORCA_ACT_SILU) {
-    const float s = sigmoid(z);
-    return s * fmaf(z, 1.0f - s, 1.0f);
+    const F2 s = sigmoid2(z);
+    return mul2(s, fma2(z, fma2(s, f2(-1.0f), f2(1.0f)), f2(1.0f)));
   }
-  return 1.0f;
+  return f2(1.0f);
 }
 
-// v = f(v), or v = f'(v), for V values with one uniform branch for all.
+// v = f(v), or v *= f'(z), for V values with one uniform branch for all.
+template <int ACT, int V> __device__ __forceinline__ void act_all(float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 2) split(act_value<ACT>(f2(v[i], v[i + 1])), v[i], v[i + 1]);
+}
+template <int ACT, int V> __device__ __forceinline__ void slope_all(const float (&z)[V], float (&v)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += 2)
+    split(mul2(f2(v[i], v[i + 1]), act_slope<ACT>(f2(z[i], z[i + 1]))), v[i], v[i + 1]);
+}
 template <int V> __device__ __forceinline__ void apply_act(int act, float (&v)[V]) {
-#define ORCA_EACH(A)          \
-  case A:                     \
-    _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] = act_value<A>(v[i]); \
-    break;
   switch (act) {
-    ORCA_EACH(ORCA_ACT_RELU)
-    ORCA_EACH(ORCA_ACT_GELU)
-    ORCA_EACH(ORCA_ACT_GELU_TANH)
-    ORCA_EACH(ORCA_ACT_SILU)
+    case ORCA_ACT_RELU: act_all<ORCA_ACT_RELU>(v); break;
+    case ORCA_ACT_GELU: act_all<ORCA_ACT_GELU>(v); break;
+    case ORCA_ACT_GELU_TANH: act_all<ORCA_ACT_GELU_TANH>(v); break;
+    case ORCA_ACT_SILU: act_all<ORCA_ACT_SILU>(v); break;
     default: break;
   }
-#undef ORCA_EACH
 }
 template <int V> __device__ __forceinline__ void mul_slope(int act, const float (&z)[V], float (&v)[V]) {
-#define ORCA_EACH(A)          \
-  case A:                     \
-    _Pragma("unroll") for (int i = 0; i < V; ++i) v[i] *= act_slope<A>(z[i]); \
-    break;
   switch (act) {
-    ORCA_EACH(ORCA_ACT_RELU)
-    ORCA_EACH(ORCA_ACT_GELU)
-    ORCA_EACH(ORCA_ACT_GELU_TANH)
-    ORCA_EACH(ORCA_ACT_SILU)
+    case ORCA_ACT_RELU: slope_all<ORCA_ACT_RELU>(z, v); break;
+    case ORCA_ACT_GELU: slope_all<ORCA_ACT_GELU>(z, v); break;
+    case ORCA_ACT_GELU_TANH: slope_all<ORCA_ACT_GELU_TANH>(z, v); break;
+    case ORCA_ACT_SILU: slope_all<ORCA_ACT_SILU>(z, v); break;
     default: break;
   }
-#undef ORCA_EACH
 }
 
 // ---------------------------------------------------------------- 8-bit checkpoints
@@ -476,9 +523,10 @@ __device__ __forceinline__ void slope_block(const uint32_t (&codes)[8], bool pac
     if (packed) ckpt_values(codes[i], down, z);
     else words_to_f32<T>(x + i * (int)sizeof(T), z);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      v[4 * i + j] *= act_slope<ACT>(z[j]);
-      z[j] = act_value<ACT>(z[j]);
+    for (int j = 0; j < 4; j += 2) {
+      const F2 y = f2(z[j], z[j + 1]);
+      split(mul2(f2(v[4 * i + j], v[4 * i + j + 1]), act_slope<ACT>(y)), v[4 * i + j], v[4 * i + j + 1]);
+      split(act_value<ACT>(y), z[j], z[j + 1]);
     }
     f32_to_words<T>(z, x + i * (int)sizeof(T));
   }
