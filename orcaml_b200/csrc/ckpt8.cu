@@ -19,7 +19,7 @@ constexpr int THREADS = 256;
 // are three contiguous arrays.  A lane takes 8 values (pack) or 16 (unpack), with
 // all its loads in flight before the first is used: HBM needs ~44 KB in flight
 // per SM.
-constexpr int PACK_STEPS = 4, UNPACK_STEPS = 4;
+constexpr int PACK_STEPS = 4, UNPACK_STEPS = 2;
 
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
