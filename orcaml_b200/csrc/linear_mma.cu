@@ -32,13 +32,17 @@ constexpr int TILE = ROWS * BK * 2;          // 16 KB
 constexpr uint32_t PAIR_A = 0x001102u, PAIR_B = 0x010120u;   // pair p: (x >> 4 * p) & 15
 constexpr int F32_PAIRS = 6;
 
-// Steps (of four MMAs) per accumulation chunk of an F32 result.  The tensor core
-// adds with a few bits less than F32; a chain of L MMAs over random data is off by
-// about 9e-10 * L^1.5 of the result's norm.  F32 operands: 72 MMAs (3 blocks of 6 plane
-// products), 5e-7, what an F32 chain of FMAs gives.  F32 gradients of 16-bit operands: 256 MMAs, 4e-6
-// against the operands' own 2^-9; emptying the accumulator every 32 MMAs
-// instead cost 13 % of the product's time.
-constexpr int CHUNK_F32 = 18, CHUNK_DW = 64;
+// Steps (of four MMAs) per accumulation chunk.  The tensor core adds with a few bits
+// less than F32, at the scale of what the accumulator holds, so the accumulator of
+// a result that is to be F32-accurate is emptied into F32 registers in between.
+//  F32 operands: after each 64-deep block of six plane products, the small ones
+//  first, so that only the last four MMAs add at full scale: off by 1.7e-7 of the
+//  result's norm (4096 x 784 x 8192; FMAs in F32: 6e-7), against 1.2e-6 after three
+//  blocks, which took 280 us instead of 298.
+//  F32 gradients and 8-bit checkpoints (whose codes flip with the sums' errors) of
+//  16-bit operands: after CHUNK steps.  4096-deep sums: 3.3e-7, against 1.8e-6 in one
+//  chain; the time is the same for gradients and 3 % more with a checkpoint.
+constexpr int CHUNK = 16;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -470,7 +474,9 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
             float v[16];
             tmem_ld_32x32b_x16(lanes + (uint32_t)(buf * ACC_COLS + q * 16), v);
 #pragma unroll
-            for (int j = 0; j < 16; ++j) acc[q * 16 + j] = __fadd_rn(acc[q * 16 + j], v[j]);
+            for (int j = 0; j < 16; j += 2)
+              split(add2(f2(acc[q * 16 + j], acc[q * 16 + j + 1]), f2(v[j], v[j + 1])), acc[q * 16 + j],
+                    acc[q * 16 + j + 1]);
           }
           if (c == nchunks - 1) break;
           release(buf);
@@ -610,8 +616,8 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
   const int rank = (int)cluster_ctarank();
   const int64_t tile = blockIdx.x / ranks, num_n = cdiv(p.N, 128);
   const int64_t col0 = tile % num_n * 128, row0 = tile / num_n * NT;
-  const int64_t steps = cdiv(p.K, BK) * p.pairs;
-  const int begin = (int)(steps * rank / ranks), end = (int)(steps * (rank + 1) / ranks);
+  const int64_t blocks = cdiv(p.K, BK);
+  const int begin = (int)(blocks * rank / ranks) * p.pairs, end = (int)(blocks * (rank + 1) / ranks) * p.pairs;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {
@@ -965,7 +971,7 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   const int64_t steps = cdiv(p.K, BK), rest = tiles % n;
   double us;
   const Tail tail = share(rest, steps, n, pair_step(HALVES, PLANES), HALVES, &us);
-  if (PLANES == 3) p.chunk = CHUNK_F32 / F32_PAIRS;
+  if (PLANES == 3) p.chunk = 1;            // in 64-deep blocks here
   if (tiles > INT32_MAX - 4096) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
   p.full = (int)tiles;
   p.tail = 0;
@@ -1063,7 +1069,7 @@ static orca_status consider(orca_ctx* ctx, const Params& p, int64_t steps, Plan*
   constexpr double STEP = NT == 16 ? 0.27 : (NT == 32 ? 0.28 : (NT == 64 ? 0.29 : 0.31));
   const int64_t tiles = cdiv(p.N, 128) * cdiv(p.M, NT);
   const double hbm = (p.pairs == 1 ? 2.0 : 6.0) * ((double)p.M + (double)p.N) * (double)p.K / 5.5e6 + 3.0;
-  for (int i = 0; i < 4 && (1 << i) <= steps; ++i) {
+  for (int i = 0; i < 4 && (1 << i) * p.pairs <= steps; ++i) {
     const int ranks = 1 << i;
     // With 16 rows two CTAs fit an SM; that hides their ends, it does not add bandwidth.
     const int64_t at_once = std::min<int64_t>(fits[i], std::max(1, ctx->sm_count / ranks));
@@ -1101,7 +1107,8 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   const int planes = dtype == ORCA_F32 ? 3 : 1;
   const int64_t steps = cdiv(p.K, BK) * p.pairs;
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
-  p.chunk = dtype == ORCA_F32 ? CHUNK_F32 : (MODE == DW && p.e.out_f32 ? CHUNK_DW : (int)steps);
+  p.chunk = dtype == ORCA_F32 ? F32_PAIRS
+            : ((MODE == DW && p.e.out_f32) || (MODE == FWD && p.e.codes) ? CHUNK : (int)steps);
   Plan plan;
   ORCA_TRY((choose<T, MODE>(ctx, p, steps, &plan)));
   if constexpr (MODE != DW) {

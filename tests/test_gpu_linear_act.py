@@ -7,9 +7,7 @@ Tolerances, all derived from the number formats:
   * the F32 sums over K products are off by at most g(K) * sum |a||b|.  An
     accumulator step of the tensor core (16 products) loses less than 2^-22 of
     the magnitudes summed so far, so g = 2^-22 * (K / 16 + 16) covers one chain;
-    F32 operands are summed in chains of at most 72 steps that are joined in F32,
-    the magnitudes growing evenly along a chain: 72 / 2 steps of the whole at
-    the 2^-23 that an F32 accumulator loses by truncation, 18 * 2^-22 and the joins;
+    F32 operands are summed in chains of 24 steps that are joined in F32;
   * activations have slopes of at most 1.13 (GELU's maximum is 1.129), slopes
     change by at most 0.81 per unit (GELU's second derivative at 0 is 0.798),
     and F32 evaluations are off by a few units of 2^-24.
