@@ -284,14 +284,14 @@ class CudaBackend:
     @staticmethod
     def ckpt8_bytes(m, n) -> int:
         """Bytes of the 8-bit checkpoint of an [m, n] matrix."""
-        return int(L.load().orca_ckpt8_bytes(m, n))
+        return int(L.load().orca_ckpt8_bytes(int(m), int(n)))
 
     def ckpt8_pack(self, x, m, n, out=None):
         """The 8-bit checkpoint (U8) of x [m, n]: groups of 32 columns share a
         power of two, each value a signed 8-bit code."""
         x = self._span(x)
         out = self._result(out, self.ckpt8_bytes(m, n), U8)
-        L.check(L.load().orca_ckpt8_pack(self._ctx, x, m, n, self._span(out)))
+        L.check(L.load().orca_ckpt8_pack(self._ctx, x, int(m), int(n), self._span(out)))
         return out
 
     def ckpt8_unpack(self, ckpt, m, n, act="none", dtype=F32, out=None):
@@ -299,7 +299,7 @@ class CudaBackend:
         a = self._choice(ACTS, act, "act")
         ckpt = self._span(ckpt)
         out = self._result(out, m * n, dtype)
-        L.check(L.load().orca_ckpt8_unpack(self._ctx, ckpt, m, n, a, self._span(out)))
+        L.check(L.load().orca_ckpt8_unpack(self._ctx, ckpt, int(m), int(n), a, self._span(out)))
         return out
 
     def linear_act_fwd(self, x, w, b, m, k, n, act="none", residual=None, keep=None, out=None,
@@ -315,7 +315,8 @@ class CudaBackend:
         if kp:
             z = self._result(z, m * n if kp == 1 else self.ckpt8_bytes(m, n), x.dtype if kp == 1 else U8)
         L.check(L.load().orca_linear_act_fwd(self._ctx, x, self._span(w), self._span(b),
-                                             self._span(residual), m, k, n, a, self._span(out), kp,
+                                             self._span(residual), int(m), int(k), int(n), a,
+                                             self._span(out), kp,
                                              self._span(z)))
         return out, z
 
@@ -333,8 +334,8 @@ class CudaBackend:
         dx = self._result(dx, m * k, dy.dtype) if need_dx else None
         dw = self._result(dw, k * n, grad_dtype) if need_dw else None
         db = self._result(db, n, grad_dtype) if need_db else None
-        L.check(L.load().orca_linear_act_bwd(self._ctx, x, self._span(w), dy, self._span(residual), m,
-                                             k, n, a, self._span(dx), self._span(dw),
+        L.check(L.load().orca_linear_act_bwd(self._ctx, x, self._span(w), dy, self._span(residual),
+                                             int(m), int(k), int(n), a, self._span(dx), self._span(dw),
                                              self._span(db)))
         return dx, dw, db
 

@@ -5,10 +5,9 @@
 // is split exactly into three BF16 planes, x = x0 + x1 + x2 (8 significant bits
 // each, by truncation), and the product is the sum of six plane products,
 // x2*y0 + x0*y2 + x1*y1 + x1*y0 + x0*y1 + x0*y0; the three left out are below
-// 2^-24 of |x||y|.  Both kinds run through the same kernels: a step of the sum
-// is one 64-deep block of one plane pair.
+// 2^-21 of |x||y| together.  Both kinds run through the same kernels.
 //
-//  * pair_kernel: 256 x 256 output tiles on clusters of two CTAs
+//  * pair_kernel: 256 x 256 or 512 x 256 output tiles on clusters of two CTAs
 //    (cta_group::2), persistent; for outputs with enough tiles.
 //  * split_kernel: 128 columns x 16..128 rows of the output per cluster, the sum
 //    split over the cluster's CTAs and joined through their shared memory; for
@@ -42,7 +41,9 @@ constexpr int F32_PAIRS = 6;
 //  F32 gradients and 8-bit checkpoints (whose codes flip with the sums' errors) of
 //  16-bit operands: after CHUNK steps.  4096-deep sums: 3.3e-7, against 1.8e-6 in one
 //  chain; the time is the same for gradients and 3 % more with a checkpoint.
-constexpr int CHUNK = 16;
+//  Other results: none, up to MAX_CHUNK steps (30 ms), well inside the time limit of
+//  the waits.
+constexpr int CHUNK = 16, MAX_CHUNK = 65536;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -1108,7 +1109,7 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   const int64_t steps = cdiv(p.K, BK) * p.pairs;
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
   p.chunk = dtype == ORCA_F32 ? F32_PAIRS
-            : ((MODE == DW && p.e.out_f32) || (MODE == FWD && p.e.codes) ? CHUNK : (int)steps);
+            : ((MODE == DW && p.e.out_f32) || (MODE == FWD && p.e.codes) ? CHUNK : (int)std::min<int64_t>(steps, MAX_CHUNK));
   Plan plan;
   ORCA_TRY((choose<T, MODE>(ctx, p, steps, &plan)));
   if constexpr (MODE != DW) {

@@ -406,10 +406,16 @@ def bwd_case(be, t, m, k, n, act, packed, residual, grads, seed=2):
     else:
         src, v = x, x.double()
     gt = torch.float32 if grads == "f32" else t
-    dx = torch.full((m, k), 9.0, dtype=t, device="cuda")
-    dw, db = torch.full((k, n), 9.0, dtype=gt, device="cuda"), torch.full((n,), 9.0, dtype=gt, device="cuda")
+    guard = 64                                     # elements behind each output
+
+    def guarded(*shape, dtype):
+        full = torch.full((math.prod(shape) + guard,), 9.0, dtype=dtype, device="cuda")
+        return full, full[:math.prod(shape)].view(shape)
+
+    (gx, dx), (gw, dw), (gb, db) = guarded(m, k, dtype=t), guarded(k, n, dtype=gt), guarded(n, dtype=gt)
     be.linear_act_bwd(sp(be, src), sp(be, w), sp(be, dy), m, k, n, act=act, x_ckpt8=packed, residual=sp(be, r),
                       dx=sp(be, dx), dw=sp(be, dw), db=sp(be, db))
+    assert all((g[-guard:] == 9.0).all() for g in (gx, gw, gb)), "written behind an output"
     w64, dy64 = w.double(), dy.double()
     back = dy64 @ w64.t()
     s = slope64(v, act)
@@ -445,6 +451,37 @@ def test_backward_large(be, m, k, n):
     if m * k * n < 2 ** 36:
         bwd_case(be, torch.float16, m, k, n, "silu", False, True, "f32")
         bwd_case(be, torch.float32, m, k, n, "gelu_tanh", True, True, "same")
+
+
+def test_backward_long_sums(be):
+    """dX of a long sum over a wide output, in the largest tiles."""
+    bwd_case(be, torch.bfloat16, 8192, 8192, 16384, "gelu", True, False, "same")
+
+
+def test_matrices_past_32_bits(be):
+    """More than 2^32 elements: rows at both ends and around 2^31 and 2^32."""
+    t, m, n, k = torch.bfloat16, 2 ** 17 + 5, 2 ** 15, 64
+    rows = torch.tensor([0, 1, 2 ** 16 - 1, 2 ** 16, 2 ** 17 - 1, 2 ** 17, m - 1], device="cuda")
+    g = gen_of(50)
+    x, w = rand(g, m, k, t=t), rand(g, k, n, scale=k ** -0.5, t=t)
+    out = torch.empty(m, n, dtype=t, device="cuda")
+    z8 = torch.empty(be.ckpt8_bytes(m, n), dtype=torch.uint8, device="cuda")
+    be.linear_act_fwd(sp(be, x), sp(be, w), None, m, k, n, act="silu", keep="ckpt8", out=sp(be, out), z=sp(be, z8))
+    z64 = x[rows].double() @ w.double()
+    off = sum_error(k, t) * (x[rows].double().abs() @ w.double().abs())
+    want = act64(z64, "silu")
+    check("out", out[rows], want, 1.01 * rounding(want, t) + 1.13 * off + 2.0 ** -21 * z64.abs())
+    values = torch.empty(m, n, dtype=t, device="cuda")
+    be.ckpt8_unpack(sp(be, z8), m, n, out=sp(be, values))
+    e = z8[exps_at(m, n):].view(m, n // GROUP)[rows].double()
+    step = torch.exp2(e - 127).repeat_interleave(GROUP, dim=1)
+    v = values[rows].double()
+    check("ckpt8", v, z64, step * torch.where(v.abs() >= 127 * step, 1.0, 0.5) * 1.0001 + off)
+    again = torch.empty_like(z8)
+    be.ckpt8_pack(sp(be, values), m, n, out=sp(be, again))
+    back = torch.empty_like(values)
+    be.ckpt8_unpack(sp(be, again), m, n, out=sp(be, back))
+    assert torch.equal(back[rows], values[rows])           # packing exact values changes nothing
 
 
 def test_sums_shared_by_clusters_repeat_their_bits(be):
