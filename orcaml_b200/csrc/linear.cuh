@@ -413,6 +413,68 @@ __device__ __forceinline__ void epilogue(const Epilogue& e, int64_t row, int64_t
   store_row<T, V>((T*)e.out + at, valid, vec, v);
 }
 
+// The same for 4 fixed columns of up to 2 rows, in two steps: load what the rows'
+// epilogues read, then finish them; the bias is loaded once.  All lanes of a warp
+// call it together, each with its 4 columns of the same rows.
+template <typename T, int MODE> struct ColumnEpilogue {
+  const Epilogue& e;
+  int64_t col;
+  int cols;                  // columns inside, 0..4
+  bool vec;
+  float bias[4], res[2][4], x[2][4];
+  __device__ ColumnEpilogue(const Epilogue& e_, int64_t col_) : e(e_), col(col_) {
+    cols = col >= e.cols ? 0 : (e.cols - col < 4 ? (int)(e.cols - col) : 4);
+    vec = e.vec && cols == 4;
+    if (MODE == FWD) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) bias[i] = 0.0f;
+      if (e.bias && cols > 0) load_row<T, 4>((const T*)e.bias + col, cols, vec, bias);
+    }
+  }
+  __device__ __forceinline__ void load(int u, int64_t row) {
+    if (MODE == DW || row >= e.rows || cols == 0) return;
+    const int64_t at = row * e.cols + col;
+    if (MODE == DX && (e.codes || e.x)) {
+      if (e.codes) ckpt_load<4>(e.codes, e.exps, row, e.cols, col, cols, e.ckpt_align, x[u]);
+      else load_row<T, 4>((const T*)e.x + at, cols, vec, x[u]);
+    }
+    if (e.residual) load_row<T, 4>((const T*)e.residual + at, cols, vec, res[u]);
+  }
+  __device__ __forceinline__ void store(int u, int64_t row, float (&v)[4]) {
+    const bool ok = row < e.rows;
+    const int valid = ok ? cols : 0;
+    const int64_t at = row * e.cols + col;
+    if (MODE == DW) {
+      if (valid <= 0) return;
+      if (e.out_f32) store_row<float, 4>((float*)e.out + at, valid, vec, v);
+      else store_row<T, 4>((T*)e.out + at, valid, vec, v);
+      return;
+    }
+    if (MODE == FWD) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += bias[i];
+      if (e.z && valid > 0) store_row<T, 4>((T*)e.z + at, valid, vec, v);
+      if (e.codes) ckpt_store<4>(e.codes, e.exps, row, e.cols, col, valid, ok, e.ckpt_align, v);
+      if (valid <= 0) return;
+      apply_act<4>(e.act, v);
+    } else {
+      if (valid <= 0) return;
+      if (e.codes || e.x) {
+        mul_slope<4>(e.act, x[u], v);
+        if (e.a) {
+          apply_act<4>(e.act, x[u]);
+          store_row<T, 4>((T*)e.a + at, valid, vec, x[u]);
+        }
+      }
+    }
+    if (e.residual) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += res[u][i];
+    }
+    store_row<T, 4>((T*)e.out + at, valid, vec, v);
+  }
+};
+
 // ---------------------------------------------------------------- 32 x 32 blocks
 // A warp's 32 rows x 32 columns, a row per lane (as TMEM gives them), and
 // row-major memory: the block goes through the warp's 4 KB of shared memory so

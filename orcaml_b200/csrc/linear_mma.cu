@@ -748,29 +748,56 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
 #pragma unroll
     for (int j = 0; j < NT; ++j) part[j * 128 + (warp & 3) * 32 + lane] = acc[j];
   }
-  cluster_sync_all();
+  if (ranks == 1) __syncthreads();
+  else cluster_sync_all();
   if (!*abort_flag) {
-    // A warp per row, 4 columns per lane; the parts of a row are all in flight at once.
-    const int j1 = NT * (rank + 1) / ranks;
-    for (int j = NT * rank / ranks + warp; j < j1 && row0 + j < p.M; j += SPLIT_THREADS / 32) {
-      float4 u[8];
+    // A warp per row, 4 columns per lane; the parts of two rows, and what their
+    // epilogues read, are in flight at once.
+    constexpr int U = 2;
+    const int col = (int)col0 + lane * 4, j1 = NT * (rank + 1) / ranks;
+    ColumnEpilogue<T, MODE> ce(p.e, col);
+    for (int j = NT * rank / ranks + warp * U; j < j1 && row0 + j < p.M; j += SPLIT_THREADS / 32 * U) {
+      float v[U][4];
+      if (ranks == 1) {
 #pragma unroll
-      for (int r = 0; r < 8; ++r)
-        if (r < ranks) u[r] = ld_cluster_f32x4(cluster_addr(part + j * 128 + lane * 4, (uint32_t)r));
-      float v[4] = {u[0].x, u[0].y, u[0].z, u[0].w};
+        for (int u = 0; u < U; ++u) {
+          const float4 x = *reinterpret_cast<const float4*>(part + (j + u < NT ? j + u : j) * 128 + lane * 4);
+          v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+        }
+      } else {
+        float4 x[U][8];
 #pragma unroll
-      for (int r = 1; r < 8; ++r) {
-        if (r < ranks) {
-          v[0] = __fadd_rn(v[0], u[r].x);
-          v[1] = __fadd_rn(v[1], u[r].y);
-          v[2] = __fadd_rn(v[2], u[r].z);
-          v[3] = __fadd_rn(v[3], u[r].w);
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int r = 0; r < 8; ++r)
+            if (r < ranks)
+              x[u][r] = ld_cluster_f32x4(cluster_addr(part + (j + u < NT ? j + u : j) * 128 + lane * 4, (uint32_t)r));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          v[u][0] = x[u][0].x; v[u][1] = x[u][0].y; v[u][2] = x[u][0].z; v[u][3] = x[u][0].w;
+#pragma unroll
+          for (int r = 1; r < 8; ++r) {
+            if (r < ranks) {
+              v[u][0] = __fadd_rn(v[u][0], x[u][r].x);
+              v[u][1] = __fadd_rn(v[u][1], x[u][r].y);
+              v[u][2] = __fadd_rn(v[u][2], x[u][r].z);
+              v[u][3] = __fadd_rn(v[u][3], x[u][r].w);
+            }
+          }
         }
       }
-      epilogue<T, MODE, 4>(p.e, row0 + j, col0 + lane * 4, v);
+      // Rows past this CTA's share or the matrix are outside for the epilogue.
+      int64_t row[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) row[u] = j + u < j1 ? row0 + j + u : p.M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) ce.load(u, row[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u) ce.store(u, row[u], v[u]);
     }
   }
   __syncwarp();
+  if (ranks == 1) return;
   cluster_sync_all();   // no CTA leaves while another still reads its part
 }
 
