@@ -229,20 +229,25 @@ struct Work {
 // B: a quarter fewer bytes from L2 and through shared memory per product, which
 // under the power limit are what is left to save.  The drain is not hidden, so 16
 // warps do it, each half being refilled as soon as it is empty.
-template <int HALVES, int PLANES> struct Shape {
+// TN = 128 (HALVES = 1): 256 x 128 tiles, for outputs with few tiles or an unlucky
+// last round.
+template <int HALVES, int TN, int PLANES> struct Shape {
   static constexpr int EPI_WARPS = 8 * HALVES;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
-  static constexpr int STAGES = PLANES == 3 ? 2 : (HALVES == 1 ? 6 : 4);
-  static constexpr int STAGE = (HALVES + 1) * PLANES * TILE;   // A tiles, B tile: this CTA's rows
+  static constexpr int B_TILE = TN / 2 * BK * 2;            // this CTA's half of B's columns
+  static constexpr int STAGE = (HALVES * TILE + B_TILE) * PLANES;
+  static constexpr int STAGES = 196608 / STAGE;
   static constexpr int BLOCK = BLOCK_SMEM / HALVES;
   static constexpr int SMEM = STAGES * STAGE + EPI_WARPS * BLOCK + 1024 + 256;
   static constexpr int M = 256 * HALVES;
-  static constexpr int BLOCKS = 4 / HALVES;                 // 32-column blocks of a half per warp
-  static constexpr int64_t PART_FLOATS = M * 256;           // one piece of a tile
+  static constexpr int WARP_COLS = TN / (2 * HALVES);       // columns of a half per warp
+  static constexpr int BLOCKS = WARP_COLS / 32;             // ... in blocks of 32
+  static constexpr int ALL_BLOCKS = BLOCKS * HALVES;
+  static constexpr int64_t PART_FLOATS = M * TN;            // one piece of a tile
   static constexpr int ARRIVALS = 2 * EPI_WARPS;            // counters of a tile
   static_assert(SMEM <= 232448, "shared memory of one CTA");
 };
-constexpr int ACC_COLS = 256;
+constexpr int ACC_COLS = 256;                               // TMEM columns between the accumulators
 
 // mbar_wait by a whole warp: one answer for all lanes.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* dev_err,
@@ -252,12 +257,12 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 
 template <typename T> constexpr int plane_count() { return std::is_same<T, float>::value ? 3 : 1; }
 
-template <typename T, int MODE, int HALVES>
-__global__ void __launch_bounds__(Shape<HALVES, plane_count<T>()>::THREADS, 1)
+template <typename T, int MODE, int HALVES, int TN>
+__global__ void __launch_bounds__(Shape<HALVES, TN, plane_count<T>()>::THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ Params p) {
   constexpr int PLANES = plane_count<T>();
-  using S = Shape<HALVES, PLANES>;
+  using S = Shape<HALVES, TN, PLANES>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -273,7 +278,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
   const uint32_t rank = cluster_ctarank();
   const bool even = rank == 0;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int num_m = (int)cdiv(p.M, S::M), num_n = (int)cdiv(p.N, 256);
+  const int num_m = (int)cdiv(p.M, S::M), num_n = (int)cdiv(p.N, TN);
   const int cluster = blockIdx.x >> 1, nclusters = gridDim.x >> 1;
   const int steps = (int)cdiv(p.K, BK);
 
@@ -322,7 +327,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       while (ok && work.get(tile, begin, stop)) {
         int tm, tn;
         tile_at(tile, num_m, num_n, p.group_m, tm, tn);
-        const int row = tm * S::M + (int)rank * 128, col = tn * 256 + (int)rank * 128;
+        const int row = tm * S::M + (int)rank * 128, col = tn * TN + (int)rank * (TN / 2);
         for (int it = begin; it < stop; ++it) {
           const int k0 = it * BK;
           if (!mbar_wait(&empty_bar[stage], phase ^ 1u, abort_flag, p.dev_err)) {
@@ -337,7 +342,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
               for (int h = 0; h < HALVES; ++h)
                 load_tile(a_dst + (l * HALVES + h) * TILE, &map_a, &full_bar[stage], p.a_mn, ROWS, row + h * 256, k0, l);
-              load_tile(a_dst + (PLANES * HALVES + l) * TILE, &map_b, &full_bar[stage], p.b_mn, ROWS, col, k0, l);
+              load_tile(a_dst + PLANES * HALVES * TILE + l * S::B_TILE, &map_b, &full_bar[stage], p.b_mn, TN / 2, col, k0, l);
             }
             issued[stage] = (int)phase;
           } else {
@@ -347,7 +352,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
               for (int h = 0; h < HALVES; ++h)
                 load_tile_pair(a_dst + (l * HALVES + h) * TILE, &map_a, bar, p.a_mn, ROWS, row + h * 256, k0, l);
-              load_tile_pair(a_dst + (PLANES * HALVES + l) * TILE, &map_b, bar, p.b_mn, ROWS, col, k0, l);
+              load_tile_pair(a_dst + PLANES * HALVES * TILE + l * S::B_TILE, &map_b, bar, p.b_mn, TN / 2, col, k0, l);
             }
             last_issue = global_ns();
           }
@@ -372,7 +377,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
   } else if (warp == 1) {
     if (even) {
-      const uint32_t id = idesc(p.bf16, p.a_mn, p.b_mn, 256, 256);
+      const uint32_t id = idesc(p.bf16, p.a_mn, p.b_mn, TN, 256);
       const uint32_t a0 = desc_lo(smem_u32(smem), p.a_mn), b0 = desc_lo(smem_u32(smem) + PLANES * HALVES * TILE, p.b_mn);
       const uint32_t a_step = desc_step(p.a_mn), b_step = desc_step(p.b_mn);
       int stage = 0;
@@ -409,7 +414,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
 #pragma unroll
                 for (int s = 0; s < BK / 16; ++s)
                   mma_f16_pair(d, desc(ah + pa * (HALVES * TILE >> 4) + s * a_step),
-                               desc(b0 + at + pb * (TILE >> 4) + s * b_step), id, (in_chunk | l | s) ? 1u : 0u);
+                               desc(b0 + at + pb * (S::B_TILE >> 4) + s * b_step), id, (in_chunk | l | s) ? 1u : 0u);
               }
               if (h == HALVES - 1) {
                 commit_both(&empty_bar[stage]);
@@ -435,8 +440,8 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
     }
   } else {
     // Warp w reads TMEM lanes [32 * (w % 4), +32) and, of each half, the columns
-    // [32 * BLOCKS * ((w - 2) / 4), +32 * BLOCKS).
-    const int quarter = warp & 3, first_col = (warp - 2) / 4 * (32 * S::BLOCKS);
+    // [WARP_COLS * ((w - 2) / 4), +WARP_COLS).
+    const int quarter = warp & 3, first_col = (warp - 2) / 4 * S::WARP_COLS;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16) + (uint32_t)first_col;
     const uint32_t tempty[2] = {cluster_addr(&tempty_bar[0], 0), cluster_addr(&tempty_bar[1], 0)};
     const uint32_t block = smem_u32(smem + S::STAGES * S::STAGE + (warp - 2) * S::BLOCK);
@@ -449,7 +454,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       int tm, tn;
       tile_at(tile, num_m, num_n, p.group_m, tm, tn);
       const int row = tm * S::M + (int)rank * 128 + quarter * 32;
-      const int col = tn * 256 + first_col;
+      const int col = tn * TN + first_col;
       const bool piece = stop - begin < steps;
       const int nchunks = (stop - begin + p.chunk - 1) / p.chunk;
       auto release = [&](int buf) {
@@ -463,15 +468,15 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       ++chunks;
       if (HALVES == 1 && ok && nchunks > 1) {
         // The sums go back to the last chunk's accumulator, where the epilogue finds
-        // them block by block as it finds those of a single chunk: holding 128 sums
+        // them block by block as it finds those of a single chunk: holding its sums
         // in registers through the epilogue spilled them, and with this much
         // shared memory in use the spills went to L2.
-        float acc[128];
+        float acc[S::WARP_COLS];
 #pragma unroll
-        for (int j = 0; j < 128; ++j) acc[j] = 0.0f;
+        for (int j = 0; j < S::WARP_COLS; ++j) acc[j] = 0.0f;
         for (int c = 0;; ++c) {
 #pragma unroll
-          for (int q = 0; q < 8; ++q) {
+          for (int q = 0; q < S::WARP_COLS / 16; ++q) {
             float v[16];
             tmem_ld_32x32b_x16(lanes + (uint32_t)(buf * ACC_COLS + q * 16), v);
 #pragma unroll
@@ -489,7 +494,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         }
         if (ok) {
 #pragma unroll
-          for (int q = 0; q < 4; ++q) tmem_st_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), acc + q * 32);
+          for (int q = 0; q < S::BLOCKS; ++q) tmem_st_32x32b_x32(lanes + (uint32_t)(buf * ACC_COLS + q * 32), acc + q * 32);
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
       }
@@ -497,11 +502,11 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
       int first = 0, count = 0;
       // This warp's part of a piece: blocks of 32 columns, four columns of each lane
       // side by side.
-      const int my_part = (int)((rank * S::EPI_WARPS + warp - 2) * 4) * 1024 + lane * 4;
+      const int my_part = (int)(rank * S::EPI_WARPS + warp - 2) * (S::ALL_BLOCKS * 1024) + lane * 4;
       if (piece) {
         float* mine = p.parts + (int64_t)(cluster * 2 + (begin == 0)) * S::PART_FLOATS + my_part;
 #pragma unroll 1
-        for (int q = 0; q < 4; ++q) {
+        for (int q = 0; q < S::ALL_BLOCKS; ++q) {
           float v[32];
           tmem_ld_32x32b_x32(lanes + (uint32_t)((buf + q / S::BLOCKS) * ACC_COLS + q % S::BLOCKS * 32), v);
 #pragma unroll
@@ -528,7 +533,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
         __threadfence();
       }
 #pragma unroll 1
-      for (int q = 0; q < 4; ++q) {
+      for (int q = 0; q < S::ALL_BLOCKS; ++q) {
         // Blocks of half 0, then of half 1.
         const int h = q / S::BLOCKS;
         const int c0 = col + q % S::BLOCKS * 32;
@@ -927,12 +932,13 @@ static orca_status make_map(CUtensorMap* map, const Planes& x, int planes, int b
 }
 
 // ---------------------------------------------------------------- plans
-// Times in microseconds that the choices below compare, measured: a step of a
-// tile of 256 or 512 rows (the second saves bytes: 8192 x 8192 x 8192 took 793 us
-// against 834), the drain that 512 rows do not hide, and what sharing a tile among `parts` clusters costs (each leaves its
+// Times in microseconds that the choices below compare, measured: a step of each
+// tile (512 rows save bytes: 8192 x 8192 x 8192 took 793 us against 834; 128 columns
+// save part of a round: 4704 x 896 over 2208 24 us against 38), the drain that 512 rows do not hide, and what sharing a tile among `parts` clusters costs (each leaves its
 // sums in L2, the last one adds them).
-static double pair_step(int halves, int planes) {
-  return planes == 3 ? 0.44 * F32_PAIRS : (halves == 1 ? 0.44 : 0.82);
+static double pair_step(int halves, int tn, int planes) {
+  const double t = halves == 2 ? 0.77 : (tn == 256 ? 0.41 : 0.29);
+  return planes == 3 ? t * F32_PAIRS : t;
 }
 static double drain_cost(int mode) { return mode == DW ? 2.0 : (mode == FWD ? 7.0 : 9.0); }
 static double share_cost(int64_t parts) { return 8.0 + 2.5 * (double)parts; }
@@ -964,11 +970,14 @@ static Tail share(int64_t rest, int64_t steps, int64_t n, double step, int halve
 }
 
 // ---------------------------------------------------------------- launches
-template <typename T, int MODE, int HALVES>
-static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUtensorMap& mb, Params p) {
+template <typename T, int MODE, int HALVES, int TN>
+static orca_status launch_pair(orca_ctx* ctx, const Planes& a, const Planes& b, Params p) {
   constexpr int PLANES = plane_count<T>();
-  using S = Shape<HALVES, PLANES>;
-  const auto kernel = pair_kernel<T, MODE, HALVES>;
+  using S = Shape<HALVES, TN, PLANES>;
+  const auto kernel = pair_kernel<T, MODE, HALVES, TN>;
+  CUtensorMap ma, mb;
+  ORCA_TRY(make_map(&ma, a, PLANES, p.bf16, p.a_mn ? BK : ROWS));
+  ORCA_TRY(make_map(&mb, b, PLANES, p.bf16, p.b_mn ? BK : TN / 2));
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -995,10 +1004,10 @@ static orca_status launch_pair(orca_ctx* ctx, const CUtensorMap& ma, const CUten
   // (4096 x 4096 x 16384: 404 us against 416).
   const int64_t a_bytes = p.M * p.K * 2 * (p.pairs == 1 ? 1 : 3);
   p.group_m = a_bytes <= (int64_t)48 << 20 ? (int)cdiv(p.M, S::M) : 2048 / S::M;
-  const int64_t tiles = cdiv(p.M, S::M) * cdiv(p.N, 256), n = fit.load();
+  const int64_t tiles = cdiv(p.M, S::M) * cdiv(p.N, TN), n = fit.load();
   const int64_t steps = cdiv(p.K, BK), rest = tiles % n;
   double us;
-  const Tail tail = share(rest, steps, n, pair_step(HALVES, PLANES), HALVES, &us);
+  const Tail tail = share(rest, steps, n, pair_step(HALVES, TN, PLANES), HALVES, &us);
   if (PLANES == 3) p.chunk = 1;            // in 64-deep blocks here
   if (tiles > INT32_MAX - 4096) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
   p.full = (int)tiles;
@@ -1084,6 +1093,7 @@ static orca_status launch_split(orca_ctx* ctx, const Planes& a, const Planes& b,
 struct Plan {
   int nt = 0;       // 0: pair_kernel
   int halves = 1;   // ... with 256 or 512 rows a tile
+  int tn = 256;     // ... and 256 or 128 columns
   int ranks = 1;
   double us = 0;
 };
@@ -1103,7 +1113,7 @@ static orca_status consider(orca_ctx* ctx, const Params& p, int64_t steps, Plan*
     const int64_t at_once = std::min<int64_t>(fits[i], std::max(1, ctx->sm_count / ranks));
     const double us = std::max(
         hbm, (double)cdiv(tiles, at_once) * ((double)cdiv(steps, ranks) * STEP + (NT == 128 ? 3.0 : 1.0)) + 6.3 + 0.05 * ranks);
-    if (us < best->us) *best = Plan{NT, 1, ranks, us};
+    if (us < best->us) *best = Plan{NT, 1, 256, ranks, us};
   }
   return ORCA_OK;
 }
@@ -1112,15 +1122,17 @@ template <typename T, int MODE>
 static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, Plan* plan) {
   const int64_t n = ctx->sm_count / 2, blocks = cdiv(p.K, BK);
   plan->us = 1e30;
-  for (int halves = 1; halves <= 2; ++halves) {
+  for (int shape = 0; shape < 3; ++shape) {
+    const int halves = shape == 2 ? 2 : 1, tn = shape == 0 ? 128 : 256;
     // The two-accumulator tile has no F32 chunks.
     if (halves == 2 && (std::is_same<T, float>::value || p.chunk < steps)) break;
-    const int64_t tiles = cdiv(p.M, 256 * halves) * cdiv(p.N, 256);
+    const int64_t tiles = cdiv(p.M, 256 * halves) * cdiv(p.N, tn);
+    const double step = pair_step(halves, tn, plane_count<T>());
     double us;
-    const double step = pair_step(halves, plane_count<T>());
     share(tiles % n, blocks, n, step, halves, &us);
-    us += (double)(tiles / n * blocks) * step + (double)cdiv(tiles, n) * (halves == 2 ? drain_cost(MODE) : 0.0) + 8.0;
-    if (us < plan->us) *plan = Plan{0, halves, 1, us};
+    us += (double)(tiles / n * blocks) * step + (double)cdiv(tiles, n) * (halves == 2 ? drain_cost(MODE) : 0.0) +
+          (tn == 256 ? 8.0 : 7.0);
+    if (us < plan->us) *plan = Plan{0, halves, tn, 1, us};
   }
   if constexpr (MODE != DW) {
     if (p.M <= 16) return consider<T, MODE, 16>(ctx, p, steps, plan);
@@ -1145,13 +1157,11 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   }
   if (plan.nt == 64) return launch_split<T, MODE, 64>(ctx, a, b, planes, p, plan.ranks);
   if (plan.nt == 128) return launch_split<T, MODE, 128>(ctx, a, b, planes, p, plan.ranks);
-  CUtensorMap ma, mb;
-  ORCA_TRY(make_map(&ma, a, planes, p.bf16, p.a_mn ? BK : ROWS));
-  ORCA_TRY(make_map(&mb, b, planes, p.bf16, p.b_mn ? BK : ROWS));
   if constexpr (!std::is_same<T, float>::value) {
-    if (plan.halves == 2) return launch_pair<T, MODE, 2>(ctx, ma, mb, p);
+    if (plan.halves == 2) return launch_pair<T, MODE, 2, 256>(ctx, a, b, p);
   }
-  return launch_pair<T, MODE, 1>(ctx, ma, mb, p);
+  if (plan.tn == 128) return launch_pair<T, MODE, 1, 128>(ctx, a, b, p);
+  return launch_pair<T, MODE, 1, 256>(ctx, a, b, p);
 }
 
 }  // namespace lin
