@@ -38,23 +38,20 @@ pack_flat_kernel(const T* __restrict__ x, int64_t vecs, uint8_t* __restrict__ co
 #pragma unroll
   for (int s = 0; s < PACK_STEPS; ++s) {
     const int64_t i = base + s * THREADS;
-    float v[8];
-    uint32_t amax = 0;
+    float v[8], amax = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = to_f32(in[s].e[j]);
-      const uint32_t a = __float_as_uint(v[j]) & 0x7fffffffu;
-      amax = a > amax ? a : amax;
-    }
+    for (int j = 0; j < 8; ++j) v[j] = to_f32(in[s].e[j]);
 #pragma unroll
-    for (int o = 1; o < 4; o <<= 1) {                // a group is 4 lanes (vecs is a multiple of 4)
-      const uint32_t other = __shfl_xor_sync(0xffffffffu, amax, o);
-      amax = other > amax ? other : amax;
-    }
+    for (int j = 0; j < 8; j += 2) amax = ckpt_max(amax, v[j], v[j + 1]);
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1)                  // a group is 4 lanes (vecs is a multiple of 4)
+      amax = ckpt_max(amax, amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (i >= vecs) continue;
     const uint32_t e = ckpt_exponent(amax);
     const float up = ckpt_up(e);
-    reinterpret_cast<uint2*>(codes)[i] = make_uint2(ckpt_word(v, up), ckpt_word(v + 4, up));
+    uint32_t w[2];
+    ckpt_words<8>(v, amax, up, w);
+    reinterpret_cast<uint2*>(codes)[i] = make_uint2(w[0], w[1]);
     if (i % 4 == 0) exps[i / 4] = (uint8_t)e;
   }
 }

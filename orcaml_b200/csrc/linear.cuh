@@ -223,11 +223,16 @@ constexpr uint32_t E_NONFINITE = 255;
 __host__ __device__ inline int64_t ckpt_groups(int64_t n) { return (n + GROUP - 1) / GROUP; }
 __host__ __device__ inline int64_t ckpt_exps_at(int64_t m, int64_t n) { return (m * n + 15) / 16 * 16; }
 
-// amax_bits: the largest of the values' bits without the sign; as integers a
-// NaN is above an infinity and that above every finite value.
-__device__ __forceinline__ uint32_t ckpt_exponent(uint32_t amax_bits) {
-  if (amax_bits >= 0x7f800000u) return E_NONFINITE;
-  const int e = (int)(amax_bits >> 23) - 6;
+// The largest magnitude of a, |v|, |w|; a NaN among them stays.
+__device__ __forceinline__ float ckpt_max(float a, float v, float w) {
+  float r;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(v), "f"(w));
+  return r;
+}
+__device__ __forceinline__ uint32_t ckpt_exponent(float amax) {
+  const uint32_t bits = __float_as_uint(amax);       // a NaN is above an infinity
+  if (bits >= 0x7f800000u) return E_NONFINITE;
+  const int e = (int)(bits >> 23) - 6;
   return (uint32_t)(e < 1 ? 1 : e);
 }
 __device__ __forceinline__ float ckpt_up(uint32_t e) {      // 2^(127 - E); 0 for a marked group
@@ -236,28 +241,38 @@ __device__ __forceinline__ float ckpt_up(uint32_t e) {      // 2^(127 - E); 0 fo
 __device__ __forceinline__ float ckpt_down(uint32_t e) {    // 2^(E - 127); NaN for a marked group
   return e == E_NONFINITE ? __uint_as_float(0x7fffffffu) : __uint_as_float(e << 23);
 }
-// The code in the low byte.  v * up is exact, and adding 1.5 * 2^23 rounds it to
-// the nearest whole number, ties to even, into the low mantissa bits: no
-// conversion instruction (those share a slow pipe with the exponentials).
-__device__ __forceinline__ uint32_t ckpt_code(float v, float up) {
-  const float q = fminf(fmaxf(v * up, -127.0f), 127.0f);
-  return __float_as_uint(q + 12582912.0f);
-}
-// Four codes as a word; none in a marked group.
-__device__ __forceinline__ uint32_t ckpt_word(const float* v, float up) {
-  const uint32_t a = __byte_perm(ckpt_code(v[0], up), ckpt_code(v[1], up), 0x0040);
-  const uint32_t b = __byte_perm(ckpt_code(v[2], up), ckpt_code(v[3], up), 0x0040);
-  return up == 0.0f ? 0u : __byte_perm(a, b, 0x5410);
+// Codes of N values, four to a word.  v * up is exact, and adding 1.5 * 2^23 rounds
+// it to the nearest whole number, ties to even, into the low mantissa bits: no
+// conversion instruction (those share a slow pipe with the exponentials).  Only
+// a group whose largest value reaches 127.5 (one in 256) needs the bounds.
+template <int N>
+__device__ __forceinline__ void ckpt_words(const float* v, float amax, float up, uint32_t* w) {
+  const F2 scale = f2(up), magic = f2(12582912.0f);
+  const bool bound = amax * up >= 127.5f;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    float q[4];
+    if (!bound) {
+      split(fma2(f2(v[i], v[i + 1]), scale, magic), q[0], q[1]);
+      split(fma2(f2(v[i + 2], v[i + 3]), scale, magic), q[2], q[3]);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) q[j] = fminf(fmaxf(v[i + j] * up, -127.0f), 127.0f) + 12582912.0f;
+    }
+    const uint32_t a = __byte_perm(__float_as_uint(q[0]), __float_as_uint(q[1]), 0x0040);
+    const uint32_t b = __byte_perm(__float_as_uint(q[2]), __float_as_uint(q[3]), 0x0040);
+    w[i / 4] = up == 0.0f ? 0u : __byte_perm(a, b, 0x5410);
+  }
 }
 
 // Values of the four codes of a word: a code plus 128 as the low mantissa byte of
 // 2^23, less 2^23 + 128 (exact; again no conversion instruction).
 __device__ __forceinline__ void ckpt_values(uint32_t word, float down, float* v) {
   const uint32_t w = word ^ 0x80808080u;
-  v[0] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7440)) - 8388736.0f) * down;
-  v[1] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7441)) - 8388736.0f) * down;
-  v[2] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7442)) - 8388736.0f) * down;
-  v[3] = (__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7443)) - 8388736.0f) * down;
+  const F2 scale = f2(down), less = f2(-8388736.0f);
+  const auto at = [&](int sel) { return __uint_as_float(__byte_perm(w, 0x4B000000u, sel)); };
+  split(mul2(add2(f2(at(0x7440), at(0x7441)), less), scale), v[0], v[1]);
+  split(mul2(add2(f2(at(0x7442), at(0x7443)), less), scale), v[2], v[3]);
 }
 
 // Codes the V values of one lane, 32 / V adjacent lanes sharing a group (all
@@ -267,27 +282,20 @@ template <int V>
 __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_t row, int64_t n,
                                            int64_t col, int valid, bool row_ok, int align,
                                            const float (&v)[V]) {
-  uint32_t amax = 0;
+  float amax = 0.0f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
-    const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-    if (i < valid) amax = a > amax ? a : amax;
-  }
+  for (int i = 0; i < V; i += 2)
+    amax = ckpt_max(amax, i < valid ? v[i] : 0.0f, i + 1 < valid ? v[i + 1] : 0.0f);
 #pragma unroll
-  for (int o = 1; o < GROUP / V; o <<= 1) {
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, amax, o);
-    amax = other > amax ? other : amax;
-  }
+  for (int o = 1; o < GROUP / V; o <<= 1) amax = ckpt_max(amax, amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if (!row_ok || valid <= 0) return;
   const uint32_t e = ckpt_exponent(amax);
   const float up = ckpt_up(e);
   if (col % GROUP == 0) exps[row * ckpt_groups(n) + col / GROUP] = (uint8_t)e;
   uint8_t* p = codes + row * n + col;
-  if (V >= 4 && valid >= V && align >= 4) {
-    uint32_t w[(V + 3) / 4];
-#pragma unroll
-    for (int i = 0; i < V / 4; ++i)
-      w[i] = ckpt_word(v + 4 * i, up);
+  uint32_t w[V / 4];
+  ckpt_words<V>(v, amax, up, w);
+  if (valid >= V && align >= 4) {
     if (V >= 16 && align >= 16) {
 #pragma unroll
       for (int i = 0; i < V / 16; ++i)
@@ -303,7 +311,7 @@ __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_
   } else {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (i < valid) p[i] = up == 0.0f ? (uint8_t)0 : (uint8_t)ckpt_code(v[i], up);
+      if (i < valid) p[i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
   }
 }
 
@@ -636,19 +644,14 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
     }
     if (e.z) block_store_f32<T>((T*)e.z + at, e.cols, rows, v, smem, lane);
     if (packed) {
-      uint32_t amax = 0;
+      float amax = 0.0f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        const uint32_t a = __float_as_uint(v[i]) & 0x7fffffffu;
-        amax = a > amax ? a : amax;
-      }
+      for (int i = 0; i < 32; i += 2) amax = ckpt_max(amax, v[i], v[i + 1]);
       const uint32_t x = ckpt_exponent(amax);
       const float up = ckpt_up(x);
       if (lane < rows) e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP] = (uint8_t)x;
       union { uint4 q[2]; uint32_t w[8]; } u;
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        u.w[i] = ckpt_word(v + 4 * i, up);
+      ckpt_words<32>(v, amax, up, u.w);
       block_store<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
     }
     apply_act<32>(e.act, v);
