@@ -116,16 +116,18 @@ __device__ __forceinline__ F2 rcp2(F2 x) { return each(x, [](float v) { return r
 __device__ __forceinline__ F2 exp2_2(F2 x) { return each(x, [](float v) { return exp2_fast(v); }); }
 constexpr float LOG2_E = 1.44269504f;
 
-// Normal upper tail Q(|z|) = erfc(|z| / sqrt 2) / 2 by formula 7.1.26 of
+// -Q(|z|), Q the normal upper tail erfc(|z| / sqrt 2) / 2, by formula 7.1.26 of
 // Abramowitz and Stegun (|error| of erf <= 1.5e-7): a polynomial in
-// t = 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2.  e = e^(-z^2 / 2).
-__device__ __forceinline__ F2 normal_tail(F2 z, F2& e) {
-  const F2 x = each(z, [](float v) { return fabsf(v); });
-  const F2 t = rcp2(fma2(f2(0.3275911f * 0.70710678f), x, f2(1.0f)));
-  F2 q = fma2(t, f2(0.5f * 1.061405429f), f2(0.5f * -1.453152027f));
-  q = fma2(t, q, f2(0.5f * 1.421413741f));
-  q = fma2(t, q, f2(0.5f * -0.284496736f));
-  q = fma2(t, q, f2(0.5f * 0.254829592f));
+// t = 1 / (1 + p x) times e^(-x^2), x = |z| / sqrt 2.  x2 = |z|, bounded so that
+// an infinity times 0 does not become a NaN (a NaN stays one through e);
+// e = e^(-z^2 / 2).
+__device__ __forceinline__ F2 normal_tail(F2 z, F2& x2, F2& e) {
+  x2 = each(z, [](float v) { return fminf(fabsf(v), 1e38f); });
+  const F2 t = rcp2(fma2(f2(0.3275911f * 0.70710678f), x2, f2(1.0f)));
+  F2 q = fma2(t, f2(-0.5f * 1.061405429f), f2(0.5f * 1.453152027f));
+  q = fma2(t, q, f2(-0.5f * 1.421413741f));
+  q = fma2(t, q, f2(0.5f * 0.284496736f));
+  q = fma2(t, q, f2(-0.5f * 0.254829592f));
   e = exp2_2(mul2(mul2(z, z), f2(-0.5f * LOG2_E)));
   return mul2(mul2(q, t), e);
 }
@@ -141,15 +143,10 @@ __device__ __forceinline__ F2 tanh_arg(F2 z) {
 template <int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
   if (ACT == ORCA_ACT_RELU) return each(z, [](float v) { return v > 0.0f ? v : 0.0f; });
   if (ACT == ORCA_ACT_GELU) {
-    // z (1 - Q) above 0, z Q below: z or 0 less |z| Q.  |z| is bounded there so
-    // that an infinity times 0 is not a NaN.
-    F2 e;
-    const F2 q = normal_tail(z, e);
-    float a, b, qa, qb;
-    split(z, a, b);
-    split(q, qa, qb);
-    return f2(fmaf(-fminf(fabsf(a), 1e38f), qa, a < 0.0f ? 0.0f : a),
-              fmaf(-fminf(fabsf(b), 1e38f), qb, b < 0.0f ? 0.0f : b));
+    // z (1 - Q) above 0, z Q below: z or 0, less |z| Q.
+    F2 x, e;
+    const F2 q = normal_tail(z, x, e);
+    return fma2(x, q, each(z, [](float v) { return fmaxf(v, 0.0f); }));
   }
   if (ACT == ORCA_ACT_GELU_TANH) return mul2(z, sigmoid2(tanh_arg(z)));
   if (ACT == ORCA_ACT_SILU) return mul2(z, sigmoid2(z));
@@ -158,12 +155,13 @@ template <int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
 template <int ACT> __device__ __forceinline__ F2 act_slope(F2 z) {
   if (ACT == ORCA_ACT_RELU) return each(z, [](float v) { return v > 0.0f ? 1.0f : 0.0f; });
   if (ACT == ORCA_ACT_GELU) {
-    F2 e;
-    const F2 q = normal_tail(z, e);
-    float a, b, qa, qb;
+    // Phi(z) = 1/2 + sign(z) (1/2 - Q), and z times the density.
+    F2 x, e;
+    const F2 h = add2(normal_tail(z, x, e), f2(0.5f));
+    float a, b, ha, hb;
     split(z, a, b);
-    split(q, qa, qb);
-    return fma2(mul2(z, f2(0.39894228f)), e, f2(a < 0.0f ? qa : 1.0f - qa, b < 0.0f ? qb : 1.0f - qb));
+    split(h, ha, hb);
+    return fma2(mul2(z, f2(0.39894228f)), e, add2(f2(copysignf(ha, a), copysignf(hb, b)), f2(0.5f)));
   }
   if (ACT == ORCA_ACT_GELU_TANH) {
     // Beyond |z| = 10 the sigmoid is 0 or 1 in f32 and the second term 0; the
