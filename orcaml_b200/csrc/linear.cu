@@ -60,7 +60,9 @@ zero_kernel(Epilogue e) {
   const int64_t vecs = cdiv(e.cols, 128) * 32;       // whole warps per row (groups of columns)
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < e.rows * vecs; i += (int64_t)gridDim.x * 256) {
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    epilogue<T, MODE, 4>(e, i / vecs, i % vecs * 4, v);
+    ColumnEpilogue<T, MODE> ce(e, i % vecs * 4);
+    ce.load(0, i / vecs);
+    ce.store(0, i / vecs, v);
   }
 }
 
@@ -168,8 +170,9 @@ static orca_status product(orca_ctx* ctx, int64_t M, int64_t N, int64_t K, const
   int al = 16;
   for (const void* p : {(const void*)e.out, e.residual, (const void*)e.z, e.x, (const void*)e.a})
     if (p) al = std::min(al, byte_alignment(p, N * (int64_t)sizeof(T)));
-  if (e.bias) al = std::min(al, byte_alignment(e.bias, 0));
-  e.vec = al == 16;
+  e.align = al;
+  if (e.out_f32) e.align = std::min(byte_alignment(e.out, N * 4), 16);
+  e.bias_vec = e.bias && byte_alignment(e.bias, 0) == 16;
   if (e.codes) e.ckpt_align = byte_alignment(e.codes, N);
   if (K > 0) return mma_product(ctx, MODE, dtype_of<T>(), M, N, K, A, a_mn, B, b_mn, e);
   const unsigned grid = (unsigned)std::min<int64_t>(cdiv(M * cdiv(N, 128) * 32, 256), (int64_t)ctx->sm_count * 16);

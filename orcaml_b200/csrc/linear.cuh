@@ -361,7 +361,8 @@ enum Mode : int { FWD = 0, DX = 1, DW = 2 };
 struct Epilogue {
   int64_t rows = 0, cols = 0;
   int act = ORCA_ACT_NONE;
-  int vec = 0;                        // 16-byte accesses are aligned in every T matrix below
+  int align = 1;                      // of the rows of every T matrix below, in bytes (16, 8, 4, 1)
+  int bias_vec = 0;                   // 16-byte loads of the bias are aligned
   int ckpt_align = 1;                 // of a checkpoint's rows, in bytes
   void* out = nullptr;                // T; DW with out_f32: float
   int out_f32 = 0;
@@ -374,52 +375,7 @@ struct Epilogue {
   void* a = nullptr;                  // DX: act(x) in T, the operand of dW, is written here
 };
 
-// V consecutive columns of one row per thread, 32 / V adjacent lanes on
-// adjacent columns.  All lanes of a warp call it together.
-template <typename T, int MODE, int V>
-__device__ __forceinline__ void epilogue(const Epilogue& e, int64_t row, int64_t col, float (&v)[V]) {
-  const bool row_ok = row < e.rows;
-  const int valid = !row_ok || col >= e.cols ? 0 : (e.cols - col < V ? (int)(e.cols - col) : V);
-  const bool vec = e.vec && valid == V;
-  const int64_t at = row * e.cols + col;
-  if (MODE == DW) {
-    if (valid <= 0) return;
-    if (e.out_f32) store_row<float, V>((float*)e.out + at, valid, vec, v);
-    else store_row<T, V>((T*)e.out + at, valid, vec, v);
-    return;
-  }
-  float t[V];
-  if (MODE == FWD) {
-    if (e.bias && valid > 0) {
-      load_row<T, V>((const T*)e.bias + col, valid, vec, t);
-#pragma unroll
-      for (int i = 0; i < V; ++i) v[i] += t[i];
-    }
-    if (e.z && valid > 0) store_row<T, V>((T*)e.z + at, valid, vec, v);
-    if (e.codes) ckpt_store<V>(e.codes, e.exps, row, e.cols, col, valid, row_ok, e.ckpt_align, v);
-    if (valid <= 0) return;
-    apply_act<V>(e.act, v);
-  } else {
-    if (valid <= 0) return;
-    if (e.codes || e.x) {
-      if (e.codes) ckpt_load<V>(e.codes, e.exps, row, e.cols, col, valid, e.ckpt_align, t);
-      else load_row<T, V>((const T*)e.x + at, valid, vec, t);
-      mul_slope<V>(e.act, t, v);
-      if (e.a) {
-        apply_act<V>(e.act, t);
-        store_row<T, V>((T*)e.a + at, valid, vec, t);
-      }
-    }
-  }
-  if (e.residual) {
-    load_row<T, V>((const T*)e.residual + at, valid, vec, t);
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] += t[i];
-  }
-  store_row<T, V>((T*)e.out + at, valid, vec, v);
-}
-
-// The same for 4 fixed columns of up to 2 rows, in two steps: load what the rows'
+// For 4 fixed columns of up to 2 rows, in two steps: load what the rows'
 // epilogues read, then finish them; the bias is loaded once.  All lanes of a warp
 // call it together, each with its 4 columns of the same rows.
 template <typename T, int MODE> struct ColumnEpilogue {
@@ -430,11 +386,11 @@ template <typename T, int MODE> struct ColumnEpilogue {
   float bias[4], res[2][4], x[2][4];
   __device__ ColumnEpilogue(const Epilogue& e_, int64_t col_) : e(e_), col(col_) {
     cols = col >= e.cols ? 0 : (e.cols - col < 4 ? (int)(e.cols - col) : 4);
-    vec = e.vec && cols == 4;
+    vec = e.align == 16 && cols == 4;
     if (MODE == FWD) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) bias[i] = 0.0f;
-      if (e.bias && cols > 0) load_row<T, 4>((const T*)e.bias + col, cols, vec, bias);
+      if (e.bias && cols > 0) load_row<T, 4>((const T*)e.bias + col, cols, e.bias_vec && cols == 4, bias);
     }
   }
   __device__ __forceinline__ void load(int u, int64_t row) {
@@ -502,51 +458,129 @@ template <int P> __device__ __forceinline__ uint32_t piece_at(uint32_t smem, int
   const int f = P == 8 ? row & 7 : (P == 4 ? (row >> 1) & 3 : (row >> 2) & 1);
   return smem + (uint32_t)(row * P + (piece ^ f)) * 16;
 }
-// u: this lane's row.  Rows from `rows` on are not written.
+// What of a block is inside the matrix: rows, and bytes of each row; and the largest
+// power of two, as a shift, that row starts and row lengths share (16 bytes at most).
+struct Inside {
+  int rows, bytes, shift;
+};
+__device__ __forceinline__ int align_shift(int align) { return 31 - __clz(align); }
+
+// Moves the block between shared memory and rows of any alignment, in units of
+// 1 << shift bytes: adjacent lanes take adjacent units.
+template <int P, bool STORE>
+__device__ __forceinline__ void block_move(uint8_t* p, int64_t stride, const Inside& in, uint32_t smem, int lane) {
+  constexpr int LOG = P == 8 ? 7 : (P == 4 ? 6 : 5);
+#pragma unroll 4
+  for (int i = lane; i < (32 * P * 16) >> in.shift; i += 32) {
+    const int r = i >> (LOG - in.shift), off = (i << in.shift) & (P * 16 - 1);
+    if (r >= in.rows || off >= in.bytes) continue;
+    const uint32_t at = piece_at<P>(smem, r, off >> 4) + (uint32_t)(off & 15);
+    uint8_t* g = p + r * stride + off;
+    switch (in.shift) {
+      case 4:
+        if (STORE) *reinterpret_cast<uint4*>(g) = lds_v4(at);
+        else sts_v4(at, *reinterpret_cast<const uint4*>(g));
+        break;
+      case 3: {
+        uint2 v;
+        if (STORE) {
+          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+          *reinterpret_cast<uint2*>(g) = v;
+        } else {
+          v = *reinterpret_cast<const uint2*>(g);
+          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
+        }
+        break;
+      }
+      case 2: {
+        uint32_t v;
+        if (STORE) {
+          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
+          *reinterpret_cast<uint32_t*>(g) = v;
+        } else {
+          v = *reinterpret_cast<const uint32_t*>(g);
+          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+        }
+        break;
+      }
+      case 1: {
+        uint16_t v;
+        if (STORE) {
+          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at));
+          *reinterpret_cast<uint16_t*>(g) = v;
+        } else {
+          v = *reinterpret_cast<const uint16_t*>(g);
+          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
+        }
+        break;
+      }
+      default: {
+        uint32_t v;
+        if (STORE) {
+          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
+          *g = (uint8_t)v;
+        } else {
+          v = *g;
+          asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+        }
+      }
+    }
+  }
+}
+
+// u: this lane's row, P pieces.
 template <int P>
-__device__ __forceinline__ void block_store(uint8_t* p, int64_t stride, int rows, const uint4 (&u)[P],
+__device__ __forceinline__ void block_store(uint8_t* p, int64_t stride, const Inside& in, const uint4 (&u)[P],
                                             uint32_t smem, int lane) {
 #pragma unroll
   for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, lane, i), u[i]);
   __syncwarp();
+  if (in.shift == 4 && in.bytes == P * 16) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int r = i * (32 / P) + lane / P;
-    const uint4 v = lds_v4(piece_at<P>(smem, r, lane % P));
-    if (r < rows) *reinterpret_cast<uint4*>(p + r * stride + (lane % P) * 16) = v;
+    for (int i = 0; i < P; ++i) {
+      const int r = i * (32 / P) + lane / P;
+      const uint4 v = lds_v4(piece_at<P>(smem, r, lane % P));
+      if (r < in.rows) *reinterpret_cast<uint4*>(p + r * stride + (lane % P) * 16) = v;
+    }
+  } else {
+    block_move<P, true>(p, stride, in, smem, lane);
   }
   __syncwarp();
 }
 template <int P>
-__device__ __forceinline__ void block_load(const uint8_t* p, int64_t stride, int rows, uint4 (&u)[P],
+__device__ __forceinline__ void block_load(const uint8_t* p, int64_t stride, const Inside& in, uint4 (&u)[P],
                                            uint32_t smem, int lane) {
+  if (in.shift == 4 && in.bytes == P * 16) {
 #pragma unroll
-  for (int i = 0; i < P; ++i) {
-    const int r = i * (32 / P) + lane / P;
-    u[i] = r < rows ? *reinterpret_cast<const uint4*>(p + r * stride + (lane % P) * 16) : make_uint4(0, 0, 0, 0);
+    for (int i = 0; i < P; ++i) {
+      const int r = i * (32 / P) + lane / P;
+      u[i] = r < in.rows ? *reinterpret_cast<const uint4*>(p + r * stride + (lane % P) * 16) : make_uint4(0, 0, 0, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, i * (32 / P) + lane / P, lane % P), u[i]);
+  } else {
+    block_move<P, false>(const_cast<uint8_t*>(p), stride, in, smem, lane);
   }
-#pragma unroll
-  for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, i * (32 / P) + lane / P, lane % P), u[i]);
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < P; ++i) u[i] = lds_v4(piece_at<P>(smem, lane, i));
   __syncwarp();
 }
 template <typename T>
-__device__ __forceinline__ void block_store_f32(T* p, int64_t ld, int rows, const float (&v)[32],
+__device__ __forceinline__ void block_store_f32(T* p, int64_t ld, const Inside& in, const float (&v)[32],
                                                 uint32_t smem, int lane) {
   constexpr int P = 2 * (int)sizeof(T);
   union { uint4 q[P]; T e[32]; } u;
 #pragma unroll
   for (int i = 0; i < 32; ++i) u.e[i] = from_f32<T>(v[i]);
-  block_store<P>(reinterpret_cast<uint8_t*>(p), ld * (int64_t)sizeof(T), rows, u.q, smem, lane);
+  block_store<P>(reinterpret_cast<uint8_t*>(p), ld * (int64_t)sizeof(T), in, u.q, smem, lane);
 }
 template <typename T>
-__device__ __forceinline__ void block_load_f32(const T* p, int64_t ld, int rows, float (&v)[32],
+__device__ __forceinline__ void block_load_f32(const T* p, int64_t ld, const Inside& in, float (&v)[32],
                                                uint32_t smem, int lane) {
   constexpr int P = 2 * (int)sizeof(T);
   union { uint4 q[P]; T e[32]; } u;
-  block_load<P>(reinterpret_cast<const uint8_t*>(p), ld * (int64_t)sizeof(T), rows, u.q, smem, lane);
+  block_load<P>(reinterpret_cast<const uint8_t*>(p), ld * (int64_t)sizeof(T), in, u.q, smem, lane);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = to_f32(u.e[i]);
 }
@@ -604,20 +638,19 @@ template <int P> __device__ __forceinline__ void pieces_to_words(const uint4 (&q
   for (int i = 0; i < P; ++i) { w[4 * i] = q[i].x; w[4 * i + 1] = q[i].y; w[4 * i + 2] = q[i].z; w[4 * i + 3] = q[i].w; }
 }
 
-// The epilogue of one block: rows row0 + lane, columns col .. col + 32.  Blocks
-// that reach past the last column or whose memory is not 16-byte aligned take
-// the row-per-lane form.
+// The epilogue of one block: rows row0 + lane, columns col .. col + 32, of which
+// those inside the matrix are touched.  Sums beyond its columns are zeros.
 template <typename T, int MODE>
 __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, int64_t col, float (&v)[32],
                                                uint32_t smem, int lane) {
   const bool packed = e.codes != nullptr;
-  if (!e.vec || col + 32 > e.cols || (packed && e.ckpt_align < 16)) {
-    epilogue<T, MODE, 32>(e, row0 + lane, col, v);
-    return;
-  }
   if (row0 >= e.rows) return;
   const int rows = e.rows - row0 < 32 ? (int)(e.rows - row0) : 32;
+  const int cols = e.cols - col < 32 ? (int)(e.cols - col) : 32;
   const int64_t at = row0 * e.cols + col;
+  // A T matrix without a wider alignment is aligned to its elements.
+  const int shift = e.align > (int)sizeof(T) ? align_shift(e.align) : (sizeof(T) == 4 ? 2 : 1);
+  const Inside in{rows, cols * (int)sizeof(T), shift};
   if (MODE == DW) {
     if (e.out_f32) {
       // 16 columns at a time: 2 KB of shared memory, as the 16-bit types have.
@@ -626,21 +659,24 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
         union { uint4 q[4]; float f[16]; } u;
 #pragma unroll
         for (int i = 0; i < 16; ++i) u.f[i] = v[16 * h + i];
-        block_store<4>(reinterpret_cast<uint8_t*>((float*)e.out + at + 16 * h), e.cols * 4, rows, u.q, smem, lane);
+        const int left = cols - 16 * h;
+        const Inside part{rows, left <= 0 ? 0 : (left < 16 ? left : 16) * 4, shift < 2 ? 2 : shift};
+        block_store<4>(reinterpret_cast<uint8_t*>((float*)e.out + at + 16 * h), e.cols * 4, part, u.q, smem, lane);
       }
     } else {
-      block_store_f32<T>((T*)e.out + at, e.cols, rows, v, smem, lane);
+      block_store_f32<T>((T*)e.out + at, e.cols, in, v, smem, lane);
     }
     return;
   }
+  const Inside in8{rows, cols, align_shift(e.ckpt_align)};
   if (MODE == FWD) {
     if (e.bias) {
       float t[32];
-      load_row<T, 32>((const T*)e.bias + col, 32, true, t);
+      load_row<T, 32>((const T*)e.bias + col, cols, e.bias_vec && cols == 32, t);
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += t[i];
     }
-    if (e.z) block_store_f32<T>((T*)e.z + at, e.cols, rows, v, smem, lane);
+    if (e.z) block_store_f32<T>((T*)e.z + at, e.cols, in, v, smem, lane);
     if (packed) {
       float amax = 0.0f;
 #pragma unroll
@@ -650,7 +686,7 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       if (lane < rows) e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP] = (uint8_t)x;
       union { uint4 q[2]; uint32_t w[8]; } u;
       ckpt_words<32>(v, amax, up, u.w);
-      block_store<2>(e.codes + at, e.cols, rows, u.q, smem, lane);
+      block_store<2>(e.codes + at, e.cols, in8, u.q, smem, lane);
     }
     apply_act<32>(e.act, v);
   } else if (packed || e.x) {
@@ -660,11 +696,11 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
     if (packed) {
       if (lane < rows) down = ckpt_down(e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP]);
       uint4 q[2];
-      block_load<2>(e.codes + at, e.cols, rows, q, smem, lane);
+      block_load<2>(e.codes + at, e.cols, in8, q, smem, lane);
       pieces_to_words<2>(q, codes);
     } else {
       uint4 q[P];
-      block_load<P>(reinterpret_cast<const uint8_t*>((const T*)e.x + at), e.cols * (int64_t)sizeof(T), rows, q, smem, lane);
+      block_load<P>(reinterpret_cast<const uint8_t*>((const T*)e.x + at), e.cols * (int64_t)sizeof(T), in, q, smem, lane);
       pieces_to_words<P>(q, x);
     }
     switch (e.act) {
@@ -678,16 +714,16 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       uint4 q[P];
 #pragma unroll
       for (int i = 0; i < P; ++i) q[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-      block_store<P>(reinterpret_cast<uint8_t*>((T*)e.a + at), e.cols * (int64_t)sizeof(T), rows, q, smem, lane);
+      block_store<P>(reinterpret_cast<uint8_t*>((T*)e.a + at), e.cols * (int64_t)sizeof(T), in, q, smem, lane);
     }
   }
   if (e.residual) {
     float t[32];
-    block_load_f32<T>((const T*)e.residual + at, e.cols, rows, t, smem, lane);
+    block_load_f32<T>((const T*)e.residual + at, e.cols, in, t, smem, lane);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] += t[i];
   }
-  block_store_f32<T>((T*)e.out + at, e.cols, rows, v, smem, lane);
+  block_store_f32<T>((T*)e.out + at, e.cols, in, v, smem, lane);
 }
 
 }  // namespace lin
