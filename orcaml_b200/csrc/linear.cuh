@@ -465,122 +465,110 @@ struct Inside {
 };
 __device__ __forceinline__ int align_shift(int align) { return 31 - __clz(align); }
 
-// Moves the block between shared memory and rows of any alignment, in units of
-// 1 << shift bytes: adjacent lanes take adjacent units.
-template <int P, bool STORE>
+__device__ __forceinline__ void lds_unit(uint32_t a, uint4& v) { v = lds_v4(a); }
+__device__ __forceinline__ void lds_unit(uint32_t a, uint2& v) {
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a));
+}
+__device__ __forceinline__ void lds_unit(uint32_t a, uint32_t& v) {
+  asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(a));
+}
+__device__ __forceinline__ void lds_unit(uint32_t a, uint16_t& v) {
+  asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(a));
+}
+__device__ __forceinline__ void lds_unit(uint32_t a, uint8_t& v) {
+  uint32_t w;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(w) : "r"(a));
+  v = (uint8_t)w;
+}
+__device__ __forceinline__ void sts_unit(uint32_t a, uint4 v) { sts_v4(a, v); }
+__device__ __forceinline__ void sts_unit(uint32_t a, uint2 v) {
+  asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(a), "r"(v.x), "r"(v.y) : "memory");
+}
+__device__ __forceinline__ void sts_unit(uint32_t a, uint32_t v) {
+  asm volatile("st.shared.b32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
+__device__ __forceinline__ void sts_unit(uint32_t a, uint16_t v) {
+  asm volatile("st.shared.b16 [%0], %1;" ::"r"(a), "h"(v) : "memory");
+}
+__device__ __forceinline__ void sts_unit(uint32_t a, uint8_t v) {
+  asm volatile("st.shared.u8 [%0], %1;" ::"r"(a), "r"((uint32_t)v) : "memory");
+}
+
+// Moves the block between shared memory and rows of the matrix in units of type U:
+// adjacent lanes take adjacent units, up to 8 of a lane's in flight.
+template <int P, bool STORE, typename U>
 __device__ __forceinline__ void block_move(uint8_t* p, int64_t stride, const Inside& in, uint32_t smem, int lane) {
-  constexpr int LOG = P == 8 ? 7 : (P == 4 ? 6 : 5);
-#pragma unroll 4
-  for (int i = lane; i < (32 * P * 16) >> in.shift; i += 32) {
-    const int r = i >> (LOG - in.shift), off = (i << in.shift) & (P * 16 - 1);
-    if (r >= in.rows || off >= in.bytes) continue;
-    const uint32_t at = piece_at<P>(smem, r, off >> 4) + (uint32_t)(off & 15);
-    uint8_t* g = p + r * stride + off;
+  constexpr int N = 32 * P * 16 / (int)sizeof(U), PER_ROW = P * 16 / (int)sizeof(U);
+  constexpr int AT_ONCE = N / 32 < 8 ? N / 32 : 8;
+#pragma unroll 1
+  for (int i0 = 0; i0 < N; i0 += 32 * AT_ONCE) {
+    U v[AT_ONCE];
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + u * 32 + lane, r = i / PER_ROW, off = i % PER_ROW * (int)sizeof(U);
+      if (STORE) lds_unit(piece_at<P>(smem, r, off >> 4) + (uint32_t)(off & 15), v[u]);
+      else v[u] = r < in.rows && off < in.bytes ? *reinterpret_cast<const U*>(p + r * stride + off) : U{};
+    }
+#pragma unroll
+    for (int u = 0; u < AT_ONCE; ++u) {
+      const int i = i0 + u * 32 + lane, r = i / PER_ROW, off = i % PER_ROW * (int)sizeof(U);
+      if (!STORE) sts_unit(piece_at<P>(smem, r, off >> 4) + (uint32_t)(off & 15), v[u]);
+      else if (r < in.rows && off < in.bytes) *reinterpret_cast<U*>(p + r * stride + off) = v[u];
+    }
+  }
+}
+// UNIT: bytes known to be aligned; 0: by in.shift.
+template <int P, bool STORE, int UNIT>
+__device__ __forceinline__ void block_move(uint8_t* p, int64_t stride, const Inside& in, uint32_t smem, int lane) {
+  if constexpr (UNIT == 16) {
+    block_move<P, STORE, uint4>(p, stride, in, smem, lane);
+  } else if constexpr (UNIT == 8) {
+    block_move<P, STORE, uint2>(p, stride, in, smem, lane);
+  } else {
     switch (in.shift) {
-      case 4:
-        if (STORE) *reinterpret_cast<uint4*>(g) = lds_v4(at);
-        else sts_v4(at, *reinterpret_cast<const uint4*>(g));
-        break;
-      case 3: {
-        uint2 v;
-        if (STORE) {
-          asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
-          *reinterpret_cast<uint2*>(g) = v;
-        } else {
-          v = *reinterpret_cast<const uint2*>(g);
-          asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(at), "r"(v.x), "r"(v.y) : "memory");
-        }
-        break;
-      }
-      case 2: {
-        uint32_t v;
-        if (STORE) {
-          asm volatile("ld.shared.b32 %0, [%1];" : "=r"(v) : "r"(at));
-          *reinterpret_cast<uint32_t*>(g) = v;
-        } else {
-          v = *reinterpret_cast<const uint32_t*>(g);
-          asm volatile("st.shared.b32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-        }
-        break;
-      }
-      case 1: {
-        uint16_t v;
-        if (STORE) {
-          asm volatile("ld.shared.b16 %0, [%1];" : "=h"(v) : "r"(at));
-          *reinterpret_cast<uint16_t*>(g) = v;
-        } else {
-          v = *reinterpret_cast<const uint16_t*>(g);
-          asm volatile("st.shared.b16 [%0], %1;" ::"r"(at), "h"(v) : "memory");
-        }
-        break;
-      }
-      default: {
-        uint32_t v;
-        if (STORE) {
-          asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(at));
-          *g = (uint8_t)v;
-        } else {
-          v = *g;
-          asm volatile("st.shared.u8 [%0], %1;" ::"r"(at), "r"(v) : "memory");
-        }
-      }
+      case 4: block_move<P, STORE, uint4>(p, stride, in, smem, lane); break;
+      case 3: block_move<P, STORE, uint2>(p, stride, in, smem, lane); break;
+      case 2: block_move<P, STORE, uint32_t>(p, stride, in, smem, lane); break;
+      case 1: block_move<P, STORE, uint16_t>(p, stride, in, smem, lane); break;
+      default: block_move<P, STORE, uint8_t>(p, stride, in, smem, lane);
     }
   }
 }
 
 // u: this lane's row, P pieces.
-template <int P>
+template <int P, int UNIT>
 __device__ __forceinline__ void block_store(uint8_t* p, int64_t stride, const Inside& in, const uint4 (&u)[P],
                                             uint32_t smem, int lane) {
 #pragma unroll
   for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, lane, i), u[i]);
   __syncwarp();
-  if (in.shift == 4 && in.bytes == P * 16) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int r = i * (32 / P) + lane / P;
-      const uint4 v = lds_v4(piece_at<P>(smem, r, lane % P));
-      if (r < in.rows) *reinterpret_cast<uint4*>(p + r * stride + (lane % P) * 16) = v;
-    }
-  } else {
-    block_move<P, true>(p, stride, in, smem, lane);
-  }
+  block_move<P, true, UNIT>(p, stride, in, smem, lane);
   __syncwarp();
 }
-template <int P>
+template <int P, int UNIT>
 __device__ __forceinline__ void block_load(const uint8_t* p, int64_t stride, const Inside& in, uint4 (&u)[P],
                                            uint32_t smem, int lane) {
-  if (in.shift == 4 && in.bytes == P * 16) {
-#pragma unroll
-    for (int i = 0; i < P; ++i) {
-      const int r = i * (32 / P) + lane / P;
-      u[i] = r < in.rows ? *reinterpret_cast<const uint4*>(p + r * stride + (lane % P) * 16) : make_uint4(0, 0, 0, 0);
-    }
-#pragma unroll
-    for (int i = 0; i < P; ++i) sts_v4(piece_at<P>(smem, i * (32 / P) + lane / P, lane % P), u[i]);
-  } else {
-    block_move<P, false>(const_cast<uint8_t*>(p), stride, in, smem, lane);
-  }
+  block_move<P, false, UNIT>(const_cast<uint8_t*>(p), stride, in, smem, lane);
   __syncwarp();
 #pragma unroll
   for (int i = 0; i < P; ++i) u[i] = lds_v4(piece_at<P>(smem, lane, i));
   __syncwarp();
 }
-template <typename T>
+template <typename T, int UNIT>
 __device__ __forceinline__ void block_store_f32(T* p, int64_t ld, const Inside& in, const float (&v)[32],
                                                 uint32_t smem, int lane) {
   constexpr int P = 2 * (int)sizeof(T);
   union { uint4 q[P]; T e[32]; } u;
 #pragma unroll
   for (int i = 0; i < 32; ++i) u.e[i] = from_f32<T>(v[i]);
-  block_store<P>(reinterpret_cast<uint8_t*>(p), ld * (int64_t)sizeof(T), in, u.q, smem, lane);
+  block_store<P, UNIT>(reinterpret_cast<uint8_t*>(p), ld * (int64_t)sizeof(T), in, u.q, smem, lane);
 }
-template <typename T>
+template <typename T, int UNIT>
 __device__ __forceinline__ void block_load_f32(const T* p, int64_t ld, const Inside& in, float (&v)[32],
                                                uint32_t smem, int lane) {
   constexpr int P = 2 * (int)sizeof(T);
   union { uint4 q[P]; T e[32]; } u;
-  block_load<P>(reinterpret_cast<const uint8_t*>(p), ld * (int64_t)sizeof(T), in, u.q, smem, lane);
+  block_load<P, UNIT>(reinterpret_cast<const uint8_t*>(p), ld * (int64_t)sizeof(T), in, u.q, smem, lane);
 #pragma unroll
   for (int i = 0; i < 32; ++i) v[i] = to_f32(u.e[i]);
 }
@@ -639,10 +627,13 @@ template <int P> __device__ __forceinline__ void pieces_to_words(const uint4 (&q
 }
 
 // The epilogue of one block: rows row0 + lane, columns col .. col + 32, of which
-// those inside the matrix are touched.  Sums beyond its columns are zeros.
-template <typename T, int MODE>
+// those inside the matrix are touched.  Sums beyond its columns are zeros.  ALIGNED:
+// rows of T are 16-byte aligned and those of codes 8-byte; a kernel of its own,
+// since the units of the other forms spill the registers of this one.
+template <typename T, int MODE, bool ALIGNED>
 __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, int64_t col, float (&v)[32],
                                                uint32_t smem, int lane) {
+  constexpr int UNIT = ALIGNED ? 16 : 0, UNIT8 = ALIGNED ? 8 : 0;
   const bool packed = e.codes != nullptr;
   if (row0 >= e.rows) return;
   const int rows = e.rows - row0 < 32 ? (int)(e.rows - row0) : 32;
@@ -661,10 +652,10 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
         for (int i = 0; i < 16; ++i) u.f[i] = v[16 * h + i];
         const int left = cols - 16 * h;
         const Inside part{rows, left <= 0 ? 0 : (left < 16 ? left : 16) * 4, shift < 2 ? 2 : shift};
-        block_store<4>(reinterpret_cast<uint8_t*>((float*)e.out + at + 16 * h), e.cols * 4, part, u.q, smem, lane);
+        block_store<4, UNIT>(reinterpret_cast<uint8_t*>((float*)e.out + at + 16 * h), e.cols * 4, part, u.q, smem, lane);
       }
     } else {
-      block_store_f32<T>((T*)e.out + at, e.cols, in, v, smem, lane);
+      block_store_f32<T, UNIT>((T*)e.out + at, e.cols, in, v, smem, lane);
     }
     return;
   }
@@ -676,7 +667,7 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] += t[i];
     }
-    if (e.z) block_store_f32<T>((T*)e.z + at, e.cols, in, v, smem, lane);
+    if (e.z) block_store_f32<T, UNIT>((T*)e.z + at, e.cols, in, v, smem, lane);
     if (packed) {
       float amax = 0.0f;
 #pragma unroll
@@ -686,7 +677,7 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       if (lane < rows) e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP] = (uint8_t)x;
       union { uint4 q[2]; uint32_t w[8]; } u;
       ckpt_words<32>(v, amax, up, u.w);
-      block_store<2>(e.codes + at, e.cols, in8, u.q, smem, lane);
+      block_store<2, UNIT8>(e.codes + at, e.cols, in8, u.q, smem, lane);
     }
     apply_act<32>(e.act, v);
   } else if (packed || e.x) {
@@ -696,11 +687,11 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
     if (packed) {
       if (lane < rows) down = ckpt_down(e.exps[(row0 + lane) * ckpt_groups(e.cols) + col / GROUP]);
       uint4 q[2];
-      block_load<2>(e.codes + at, e.cols, in8, q, smem, lane);
+      block_load<2, UNIT8>(e.codes + at, e.cols, in8, q, smem, lane);
       pieces_to_words<2>(q, codes);
     } else {
       uint4 q[P];
-      block_load<P>(reinterpret_cast<const uint8_t*>((const T*)e.x + at), e.cols * (int64_t)sizeof(T), in, q, smem, lane);
+      block_load<P, UNIT>(reinterpret_cast<const uint8_t*>((const T*)e.x + at), e.cols * (int64_t)sizeof(T), in, q, smem, lane);
       pieces_to_words<P>(q, x);
     }
     switch (e.act) {
@@ -714,16 +705,16 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       uint4 q[P];
 #pragma unroll
       for (int i = 0; i < P; ++i) q[i] = make_uint4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-      block_store<P>(reinterpret_cast<uint8_t*>((T*)e.a + at), e.cols * (int64_t)sizeof(T), in, q, smem, lane);
+      block_store<P, UNIT>(reinterpret_cast<uint8_t*>((T*)e.a + at), e.cols * (int64_t)sizeof(T), in, q, smem, lane);
     }
   }
   if (e.residual) {
     float t[32];
-    block_load_f32<T>((const T*)e.residual + at, e.cols, in, t, smem, lane);
+    block_load_f32<T, UNIT>((const T*)e.residual + at, e.cols, in, t, smem, lane);
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] += t[i];
   }
-  block_store_f32<T>((T*)e.out + at, e.cols, in, v, smem, lane);
+  block_store_f32<T, UNIT>((T*)e.out + at, e.cols, in, v, smem, lane);
 }
 
 }  // namespace lin

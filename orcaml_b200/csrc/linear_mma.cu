@@ -257,7 +257,7 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volati
 
 template <typename T> constexpr int plane_count() { return std::is_same<T, float>::value ? 3 : 1; }
 
-template <typename T, int MODE, int HALVES, int TN>
+template <typename T, int MODE, int HALVES, int TN, bool ALIGNED>
 __global__ void __launch_bounds__(Shape<HALVES, TN, plane_count<T>()>::THREADS, 1)
 pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
             const __grid_constant__ Params p) {
@@ -563,7 +563,7 @@ pair_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ C
           tmem_ld_32x32b_x32(lanes + (uint32_t)((buf + h) * ACC_COLS + q % S::BLOCKS * 32), v);
           if (q % S::BLOCKS == S::BLOCKS - 1) release(buf + h);     // read out: refill it
         }
-        if (c0 < p.N) block_epilogue<T, MODE>(p.e, row + h * 256, c0, v, block, lane);
+        if (c0 < p.N) block_epilogue<T, MODE, ALIGNED>(p.e, row + h * 256, c0, v, block, lane);
       }
     }
     if (!ok) raise_abort();
@@ -970,11 +970,11 @@ static Tail share(int64_t rest, int64_t steps, int64_t n, double step, int halve
 }
 
 // ---------------------------------------------------------------- launches
-template <typename T, int MODE, int HALVES, int TN>
+template <typename T, int MODE, int HALVES, int TN, bool ALIGNED>
 static orca_status launch_pair(orca_ctx* ctx, const Planes& a, const Planes& b, Params p) {
   constexpr int PLANES = plane_count<T>();
   using S = Shape<HALVES, TN, PLANES>;
-  const auto kernel = pair_kernel<T, MODE, HALVES, TN>;
+  const auto kernel = pair_kernel<T, MODE, HALVES, TN, ALIGNED>;
   CUtensorMap ma, mb;
   ORCA_TRY(make_map(&ma, a, PLANES, p.bf16, p.a_mn ? BK : ROWS));
   ORCA_TRY(make_map(&mb, b, PLANES, p.bf16, p.b_mn ? BK : TN / 2));
@@ -1119,10 +1119,10 @@ static orca_status consider(orca_ctx* ctx, const Params& p, int64_t steps, Plan*
 }
 
 template <typename T, int MODE>
-static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, Plan* plan) {
+static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, bool aligned, Plan* plan) {
   const int64_t n = ctx->sm_count / 2, blocks = cdiv(p.K, BK);
   plan->us = 1e30;
-  for (int shape = 0; shape < 3; ++shape) {
+  for (int shape = 0; shape < (aligned ? 3 : 1); ++shape) {
     const int halves = shape == 2 ? 2 : 1, tn = shape == 0 ? 128 : 256;
     // The two-accumulator tile has no F32 chunks.
     if (halves == 2 && (std::is_same<T, float>::value || p.chunk < steps)) break;
@@ -1150,18 +1150,21 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   p.chunk = dtype == ORCA_F32 ? F32_PAIRS
             : ((MODE == DW && p.e.out_f32) || (MODE == FWD && p.e.codes) ? CHUNK : (int)std::min<int64_t>(steps, MAX_CHUNK));
   Plan plan;
-  ORCA_TRY((choose<T, MODE>(ctx, p, steps, &plan)));
+  // Outputs without aligned rows have one tile shape.
+  const bool aligned = p.e.align == 16 && (!p.e.codes || p.e.ckpt_align >= 8);
+  ORCA_TRY((choose<T, MODE>(ctx, p, steps, aligned, &plan)));
   if constexpr (MODE != DW) {
     if (plan.nt == 16) return launch_split<T, MODE, 16>(ctx, a, b, planes, p, plan.ranks);
     if (plan.nt == 32) return launch_split<T, MODE, 32>(ctx, a, b, planes, p, plan.ranks);
   }
   if (plan.nt == 64) return launch_split<T, MODE, 64>(ctx, a, b, planes, p, plan.ranks);
   if (plan.nt == 128) return launch_split<T, MODE, 128>(ctx, a, b, planes, p, plan.ranks);
+  if (!aligned) return launch_pair<T, MODE, 1, 128, false>(ctx, a, b, p);
   if constexpr (!std::is_same<T, float>::value) {
-    if (plan.halves == 2) return launch_pair<T, MODE, 2, 256>(ctx, a, b, p);
+    if (plan.halves == 2) return launch_pair<T, MODE, 2, 256, true>(ctx, a, b, p);
   }
-  if (plan.tn == 128) return launch_pair<T, MODE, 1, 128>(ctx, a, b, p);
-  return launch_pair<T, MODE, 1, 256>(ctx, a, b, p);
+  if (plan.tn == 128) return launch_pair<T, MODE, 1, 128, true>(ctx, a, b, p);
+  return launch_pair<T, MODE, 1, 256, true>(ctx, a, b, p);
 }
 
 }  // namespace lin
