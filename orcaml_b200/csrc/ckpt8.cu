@@ -18,7 +18,9 @@ constexpr int THREADS = 256;
 // Rows of whole groups, 16-byte aligned: the matrix, its codes and its exponents
 // are three contiguous arrays.  A lane takes 8 values (pack) or 16 (unpack), with
 // all its loads in flight before the first is used: HBM needs ~44 KB in flight
-// per SM.
+// per SM.  4096 x 16384 BF16: pack 31.6 us (6.5 TB/s; before its arithmetic
+// shrank 39, with 2 steps 41, with 1 46), unpack 35 us, through GELU 43 (two operations of
+// the exponential and reciprocal units a value; 49 with 4 steps).
 constexpr int PACK_STEPS = 4, UNPACK_STEPS = 2;
 
 template <typename T>
