@@ -844,15 +844,28 @@ prepare_kernel(const __grid_constant__ Prepare job) {
       load_row<float, 8>(p, cols - c < 8 ? (int)(cols - c) : 8, whole, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const uint32_t b0 = __float_as_uint(v[j]) & 0xffff0000u;
+        const uint32_t bits = __float_as_uint(v[j]), b0 = bits & 0xffff0000u;
         const float r1 = v[j] - __uint_as_float(b0);
         const uint32_t b1 = __float_as_uint(r1) & 0xffff0000u;
         const float r2 = r1 - __uint_as_float(b1);
-        // An infinity or a NaN has no remainder: its first plane carries it.
-        const bool fine = (b0 & 0x7f800000u) != 0x7f800000u;
-        u[0].e[j] = (uint16_t)((fine ? b0 : (__float_as_uint(v[j]) | (v[j] != v[j] ? 0x400000u : 0u))) >> 16);
-        u[1].e[j] = fine ? (uint16_t)(b1 >> 16) : (uint16_t)0;
-        u[2].e[j] = fine ? (uint16_t)(__float_as_uint(r2) >> 16) : (uint16_t)0;
+        u[0].e[j] = (uint16_t)(b0 >> 16);
+        u[1].e[j] = (uint16_t)(b1 >> 16);
+        u[2].e[j] = (uint16_t)(__float_as_uint(r2) >> 16);
+        // Plane 2 meets only plane 0 of the other operand, so an infinity is carried there
+        // (planes +-1, 0, +-inf): meeting planes 1 and 2, which are zero for values of few
+        // bits, it would make NaN.  Plane 0 is zero for nothing but zero for the same reason:
+        // values below the smallest BF16 become that.
+        if ((bits & 0x7fffffffu) > 0x7f800000u) {
+          u[0].e[j] = (uint16_t)((bits >> 16) | 0x40u);
+          u[1].e[j] = u[2].e[j] = 0;
+        } else if ((bits & 0x7fffffffu) == 0x7f800000u) {
+          u[0].e[j] = (uint16_t)((bits >> 16 & 0x8000u) | 0x3f80u);
+          u[1].e[j] = 0;
+          u[2].e[j] = (uint16_t)(bits >> 16);
+        } else if ((b0 & 0x7fffffffu) == 0 && bits != b0) {
+          u[0].e[j] = (uint16_t)((b0 >> 16) | 1u);
+          u[1].e[j] = u[2].e[j] = 0;
+        }
       }
     } else {
       const uint16_t* p = (const uint16_t*)job.x[o] + r * cols + c;
