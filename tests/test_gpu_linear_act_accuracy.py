@@ -1,0 +1,39 @@
+"""How far F32 results of the feed-forward operators are from 64 bits, as norms
+over whole matrices of random operands: u = 2^-24.
+
+An accumulator of the tensor core loses up to 2 u of what it holds at each step of
+16 products, toward zero; 0.72 u on average over a binade.  Over n steps of a random
+walk those losses add up to 0.72 u n / sqrt(3) of the chain's norm, and chains are
+independent of one another.  Joining c chains in F32 adds u / sqrt(3) of the sum
+so far each time, together u sqrt(c / 6) of the result's.
+
+F32 operands: four steps of a 64-deep block add at full scale, 1.0e-7; 64 blocks
+(a sum of 4096) add 1.9e-7; the three plane products left out are 2^-24 of each
+product on average, toward zero, 0.6e-7.  As squares 2.2e-7 at 4096; the limit is 4e-7.  Leaving
+out one more plane product costs 1e-5.
+"""
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_gpu_linear_act import be, gen_of, rand, sp  # noqa: E402,F401
+
+pytestmark = pytest.mark.gpu
+
+
+def rel(got, want):
+    return float((got.double() - want).norm() / want.norm())
+
+
+# One row to several rounds of tiles, aligned rows and others.
+@pytest.mark.parametrize("m,k,n", [(1, 784, 1024), (16, 4096, 784), (64, 784, 517), (300, 4096, 520), (1100, 784, 1096),
+                                   (1100, 785, 1097), (2320, 4096, 2312)])
+def test_f32_products(be, m, k, n):  # noqa: F811
+    g = gen_of(m + k + n)
+    x, w, dy = rand(g, m, k), rand(g, k, n), rand(g, m, n)
+    out, dx, dw = (torch.full_like(v, 7.0) for v in (dy, x, w))
+    be.linear_act_fwd(sp(be, x), sp(be, w), None, m, k, n, out=sp(be, out))
+    be.linear_act_bwd(sp(be, x), sp(be, w), sp(be, dy), m, k, n, dx=sp(be, dx), dw=sp(be, dw), need_db=False)
+    x, w, dy = x.double(), w.double(), dy.double()
+    off = [rel(out, x @ w), rel(dx, dy @ w.t()), rel(dw, x.t() @ dy)]
+    assert max(off) <= 4e-7, off
