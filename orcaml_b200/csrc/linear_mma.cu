@@ -38,12 +38,16 @@ constexpr int F32_PAIRS = 6;
 //  first, so that only the last four MMAs add at full scale: off by 1.7e-7 of the
 //  result's norm (4096 x 784 x 8192; FMAs in F32: 6e-7), against 1.2e-6 after three
 //  blocks, which took 280 us instead of 298.
-//  F32 gradients and 8-bit checkpoints (whose codes flip with the sums' errors) of
-//  16-bit operands: after CHUNK steps.  4096-deep sums: 3.3e-7, against 1.8e-6 in one
-//  chain; the time is the same for gradients and 3 % more with a checkpoint.
+//  F32 gradients of 16-bit operands: after GRAD_CHUNK steps, off by 4.7e-7 of their norm
+//  whatever the sum's length (16 steps: 1.0e-6; 4: 2.4e-7; FMAs in F32: 2.5e-7 over
+//  1024 rows, 6.1e-7 over 4096, 1.5e-6 over 16384).  The backward of 4096 x 4096 x 16384
+//  takes 884 to 905 us, 0 to 1 % more than with 16 steps; with 4 it takes 3 % more.
+//  8-bit checkpoints, whose codes flip with the sums' errors: after CKPT_CHUNK steps,
+//  1.0e-6.  4096 x 4096 x 16384 with GELU and the checkpoint decoded takes 480 us, with 8 steps 504,
+//  with 4 530; half a code is 2^-8 of the group's largest value or more.
 //  Other results: none, up to MAX_CHUNK steps (30 ms), well inside the time limit of
 //  the waits.
-constexpr int CHUNK = 16, MAX_CHUNK = 65536;
+constexpr int GRAD_CHUNK = 8, CKPT_CHUNK = 16, MAX_CHUNK = 65536;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -1167,7 +1171,8 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   const int64_t steps = cdiv(p.K, BK) * p.pairs;
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
   p.chunk = dtype == ORCA_F32 ? F32_PAIRS
-            : ((MODE == DW && p.e.out_f32) || (MODE == FWD && p.e.codes) ? CHUNK : (int)std::min<int64_t>(steps, MAX_CHUNK));
+            : (MODE == DW && p.e.out_f32 ? GRAD_CHUNK
+            : (MODE == FWD && p.e.codes ? CKPT_CHUNK : (int)std::min<int64_t>(steps, MAX_CHUNK)));
   Plan plan;
   // Outputs without aligned rows have one tile shape.
   const bool aligned = p.e.align == 16 && (!p.e.codes || p.e.ckpt_align >= 8);
