@@ -266,7 +266,8 @@ orca_status orca_adamw_step(orca_ctx* ctx, orca_buf* p, const orca_buf* g, orca_
 /* ---- feed-forward operators: linear with activation and residual, 8-bit activation
  * checkpoints (no counterpart in the reference) -------------------------------------
  * Beside orca_linear_fwd / orca_linear_bwd: BF16, F16 and F32 operands (sums in
- * F32; F32 operands give F32-accurate products), any of the activations below,
+ * F32; F32 operands give F32-accurate products, each operand taken to its 24 bits
+ * or to 2^-133, whichever is coarser), any of the activations below,
  * a residual, and the pre-activation kept for the backward pass plainly or in
  * 8 bits.  Inputs and outputs are spans: memory of the context's device that
  * the caller owns (an orca_buf's orca_buf_device_ptr, or another allocator's),

@@ -2,8 +2,9 @@
 // tensor cores.
 //
 // BF16 and F16 operands go to tcgen05.mma kind::f16 as they are.  An F32 operand
-// is split exactly into three BF16 planes, x = x0 + x1 + x2 (8 significant bits
-// each, by truncation), and the product is the sum of six plane products,
+// is split into three BF16 planes, x = x0 + x1 + x2 (8 significant bits each, by
+// truncation; exact down to BF16's smallest step 2^-133, so all 24 bits of values
+// from 2^-110 up), and the product is the sum of six plane products,
 // x2*y0 + x0*y2 + x1*y1 + x1*y0 + x0*y1 + x0*y0; the three left out are below
 // 2^-21 of |x||y| together.  Both kinds run through the same kernels.
 //

@@ -19,7 +19,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_linear_act import TYPES, be, gen_of, rand, sp  # noqa: E402,F401
+from tests.test_gpu_linear_act import TYPES, be, check, gen_of, rand, sp, sum_error  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -51,3 +51,29 @@ def test_f32_gradients_of_16_bits(be, kind, m, k, n):  # noqa: F811
     dw = torch.full((k, n), 7.0, device="cuda")
     be.linear_act_bwd(sp(be, x), None, sp(be, dy), m, k, n, dw=sp(be, dw), need_dx=False, need_db=False)
     assert rel(dw, x.double().t() @ dy.double()) <= 8e-7
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -100, 2.0 ** -110, 1e-35, 1e-37, 1e-39, 1e-41])
+@pytest.mark.parametrize("m,k,n", [(4, 200, 136), (1100, 264, 1288), (1100, 265, 1287)])
+def test_small_f32_operands(be, m, k, n, scale):  # noqa: F811
+    """Each operand is off by 2^-133 at most, beside the sums' error; accumulators
+    that hold less than 2^-126 lose up to 2^-149 at each of 24 steps of a block."""
+    g = gen_of(m + k + n)
+    x, w = (rand(g, m, k).double() * scale).float(), rand(g, k, n)
+    out = torch.empty(m, n, device="cuda")
+    for a, b in ((x, w), (x.abs(), w.abs())):
+        be.linear_act_fwd(sp(be, a), sp(be, b), None, m, k, n, out=sp(be, out))
+        a, b = a.double(), b.double()
+        bound = sum_error(k, torch.float32) * (a.abs() @ b.abs()) + 24 * (k // 64 + 1) * 2.0 ** -149
+        check("out", out, a @ b, bound + 2.0 ** -133 * (b.abs().sum(0) + a.abs().sum(1)[:, None]))
+
+
+def test_f32_products_below_the_normal_range(be):  # noqa: F811
+    m, k, n = 70, 264, 136
+    g = gen_of(3)
+    x, w = ((rand(g, *s).double() * 2.0 ** -66).float() for s in ((m, k), (k, n)))
+    out = torch.empty(m, n, device="cuda")
+    be.linear_act_fwd(sp(be, x), sp(be, w), None, m, k, n, out=sp(be, out))
+    x, w = x.double(), w.double()
+    bound = sum_error(k, torch.float32) * (x.abs() @ w.abs()) + 24 * (k // 64 + 1) * 2.0 ** -149
+    check("out", out, x @ w, bound + 2.0 ** -133 * (w.abs().sum(0) + x.abs().sum(1)[:, None]))
