@@ -610,6 +610,12 @@ __device__ __forceinline__ float4 ld_cluster_f32x4(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ uint32_t ld_cluster_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr));
+  return v;
+}
+
 template <typename T, int MODE, int NT>
 __global__ void __launch_bounds__(SPLIT_THREADS, 1)
 split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ CUtensorMap map_q,
@@ -766,51 +772,54 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
   }
   if (ranks == 1) __syncthreads();
   else cluster_sync_all();
-  if (!*abort_flag) {
-    // A warp per row, 4 columns per lane; the parts of two rows, and what their
-    // epilogues read, are in flight at once.
-    constexpr int U = 2;
-    const int col = (int)col0 + lane * 4, j1 = NT * (rank + 1) / ranks;
-    ColumnEpilogue<T, MODE> ce(p.e, col);
-    for (int j = NT * rank / ranks + warp * U; j < j1 && row0 + j < p.M; j += SPLIT_THREADS / 32 * U) {
-      float v[U][4];
-      if (ranks == 1) {
+  // A CTA that gave up has no whole part, and none of its cluster stores sums with it.  The
+  // lanes fetch the flags beside the first parts.
+  uint32_t gave_up = (uint32_t)*abort_flag;
+  if (ranks > 1 && lane < ranks) gave_up = ld_cluster_u32(cluster_addr(const_cast<int*>(abort_flag), (uint32_t)lane));
+  // A warp per row, 4 columns per lane; the parts of two rows, and what their
+  // epilogues read, are in flight at once.
+  constexpr int U = 2;
+  const int col = (int)col0 + lane * 4, j1 = NT * (rank + 1) / ranks;
+  ColumnEpilogue<T, MODE> ce(p.e, col);
+  for (int j = NT * rank / ranks + warp * U; j < j1 && row0 + j < p.M; j += SPLIT_THREADS / 32 * U) {
+    float v[U][4];
+    if (ranks == 1) {
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const float4 x = *reinterpret_cast<const float4*>(part + (j + u < NT ? j + u : j) * 128 + lane * 4);
-          v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
-        }
-      } else {
-        float4 x[U][8];
+      for (int u = 0; u < U; ++u) {
+        const float4 x = *reinterpret_cast<const float4*>(part + (j + u < NT ? j + u : j) * 128 + lane * 4);
+        v[u][0] = x.x; v[u][1] = x.y; v[u][2] = x.z; v[u][3] = x.w;
+      }
+    } else {
+      float4 x[U][8];
 #pragma unroll
-        for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u)
 #pragma unroll
-          for (int r = 0; r < 8; ++r)
-            if (r < ranks)
-              x[u][r] = ld_cluster_f32x4(cluster_addr(part + (j + u < NT ? j + u : j) * 128 + lane * 4, (uint32_t)r));
+        for (int r = 0; r < 8; ++r)
+          if (r < ranks)
+            x[u][r] = ld_cluster_f32x4(cluster_addr(part + (j + u < NT ? j + u : j) * 128 + lane * 4, (uint32_t)r));
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-          v[u][0] = x[u][0].x; v[u][1] = x[u][0].y; v[u][2] = x[u][0].z; v[u][3] = x[u][0].w;
+      for (int u = 0; u < U; ++u) {
+        v[u][0] = x[u][0].x; v[u][1] = x[u][0].y; v[u][2] = x[u][0].z; v[u][3] = x[u][0].w;
 #pragma unroll
-          for (int r = 1; r < 8; ++r) {
-            if (r < ranks) {
-              v[u][0] = __fadd_rn(v[u][0], x[u][r].x);
-              v[u][1] = __fadd_rn(v[u][1], x[u][r].y);
-              v[u][2] = __fadd_rn(v[u][2], x[u][r].z);
-              v[u][3] = __fadd_rn(v[u][3], x[u][r].w);
-            }
+        for (int r = 1; r < 8; ++r) {
+          if (r < ranks) {
+            v[u][0] = __fadd_rn(v[u][0], x[u][r].x);
+            v[u][1] = __fadd_rn(v[u][1], x[u][r].y);
+            v[u][2] = __fadd_rn(v[u][2], x[u][r].z);
+            v[u][3] = __fadd_rn(v[u][3], x[u][r].w);
           }
         }
       }
-      // Rows past this CTA's share or the matrix are outside for the epilogue.
-      int64_t row[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) row[u] = j + u < j1 ? row0 + j + u : p.M;
-#pragma unroll
-      for (int u = 0; u < U; ++u) ce.load(u, row[u]);
-#pragma unroll
-      for (int u = 0; u < U; ++u) ce.store(u, row[u], v[u]);
     }
+    if (__any_sync(0xffffffffu, gave_up != 0)) break;
+    // Rows past this CTA's share or the matrix are outside for the epilogue.
+    int64_t row[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) row[u] = j + u < j1 ? row0 + j + u : p.M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) ce.load(u, row[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u) ce.store(u, row[u], v[u]);
   }
   __syncwarp();
   if (ranks == 1) return;
