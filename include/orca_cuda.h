@@ -78,7 +78,8 @@ orca_status orca_ctx_create(int device, orca_ctx** out);
  * legacy default stream) instead of a stream of its own, so that this
  * library's calls are ordered with the caller's other work without events and
  * can be captured into a CUDA graph with it.  The stream stays the caller's and
- * must outlive the context. */
+ * must outlive the context; a graph that holds captured calls must not be
+ * launched after the context is destroyed (its kernels report to the context). */
 orca_status orca_ctx_create_on_stream(int device, void* stream, orca_ctx** out);
 orca_status orca_ctx_destroy(orca_ctx* ctx);
 /* Wait for all enqueued work; ORCA_TIMEOUT after timeout_s seconds (<=0: 600 s). */
@@ -275,7 +276,11 @@ orca_status orca_adamw_step(orca_ctx* ctx, orca_buf* p, const orca_buf* g, orca_
  * allocated that outlives the call, so the calls can be captured into a CUDA
  * graph.  Outputs must not overlap inputs or one another, except that out (dx)
  * may be the residual's memory itself.  A call touches no more of a span than the sizes
- * say.  Memory must stay valid until the context's stream has passed the call. */
+ * say.  Memory must stay valid until the context's stream has passed the call.
+ * A device-side wait that runs out leaves results of its call unwritten, in a
+ * replayed graph too, and only orca_ctx_sync (or another call that waits for the
+ * device) on the same context reports it, ORCA_TIMEOUT: a caller who waits by means of
+ * its own calls that before it relies on what the operators wrote. */
 typedef struct {
   void* data;                /* device memory (NULL only when len is 0) */
   size_t len;                /* elements */
