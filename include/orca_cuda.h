@@ -111,6 +111,9 @@ void* orca_buf_device_ptr(const orca_buf* buf);
 /* ---- Backend trait methods (orca-tensor/src/backend.rs) -------------------- */
 orca_status orca_zeros(orca_ctx* ctx, const int64_t* dims, int rank, orca_dtype dtype,
                        orca_buf** out);                                       /* :27 */
+/* The same without the zeros: the contents are undefined until a call has written them. */
+orca_status orca_empty(orca_ctx* ctx, const int64_t* dims, int rank, orca_dtype dtype,
+                       orca_buf** out);
 orca_status orca_from_f32_slice(orca_ctx* ctx, const int64_t* dims, int rank,
                                 const float* data, orca_buf** out);           /* :31 */
 orca_status orca_to_f32_vec(orca_ctx* ctx, const orca_buf* buf, float* dst,

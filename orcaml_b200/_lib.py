@@ -90,6 +90,7 @@ _SIGS = {
     "orca_buf_dtype": ([c_void_p], c_int),
     "orca_buf_device_ptr": ([c_void_p], c_void_p),
     "orca_zeros": ([c_void_p, P_int64, c_int, c_int, PP], c_int),
+    "orca_empty": ([c_void_p, P_int64, c_int, c_int, PP], c_int),
     "orca_from_f32_slice": ([c_void_p, P_int64, c_int, c_void_p, PP], c_int),
     "orca_to_f32_vec": ([c_void_p, c_void_p, c_void_p, c_size_t], c_int),
     "orca_from_bytes": ([c_void_p, P_int64, c_int, c_void_p, c_size_t, c_int, PP], c_int),

@@ -118,6 +118,11 @@ class CudaBackend:
         d, r = L.dims(shape)
         return self._out(L.load().orca_zeros, d, r, int(dtype))
 
+    def empty(self, shape: Sequence[int], dtype: int = F32) -> CudaStorage:
+        """A storage whose contents are undefined until a call has written them."""
+        d, r = L.dims(shape)
+        return self._out(L.load().orca_empty, d, r, int(dtype))
+
     def from_f32_slice(self, shape: Sequence[int], data) -> CudaStorage:
         a = np.ascontiguousarray(data, dtype=np.float32).reshape(-1)
         if a.size != int(np.prod(shape, dtype=np.int64)):
@@ -271,7 +276,13 @@ class CudaBackend:
         return s
 
     def _result(self, out, numel, dtype):
-        return out if out is not None else self.zeros([int(numel)], dtype)
+        return out if out is not None else self.empty([int(numel)], dtype)
+
+    def _checkpoint(self, out, m, n):
+        # The kernels write codes and exponents, not the bytes between them.
+        if out is None and m * n % 16:
+            return self.zeros([self.ckpt8_bytes(m, n)], U8)
+        return self._result(out, self.ckpt8_bytes(m, n), U8)
 
     @staticmethod
     def _choice(table, value, what):
@@ -290,7 +301,7 @@ class CudaBackend:
         """The 8-bit checkpoint (U8) of x [m, n]: groups of 32 columns share a
         power of two, each value a signed 8-bit code."""
         x = self._span(x)
-        out = self._result(out, self.ckpt8_bytes(m, n), U8)
+        out = self._checkpoint(out, m, n)
         L.check(L.load().orca_ckpt8_pack(self._ctx, x, int(m), int(n), self._span(out)))
         return out
 
@@ -313,7 +324,7 @@ class CudaBackend:
         x = self._span(x)
         out = self._result(out, m * n, x.dtype)
         if kp:
-            z = self._result(z, m * n if kp == 1 else self.ckpt8_bytes(m, n), x.dtype if kp == 1 else U8)
+            z = self._result(z, m * n, x.dtype) if kp == 1 else self._checkpoint(z, m, n)
         L.check(L.load().orca_linear_act_fwd(self._ctx, x, self._span(w), self._span(b),
                                              self._span(residual), int(m), int(k), int(n), a,
                                              self._span(out), kp,

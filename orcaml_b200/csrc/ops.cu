@@ -543,6 +543,16 @@ orca_status orca_zeros(orca_ctx* ctx, const int64_t* dims, int rank, orca_dtype 
   return ORCA_OK;
 }
 
+orca_status orca_empty(orca_ctx* ctx, const int64_t* dims, int rank, orca_dtype dtype,
+                       orca_buf** out) {
+  ORCA_TRY(check_ctx(ctx));
+  LOCK(ctx);
+  ShapeInfo s;
+  int64_t n = 0;
+  ORCA_TRY(to_shape(dims, rank, s, &n));
+  return new_buf(ctx, (size_t)n, dtype, out);
+}
+
 orca_status orca_from_f32_slice(orca_ctx* ctx, const int64_t* dims, int rank, const float* data,
                                 orca_buf** out) {
   ORCA_TRY(check_ctx(ctx));

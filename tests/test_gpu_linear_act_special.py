@@ -109,3 +109,27 @@ def test_both_operands_infinite(be, rows):  # noqa: F811
     if m > 1:
         assert (out[1:, 0] == math.inf).all() and (out[1:, 1] == -math.inf).all()
         assert torch.equal(out[1:, 4:], torch.full_like(out[1:, 4:], k))
+
+
+@pytest.mark.parametrize("m,n", [(3, 33), (64, 40), (5, 31)])
+def test_new_checkpoints_have_all_their_bytes(be, m, n):  # noqa: F811
+    """Storages that the calls make, in memory that held other bytes before."""
+    import numpy as np
+    from tests.test_gpu_linear_act import encode
+    x = rand(gen_of(m), m, n)
+    size = be.ckpt8_bytes(m, n)
+    for _ in range(3):
+        dirty = be.from_bytes([size], b"\xff" * size, 6)
+        del dirty
+        ck = be.ckpt8_pack(sp(be, x), m, n)
+        assert np.array_equal(np.frombuffer(be.to_bytes(ck), np.uint8), encode(x))
+        del ck
+
+
+def test_empty_storage(be):  # noqa: F811
+    from orcaml_b200 import _lib as L
+    s = be.empty([3, 5])
+    assert len(s) == 15 and s.device_ptr
+    assert len(be.empty([0, 4])) == 0
+    with pytest.raises(L.OrcaError):
+        be.empty([3, -1])
