@@ -277,9 +277,10 @@ orca_status orca_adamw_step(orca_ctx* ctx, orca_buf* p, const orca_buf* g, orca_
  * the caller owns (an orca_buf's orca_buf_device_ptr, or another allocator's),
  * row-major and contiguous, of any alignment to whole elements.  Nothing is
  * allocated that outlives the call, so the calls can be captured into a CUDA
- * graph.  Outputs must not overlap inputs or one another, except that out (dx)
- * may be the residual's memory itself.  A call touches no more of a span than the sizes
- * say.  Memory must stay valid until the context's stream has passed the call.
+ * graph.  A call touches no more of a span than the sizes say, however long the span
+ * is, and nothing of an input that it does not read.  In the memory that it touches,
+ * outputs must not overlap inputs or one another, except that out (dx) may be the
+ * residual's memory itself.  Memory must stay valid until the context's stream has passed the call.
  * A device-side wait that runs out leaves results of its call unwritten, in a
  * replayed graph too, and only orca_ctx_sync (or another call that waits for the
  * device) on the same context reports it, ORCA_TIMEOUT: a caller who waits by means of

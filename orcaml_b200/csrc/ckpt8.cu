@@ -268,7 +268,7 @@ orca_status orca_ckpt8_pack(orca_ctx* ctx, const orca_span* x, int64_t m, int64_
   ORCA_TRY(need_float(x, "ckpt8_pack: x"));
   ORCA_TRY(need_span(ctx, ckpt, bytes, "ckpt8_pack: ckpt"));
   if (ckpt->dtype != ORCA_U8) return fail(ORCA_DTYPE_MISMATCH, "ckpt8_pack: ckpt must be U8");
-  ORCA_TRY(need_apart(ckpt, x, "ckpt8_pack: ckpt and x"));
+  ORCA_TRY(need_apart(used(ckpt, bytes), used(x, m * n), "ckpt8_pack: ckpt and x"));
   return ckpt8_pack_launch(ctx, x->data, x->dtype, m, n, (uint8_t*)ckpt->data);
 }
 
@@ -284,7 +284,7 @@ orca_status orca_ckpt8_unpack(orca_ctx* ctx, const orca_span* ckpt, int64_t m, i
   if (ckpt->dtype != ORCA_U8) return fail(ORCA_DTYPE_MISMATCH, "ckpt8_unpack: ckpt must be U8");
   ORCA_TRY(need_span(ctx, out, m * n, "ckpt8_unpack: out"));
   ORCA_TRY(need_float(out, "ckpt8_unpack: out"));
-  ORCA_TRY(need_apart(out, ckpt, "ckpt8_unpack: out and ckpt"));
+  ORCA_TRY(need_apart(used(out, m * n), used(ckpt, bytes), "ckpt8_unpack: out and ckpt"));
   return ckpt8_unpack_launch(ctx, (const uint8_t*)ckpt->data, m, n, act, out->data, out->dtype);
 }
 

@@ -42,10 +42,14 @@ orca_status need_span(orca_ctx* ctx, const orca_span* s, int64_t len, const char
   return ORCA_OK;
 }
 
-orca_status need_apart(const orca_span* out, const orca_span* other, const char* what) {
-  if (!out || !other || !out->len || !other->len) return ORCA_OK;
-  const uintptr_t a = reinterpret_cast<uintptr_t>(out->data), b = reinterpret_cast<uintptr_t>(other->data);
-  if (a < b + other->len * dtype_size(other->dtype) && b < a + out->len * dtype_size(out->dtype))
+Extent used(const orca_span* s, int64_t len) {
+  if (!s || len <= 0) return Extent{0, 0};
+  return Extent{reinterpret_cast<uintptr_t>(s->data), (size_t)len * dtype_size(s->dtype)};
+}
+
+orca_status need_apart(Extent out, Extent other, const char* what) {
+  if (!out.bytes || !other.bytes) return ORCA_OK;
+  if (out.at < other.at + other.bytes && other.at < out.at + out.bytes)
     return fail(ORCA_INVALID_ARGUMENT, "%s overlap", what);
   return ORCA_OK;
 }
@@ -276,8 +280,8 @@ static orca_status need_act(orca_act act, const char* what) {
 
 // out may be the residual's memory itself: each element is read before the
 // same thread writes it.
-static orca_status need_apart_or_same(const orca_span* out, const orca_span* residual, const char* what) {
-  if (out && residual && out->data == residual->data) return ORCA_OK;
+static orca_status need_apart_or_same(Extent out, Extent residual, const char* what) {
+  if (out.at == residual.at) return ORCA_OK;
   return need_apart(out, residual, what);
 }
 
@@ -316,14 +320,16 @@ orca_status orca_linear_act_fwd(orca_ctx* ctx, const orca_span* x, const orca_sp
     ORCA_TRY(need_span(ctx, z, packed ? (int64_t)orca_ckpt8_bytes(m, n) : m * n, "linear_act_fwd: z"));
     ORCA_TRY(need_type(z, packed ? ORCA_U8 : x->dtype, "linear_act_fwd: z"));
   }
-  for (const orca_span* o : {out, z}) {
-    ORCA_TRY(need_apart(o, x, "linear_act_fwd: an output and x"));
-    ORCA_TRY(need_apart(o, w, "linear_act_fwd: an output and w"));
-    ORCA_TRY(need_apart(o, b, "linear_act_fwd: an output and b"));
+  const Extent ux = used(x, m * k), uw = used(w, k * n), ub = used(b, n), ur = used(residual, m * n), uo = used(out, m * n);
+  const Extent uz = used(z, keep == ORCA_KEEP_CKPT8 ? (int64_t)orca_ckpt8_bytes(m, n) : m * n);
+  for (const Extent o : {uo, uz}) {
+    ORCA_TRY(need_apart(o, ux, "linear_act_fwd: an output and x"));
+    ORCA_TRY(need_apart(o, uw, "linear_act_fwd: an output and w"));
+    ORCA_TRY(need_apart(o, ub, "linear_act_fwd: an output and b"));
   }
-  ORCA_TRY(need_apart_or_same(out, residual, "linear_act_fwd: out and residual"));
-  ORCA_TRY(need_apart(z, residual, "linear_act_fwd: z and residual"));
-  ORCA_TRY(need_apart(out, z, "linear_act_fwd: out and z"));
+  ORCA_TRY(need_apart_or_same(uo, ur, "linear_act_fwd: out and residual"));
+  ORCA_TRY(need_apart(uz, ur, "linear_act_fwd: z and residual"));
+  ORCA_TRY(need_apart(uo, uz, "linear_act_fwd: out and z"));
   lin::Epilogue e;
   e.act = act;
   e.out = out->data;
@@ -352,13 +358,18 @@ orca_status orca_linear_act_bwd(orca_ctx* ctx, const orca_span* x, const orca_sp
   ORCA_TRY(need_span(ctx, dy, m * n, "linear_act_bwd: dy"));
   ORCA_TRY(need_float(dy, "linear_act_bwd: dy"));
   const orca_dtype t = dy->dtype;
+  Extent ux{0, 0}, uw{0, 0}, ur{0, 0};        // of what is read
   if (dw || (dx && act != ORCA_ACT_NONE)) {
     if (!x) return fail(ORCA_INVALID_ARGUMENT, "linear_act_bwd: x: null span");
     const bool packed = x->dtype == ORCA_U8;
-    ORCA_TRY(need_span(ctx, x, packed ? (int64_t)orca_ckpt8_bytes(m, k) : m * k, "linear_act_bwd: x"));
+    const int64_t len = packed ? (int64_t)orca_ckpt8_bytes(m, k) : m * k;
+    ORCA_TRY(need_span(ctx, x, len, "linear_act_bwd: x"));
     if (!packed) ORCA_TRY(need_type(x, t, "linear_act_bwd: x"));
+    ux = used(x, len);
   }
   if (dx) {
+    uw = used(w, k * n);
+    ur = used(residual, m * k);
     ORCA_TRY(need_span(ctx, w, k * n, "linear_act_bwd: w"));
     ORCA_TRY(need_type(w, t, "linear_act_bwd: w"));
     if (residual) {
@@ -376,17 +387,18 @@ orca_status orca_linear_act_bwd(orca_ctx* ctx, const orca_span* x, const orca_sp
     ORCA_TRY(need_span(ctx, db, n, "linear_act_bwd: db"));
     if (db->dtype != ORCA_F32) ORCA_TRY(need_type(db, t, "linear_act_bwd: db"));
   }
-  for (const orca_span* o : {dx, dw, db}) {
-    ORCA_TRY(need_apart(o, x, "linear_act_bwd: an output and x"));
-    ORCA_TRY(need_apart(o, w, "linear_act_bwd: an output and w"));
-    ORCA_TRY(need_apart(o, dy, "linear_act_bwd: an output and dy"));
+  const Extent uy = used(dy, m * n), ox = used(dx, m * k), ow = used(dw, k * n), ob = used(db, n);
+  for (const Extent o : {ox, ow, ob}) {
+    ORCA_TRY(need_apart(o, ux, "linear_act_bwd: an output and x"));
+    ORCA_TRY(need_apart(o, uw, "linear_act_bwd: an output and w"));
+    ORCA_TRY(need_apart(o, uy, "linear_act_bwd: an output and dy"));
   }
-  ORCA_TRY(need_apart_or_same(dx, residual, "linear_act_bwd: dx and residual"));
-  ORCA_TRY(need_apart(dw, residual, "linear_act_bwd: dw and residual"));
-  ORCA_TRY(need_apart(db, residual, "linear_act_bwd: db and residual"));
-  ORCA_TRY(need_apart(dx, dw, "linear_act_bwd: dx and dw"));
-  ORCA_TRY(need_apart(dx, db, "linear_act_bwd: dx and db"));
-  ORCA_TRY(need_apart(dw, db, "linear_act_bwd: dw and db"));
+  ORCA_TRY(need_apart_or_same(ox, ur, "linear_act_bwd: dx and residual"));
+  ORCA_TRY(need_apart(ow, ur, "linear_act_bwd: dw and residual"));
+  ORCA_TRY(need_apart(ob, ur, "linear_act_bwd: db and residual"));
+  ORCA_TRY(need_apart(ox, ow, "linear_act_bwd: dx and dw"));
+  ORCA_TRY(need_apart(ox, ob, "linear_act_bwd: dx and db"));
+  ORCA_TRY(need_apart(ow, ob, "linear_act_bwd: dw and db"));
   if (t == ORCA_F32) return lin::backward<float>(ctx, x, w, dy, residual, m, k, n, act, dx, dw, db);
   if (t == ORCA_F16) return lin::backward<__half>(ctx, x, w, dy, residual, m, k, n, act, dx, dw, db);
   return lin::backward<__nv_bfloat16>(ctx, x, w, dy, residual, m, k, n, act, dx, dw, db);

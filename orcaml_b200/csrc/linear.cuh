@@ -767,7 +767,13 @@ orca_status mma_product(orca_ctx* ctx, int mode, orca_dtype dtype, int64_t M, in
 
 // Checks of spans (linear.cu).
 orca_status need_span(orca_ctx* ctx, const orca_span* s, int64_t len, const char* what);
-orca_status need_apart(const orca_span* out, const orca_span* other, const char* what);
+// The memory of a span's first len elements: what a call touches of it.
+struct Extent {
+  uintptr_t at;
+  size_t bytes;
+};
+Extent used(const orca_span* s, int64_t len);
+orca_status need_apart(Extent out, Extent other, const char* what);
 orca_status need_float(const orca_span* s, const char* what);
 orca_status need_dim(int64_t v, const char* what);
 
