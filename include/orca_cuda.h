@@ -320,6 +320,8 @@ orca_status orca_ckpt8_unpack(orca_ctx* ctx, const orca_span* ckpt, int64_t m, i
 /* out = act(z) + residual with z = x @ w + b, in one pass: x [m, k], w [k, n]
  * ([in, out]), b [n] (nullable), residual [m, n] (nullable), all of one type;
  * bias, activation and residual are applied to the F32 sums and rounded once.
+ * Activations are F32 evaluations within 2^-21 of |z|, slopes (orca_linear_act_bwd)
+ * within 2^-21 of 1 + |z|.
  * keep says what is written to z (NULL for ORCA_KEEP_NONE): the
  * pre-activation in the operands' type, or its 8-bit checkpoint (U8), both of the
  * unrounded sums.  k = 0 gives z = b. */

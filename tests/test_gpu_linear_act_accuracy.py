@@ -19,7 +19,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_linear_act import TYPES, be, check, gen_of, rand, sp, sum_error  # noqa: E402,F401
+from tests.test_gpu_linear_act import TYPES, act64, be, check, gen_of, rand, slope64, sp, sum_error  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -77,3 +77,19 @@ def test_f32_products_below_the_normal_range(be):  # noqa: F811
     x, w = x.double(), w.double()
     bound = sum_error(k, torch.float32) * (x.abs() @ w.abs()) + 24 * (k // 64 + 1) * 2.0 ** -149
     check("out", out, x @ w, bound + 2.0 ** -133 * (w.abs().sum(0) + x.abs().sum(1)[:, None]))
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_activations_and_slopes_in_f32(be, act):  # noqa: F811
+    """Values within 2^-21 of |z| and slopes within 2^-21 of 1 + |z|, as the header
+    says; a sum of no products with the bias z is z itself, and with w = dy = 1 dx is the slope."""
+    z = torch.cat([torch.linspace(-12, 12, 2 ** 20 + 1, device="cuda"), rand(gen_of(1), 2 ** 18)])
+    n = z.numel()
+    none, one = be.span(None, 0, 0), torch.ones(1, device="cuda")
+    out, dx = torch.empty_like(z), torch.empty_like(z)
+    be.linear_act_fwd(none, none, sp(be, z), 1, 0, n, act=act, out=sp(be, out))
+    be.linear_act_bwd(sp(be, z), sp(be, one), sp(be, torch.ones_like(z)), n, 1, 1, act=act, dx=sp(be, dx), need_dw=False,
+                      need_db=False)
+    z = z.double()
+    check("value", out, act64(z, act), 2.0 ** -21 * z.abs() + 2.0 ** -126)
+    check("slope", dx, slope64(z, act), 2.0 ** -21 * (1 + z.abs()))
