@@ -29,7 +29,7 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 template <typename T, int V>
 __device__ __forceinline__ void load_row(const T* p, int valid, bool vec, float (&v)[V]) {
   constexpr int BYTES = V * (int)sizeof(T);
-  if (vec && V > 1) {
+  if (vec) {
     union { uint4 q[(BYTES + 15) / 16]; uint2 d; T e[V]; } u;
     if (BYTES >= 16) {
 #pragma unroll
@@ -48,7 +48,7 @@ __device__ __forceinline__ void load_row(const T* p, int valid, bool vec, float 
 template <typename T, int V>
 __device__ __forceinline__ void store_row(T* p, int valid, bool vec, const float (&v)[V]) {
   constexpr int BYTES = V * (int)sizeof(T);
-  if (vec && V > 1) {
+  if (vec) {
     union { uint4 q[(BYTES + 15) / 16]; uint2 d; T e[V]; } u;
 #pragma unroll
     for (int i = 0; i < V; ++i) u.e[i] = from_f32<T>(v[i]);
@@ -153,8 +153,7 @@ template <int ACT> __device__ __forceinline__ F2 act_value(F2 z) {
     return fma2(x, q, each(z, [](float v) { return fmaxf(v, 0.0f); }));
   }
   if (ACT == ORCA_ACT_GELU_TANH) return mul2(z, sigmoid2(tanh_arg(z)));
-  if (ACT == ORCA_ACT_SILU) return mul2(z, sigmoid2(z));
-  return z;
+  return mul2(z, sigmoid2(z));   // SiLU
 }
 template <int ACT> __device__ __forceinline__ F2 act_slope(F2 z) {
   if (ACT == ORCA_ACT_RELU) return each(z, [](float v) { return v > 0.0f ? 1.0f : 0.0f; });
@@ -176,11 +175,8 @@ template <int ACT> __device__ __forceinline__ F2 act_slope(F2 z) {
     const F2 r = fma2(mul2(mul2(y, s), fma2(s, f2(-1.0f), f2(1.0f))), up, s);
     return add2(r, fma2(z, f2(-1.0f), z));
   }
-  if (ACT == ORCA_ACT_SILU) {
-    const F2 s = sigmoid2(z);
-    return mul2(s, fma2(z, fma2(s, f2(-1.0f), f2(1.0f)), f2(1.0f)));
-  }
-  return f2(1.0f);
+  const F2 s = sigmoid2(z);      // SiLU
+  return mul2(s, fma2(z, fma2(s, f2(-1.0f), f2(1.0f)), f2(1.0f)));
 }
 
 // v = f(v), or v *= f'(z), for V values with one uniform branch for all.
@@ -279,7 +275,7 @@ __device__ __forceinline__ void ckpt_values(uint32_t word, float down, float* v)
 
 // Codes the V values of one lane, 32 / V adjacent lanes sharing a group (all
 // of them call this), and stores codes and exponent.  Columns from `valid` on
-// are outside.  `words`: 4-byte (V >= 4) stores are aligned; `quads`: 16-byte.
+// are outside.  V is 4 or 8; `align`: of the rows of codes, in bytes (16, 8, 4, 1).
 template <int V>
 __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_t row, int64_t n,
                                            int64_t col, int valid, bool row_ok, int align,
@@ -298,14 +294,8 @@ __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_
   uint32_t w[V / 4];
   ckpt_words<V>(v, amax, up, w);
   if (valid >= V && align >= 4) {
-    if (V >= 16 && align >= 16) {
-#pragma unroll
-      for (int i = 0; i < V / 16; ++i)
-        reinterpret_cast<uint4*>(p)[i] = make_uint4(w[4 * i], w[4 * i + 1], w[4 * i + 2], w[4 * i + 3]);
-    } else if (V >= 8 && align >= 8) {
-#pragma unroll
-      for (int i = 0; i < V / 8; ++i)
-        reinterpret_cast<uint2*>(p)[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+    if (V == 8 && align >= 8) {
+      *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[V / 4 - 1]);
     } else {
 #pragma unroll
       for (int i = 0; i < V / 4; ++i) reinterpret_cast<uint32_t*>(p)[i] = w[i];
@@ -317,28 +307,20 @@ __device__ __forceinline__ void ckpt_store(uint8_t* codes, uint8_t* exps, int64_
   }
 }
 
-// The V values at (row, col .. col + V) of a checkpoint; V divides 32 and col
-// is a multiple of V, so they share one exponent.
+// The V (4 or 8) values at (row, col .. col + V) of a checkpoint; col is a multiple of
+// V, so they share one exponent.
 template <int V>
 __device__ __forceinline__ void ckpt_load(const uint8_t* codes, const uint8_t* exps, int64_t row,
                                           int64_t n, int64_t col, int valid, int align,
                                           float (&v)[V]) {
   const float down = valid > 0 ? ckpt_down(exps[row * ckpt_groups(n) + col / GROUP]) : 0.0f;
   const uint8_t* p = codes + row * n + col;
-  if (V >= 4 && valid >= V && align >= 4) {
-    uint32_t w[(V + 3) / 4];
-    if (V >= 16 && align >= 16) {
-#pragma unroll
-      for (int i = 0; i < V / 16; ++i) {
-        const uint4 q = reinterpret_cast<const uint4*>(p)[i];
-        w[4 * i] = q.x; w[4 * i + 1] = q.y; w[4 * i + 2] = q.z; w[4 * i + 3] = q.w;
-      }
-    } else if (V >= 8 && align >= 8) {
-#pragma unroll
-      for (int i = 0; i < V / 8; ++i) {
-        const uint2 q = reinterpret_cast<const uint2*>(p)[i];
-        w[2 * i] = q.x; w[2 * i + 1] = q.y;
-      }
+  if (valid >= V && align >= 4) {
+    uint32_t w[V / 4];
+    if (V == 8 && align >= 8) {
+      const uint2 q = *reinterpret_cast<const uint2*>(p);
+      w[0] = q.x;
+      w[V / 4 - 1] = q.y;
     } else {
 #pragma unroll
       for (int i = 0; i < V / 4; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
@@ -702,8 +684,7 @@ __device__ __forceinline__ void block_epilogue(const Epilogue& e, int64_t row0, 
       case ORCA_ACT_RELU: slope_block<T, ORCA_ACT_RELU>(codes, packed, down, x, v); break;
       case ORCA_ACT_GELU: slope_block<T, ORCA_ACT_GELU>(codes, packed, down, x, v); break;
       case ORCA_ACT_GELU_TANH: slope_block<T, ORCA_ACT_GELU_TANH>(codes, packed, down, x, v); break;
-      case ORCA_ACT_SILU: slope_block<T, ORCA_ACT_SILU>(codes, packed, down, x, v); break;
-      default: slope_block<T, ORCA_ACT_NONE>(codes, packed, down, x, v);
+      default: slope_block<T, ORCA_ACT_SILU>(codes, packed, down, x, v);   // x is there with an activation only
     }
     if (e.a) {
       uint4 q[P];

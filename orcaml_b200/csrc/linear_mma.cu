@@ -46,8 +46,8 @@ constexpr int F32_PAIRS = 6;
 //  8-bit checkpoints, whose codes flip with the sums' errors: after CKPT_CHUNK steps,
 //  1.0e-6.  4096 x 4096 x 16384 with GELU and the checkpoint decoded takes 480 us, with 8 steps 504,
 //  with 4 530; half a code is 2^-8 of the group's largest value or more.
-//  Other results: none, up to MAX_CHUNK steps (30 ms), well inside the time limit of
-//  the waits.
+//  Other results: none, up to MAX_CHUNK steps (27 ms, 50 ms with 512-row tiles), well
+//  inside the time limit of the waits (2 s).
 constexpr int GRAD_CHUNK = 8, CKPT_CHUNK = 16, MAX_CHUNK = 65536;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
@@ -169,7 +169,7 @@ __device__ __forceinline__ void load_tile_pair(uint8_t* dst, const CUtensorMap* 
 }
 
 __device__ __forceinline__ void tile_at(int tile, int num_m, int num_n, int group_m, int& tm, int& tn) {
-  const int size = group_m * num_n;           // at most the tiles: below 2^31
+  const int size = group_m * num_n;           // group_m <= num_m: at most the tiles, below 2^31
   const int first = tile / size * group_m;
   const int gm = num_m - first < group_m ? num_m - first : group_m;
   const int r = tile % size;
@@ -1036,8 +1036,8 @@ static orca_status launch_pair(orca_ctx* ctx, const Planes& a, const Planes& b, 
   // stays in L2 (48 MB of 126), all its rows form one group and B is read once
   // (4096 x 4096 x 16384: 404 us against 416).
   const int64_t a_bytes = p.M * p.K * 2 * (p.pairs == 1 ? 1 : 3);
-  p.group_m = a_bytes <= (int64_t)48 << 20 ? (int)cdiv(p.M, S::M) : 2048 / S::M;
-  const int64_t tiles = cdiv(p.M, S::M) * cdiv(p.N, TN), n = fit.load();
+  const int64_t num_m = cdiv(p.M, S::M), tiles = num_m * cdiv(p.N, TN), n = fit.load();
+  p.group_m = (int)(a_bytes <= (int64_t)48 << 20 ? num_m : std::min<int64_t>(num_m, 2048 / S::M));
   const int64_t steps = cdiv(p.K, BK), rest = tiles % n;
   double us;
   const Tail tail = share(rest, steps, n, pair_step(HALVES, TN, PLANES), HALVES, &us);
