@@ -36,6 +36,9 @@ orca_status fail(orca_status s, const char* fmt, ...) {
   vsnprintf(buf, sizeof(buf), fmt, ap);
   va_end(ap);
   g_last_error = buf;
+  // The runtime keeps a refused call's error for whoever asks next: a later launch,
+  // ours or the caller's, would report it as its own.
+  if (s == ORCA_CUDA_ERROR) (void)cudaGetLastError();
   return s;
 }
 

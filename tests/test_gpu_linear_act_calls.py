@@ -87,3 +87,16 @@ def test_inputs_that_are_not_read(be):  # noqa: F811
     be.linear_act_bwd(sp(be, got), sp(be, got), sp(be, dy), M, K, N, act="relu", residual=sp(be, got), db=sp(be, got),
                       need_dx=False, need_dw=False)
     assert torch.equal(got, db)
+
+
+def test_a_failed_call_leaves_no_error_behind(be):  # noqa: F811
+    """An allocation that is refused (64 TiB) is reported by its own call, not by the
+    next launch of this library or of the caller's."""
+    from orcaml_b200 import _lib as L
+    x = rand(gen_of(4), M, K, t=T)
+    ck = torch.zeros(be.ckpt8_bytes(M, K), dtype=torch.uint8, device="cuda")
+    for after in (lambda: be.ckpt8_pack(sp(be, x), M, K, out=sp(be, ck)), lambda: x + 1):
+        with pytest.raises(L.OrcaError, match="allocation"):
+            be.empty([2 ** 44], 0)
+        after()
+    torch.cuda.synchronize()
