@@ -301,7 +301,8 @@ typedef enum {
 
 typedef enum { ORCA_KEEP_NONE = 0, ORCA_KEEP_Z = 1, ORCA_KEEP_CKPT8 = 2 } orca_keep;
 
-/* Bytes of the 8-bit checkpoint of an [m, n] matrix (0 for negative sizes): m*n
+/* Bytes of the 8-bit checkpoint of an [m, n] matrix (0 for negative sizes and for sizes
+ * near 2^31 and above, which no call takes): m*n
  * signed codes, row after row, then from the next multiple of 16 bytes one
  * exponent byte E per row and group of 32 columns (the last group of a row may
  * be shorter).  A code q stands for q * 2^(E - 127), exact in BF16.  Packing

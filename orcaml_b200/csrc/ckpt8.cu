@@ -254,7 +254,7 @@ static orca_status ckpt_bytes(int64_t m, int64_t n, int64_t* out, const char* wh
 extern "C" {
 
 size_t orca_ckpt8_bytes(int64_t m, int64_t n) {
-  if (m <= 0 || n <= 0) return 0;
+  if (m <= 0 || n <= 0 || m > MAX_DIM || n > MAX_DIM) return 0;
   return (size_t)(lin::ckpt_exps_at(m, n) + m * lin::ckpt_groups(n));
 }
 

@@ -9,8 +9,7 @@ namespace orca {
 
 // ---------------------------------------------------------------- checks
 orca_status need_dim(int64_t v, const char* what) {
-  // Below 2^31 a size fits the TMA coordinates and products of two stay far from 2^63.
-  if (v < 0 || v > INT32_MAX - 4096)
+  if (v < 0 || v > MAX_DIM)
     return fail(ORCA_INVALID_ARGUMENT, "%s: size %lld is out of range", what, (long long)v);
   return ORCA_OK;
 }

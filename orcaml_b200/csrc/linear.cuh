@@ -761,5 +761,6 @@ Extent used(const orca_span* s, int64_t len);
 orca_status need_apart(Extent out, Extent other, const char* what);
 orca_status need_float(const orca_span* s, const char* what);
 orca_status need_dim(int64_t v, const char* what);
+constexpr int64_t MAX_DIM = INT32_MAX - 4096;   // sizes fit the TMA coordinates, products of two stay far from 2^63
 
 }  // namespace orca

@@ -19,6 +19,11 @@ class Recorder:
         return call
 
 
+@pytest.mark.parametrize("m,n,want", [(2 ** 40, 2 ** 40, 0), (2 ** 33, 1, 0), (1, 2 ** 31, 0), (2 ** 31 - 4097, 32, (2 ** 31 - 4097) * 33)])
+def test_checkpoint_bytes_of_sizes_that_no_call_takes(m, n, want):
+    assert CudaBackend.ckpt8_bytes(m, n) == want
+
+
 @pytest.fixture
 def be(monkeypatch):
     b = CudaBackend.__new__(CudaBackend)
