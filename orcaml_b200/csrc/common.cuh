@@ -115,13 +115,14 @@ __host__ __device__ inline int64_t cdiv(int64_t a, int64_t b) { return (a + b - 
 // Split of an fp32 value into a TF32-exact high part (round to nearest, ties
 // away, on the 10 explicit mantissa bits kept) and the exact fp32 residual:
 // x == hi + lo bit-exactly.  Three TF32 products hi*hi + hi*lo + lo*hi give an
-// fp32-accurate product.
+// fp32-accurate product.  An infinity is +-1 and +-inf (a NaN +-1 and NaN): as a low
+// part it meets only the other operand's high part, which is zero for nothing from
+// 2^-137 up, while its low part is zero for any value of few bits and would make NaN.
 __device__ __forceinline__ float tf32_hi(float x) {
-  uint32_t u = __float_as_uint(x);
-  if ((u & 0x7f800000u) == 0x7f800000u) return x;         // inf / nan unchanged
-  uint32_t r = (u + 0x1000u) & 0xffffe000u;
-  if ((r & 0x7f800000u) == 0x7f800000u) r = u & 0xffffe000u;  // would overflow: truncate
-  return __uint_as_float(r);
+  const uint32_t u = __float_as_uint(x), a = u & 0x7fffffffu;
+  uint32_t r = min((a + 0x1000u) & 0xffffe000u, 0x7f7fe000u);   // would overflow: truncate
+  if (a >= 0x7f800000u) r = 0x3f800000u;
+  return __uint_as_float(r | (u & 0x80000000u));
 }
 
 __device__ __forceinline__ void split_tf32(float x, float& hi, float& lo) {
