@@ -46,9 +46,12 @@ constexpr int F32_PAIRS = 6;
 //  8-bit checkpoints, whose codes flip with the sums' errors: after CKPT_CHUNK steps,
 //  1.0e-6.  4096 x 4096 x 16384 with GELU and the checkpoint decoded takes 480 us, with 8 steps 504,
 //  with 4 530; half a code is 2^-8 of the group's largest value or more.
-//  Other results: none, up to MAX_CHUNK steps (27 ms, 50 ms with 512-row tiles), well
-//  inside the time limit of the waits (2 s).
-constexpr int GRAD_CHUNK = 8, CKPT_CHUNK = 16, MAX_CHUNK = 65536;
+//  16-bit results: after F16_CHUNK or BF16_CHUNK steps, off by 3e-5 or 2.5e-4 of the norm, an
+//  eighth of what rounding them is off by (2.1e-4 and 1.7e-3; over 2^20 rows one chain
+//  was off by 2.5e-4 in either type).  Sums of up to 32768 and 262144 rows are one chain in any
+//  case, which 512-row tiles need: dW of 2048 x 1024 over 2^20 rows takes 3.5 ms in BF16 and, from
+//  smaller tiles, 4.6 in F16.
+constexpr int GRAD_CHUNK = 8, CKPT_CHUNK = 16, F16_CHUNK = 512, BF16_CHUNK = 4096;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride
@@ -1042,6 +1045,7 @@ static orca_status launch_pair(orca_ctx* ctx, const Planes& a, const Planes& b, 
   double us;
   const Tail tail = share(rest, steps, n, pair_step(HALVES, TN, PLANES), HALVES, &us);
   if (PLANES == 3) p.chunk = 1;            // in 64-deep blocks here
+  if (HALVES == 2) p.chunk = (int)steps;   // one chain
   if (tiles > INT32_MAX - 4096) return fail(ORCA_INVALID_ARGUMENT, "linear: too many tiles");
   p.full = (int)tiles;
   p.tail = 0;
@@ -1157,12 +1161,12 @@ static orca_status choose(orca_ctx* ctx, const Params& p, int64_t steps, bool al
   plan->us = 1e30;
   for (int shape = 0; shape < (aligned ? 3 : 1); ++shape) {
     const int halves = shape == 2 ? 2 : 1, tn = shape == 0 ? 128 : 256;
-    // The two-accumulator tile has no F32 chunks.
-    if (halves == 2 && (std::is_same<T, float>::value || p.chunk < steps)) break;
     const int64_t tiles = cdiv(p.M, 256 * halves) * cdiv(p.N, tn);
     const double step = pair_step(halves, tn, plane_count<T>());
     double us;
-    share(tiles % n, blocks, n, step, halves, &us);
+    const Tail tail = share(tiles % n, blocks, n, step, halves, &us);
+    // The two-accumulator tile has no chunks: a tile, or a cluster's share of one, is one chain.
+    if (halves == 2 && (std::is_same<T, float>::value || p.chunk < (tiles < n ? tail.steps : blocks))) break;
     us += (double)(tiles / n * blocks) * step + (double)cdiv(tiles, n) * (halves == 2 ? drain_cost(MODE) : 0.0) +
           (tn == 256 ? 8.0 : 7.0);
     if (us < plan->us) *plan = Plan{0, halves, tn, 1, us};
@@ -1182,7 +1186,8 @@ static orca_status dispatch(orca_ctx* ctx, orca_dtype dtype, const Planes& a, co
   if (steps > INT32_MAX) return fail(ORCA_INVALID_ARGUMENT, "linear: the sum is too long");
   p.chunk = dtype == ORCA_F32 ? F32_PAIRS
             : (MODE == DW && p.e.out_f32 ? GRAD_CHUNK
-            : (MODE == FWD && p.e.codes ? CKPT_CHUNK : (int)std::min<int64_t>(steps, MAX_CHUNK)));
+            : (MODE == FWD && p.e.codes ? CKPT_CHUNK
+            : (int)std::min<int64_t>(steps, dtype == ORCA_F16 ? F16_CHUNK : BF16_CHUNK)));
   Plan plan;
   // Outputs without aligned rows have one tile shape.
   const bool aligned = p.e.align == 16 && (!p.e.codes || p.e.ckpt_align >= 8);

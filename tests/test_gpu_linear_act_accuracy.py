@@ -93,3 +93,17 @@ def test_activations_and_slopes_in_f32(be, act):  # noqa: F811
     z = z.double()
     check("value", out, act64(z, act), 2.0 ** -21 * z.abs() + 2.0 ** -126)
     check("slope", dx, slope64(z, act), 2.0 ** -21 * (1 + z.abs()))
+
+
+@pytest.mark.parametrize("m,k,n", [(2 ** 15 + 64, 512, 512), (2 ** 20, 512, 512), (2 ** 20 + 5, 1024, 520), (2 ** 20, 64, 64)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_16_bit_results_of_long_sums(be, kind, m, k, n):  # noqa: F811
+    """Chains of 2048 (F16) and 16384 (BF16) steps are off by 0.72 u * steps / sqrt(3) of the norm,
+    5.1e-5 and 4.1e-4; beside the rounding, 2.1e-4 and 1.7e-3 rms, that is 3 % more, as squares."""
+    t = TYPES[kind]
+    g = gen_of(5)
+    x, dy = rand(g, m, k, t=t), rand(g, m, n, scale=1 / 64, t=t)
+    dw = torch.full((k, n), 7.0, dtype=t, device="cuda")
+    be.linear_act_bwd(sp(be, x), None, sp(be, dy), m, k, n, dw=sp(be, dw), need_dx=False, need_db=False)
+    want = sum(x[i:i + 2 ** 16, :64].double().t() @ dy[i:i + 2 ** 16].double() for i in range(0, m, 2 ** 16))
+    assert rel(dw[:64], want) <= 1.05 * rel(want.to(t), want)
