@@ -283,8 +283,8 @@ orca_status orca_adamw_step(orca_ctx* ctx, orca_buf* p, const orca_buf* g, orca_
  * residual's memory itself.  Memory must stay valid until the context's stream has passed the call.
  * A device-side wait that runs out leaves results of its call unwritten, in a
  * replayed graph too, and only orca_ctx_sync (or another call that waits for the
- * device) on the same context reports it, ORCA_TIMEOUT: a caller who waits by means of
- * its own calls that before it relies on what the operators wrote. */
+ * device) on the same context reports it, ORCA_TIMEOUT.  A caller who waits by means of
+ * its own makes that call too before it relies on what the operators wrote. */
 typedef struct {
   void* data;                /* device memory (NULL only when len is 0) */
   size_t len;                /* elements */
@@ -297,7 +297,8 @@ typedef enum {
   ORCA_ACT_GELU = 2,         /* z (1 + erf(z / sqrt 2)) / 2 */
   ORCA_ACT_GELU_TANH = 3,    /* z (1 + tanh(sqrt(2 / pi) (z + 0.044715 z^3))) / 2 */
   ORCA_ACT_SILU = 4          /* z / (1 + exp(-z)) */
-} orca_act;
+} orca_act;                  /* at +inf: inf; at -inf: 0 (RELU, GELU) or NaN (GELU_TANH, SILU, as written);
+                              * slopes at infinities: 1 and 0 (RELU), NaN else */
 
 typedef enum { ORCA_KEEP_NONE = 0, ORCA_KEEP_Z = 1, ORCA_KEEP_CKPT8 = 2 } orca_keep;
 

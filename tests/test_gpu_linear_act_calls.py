@@ -4,7 +4,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_linear_act import be, code_of, gen_of, rand, sp  # noqa: E402,F401
+from tests.test_gpu_linear_act import TYPES, be, code_of, gen_of, rand, sp  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -100,3 +100,16 @@ def test_a_failed_call_leaves_no_error_behind(be):  # noqa: F811
             be.empty([2 ** 44], 0)
         after()
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("m,k,n", [(3, 64, 96), (33, 21, 50), (300, 264, 72), (1100, 1287, 264), (2320, 2312, 4104)])
+@pytest.mark.parametrize("kind", ["bf16", "f32"])
+def test_dx_may_be_the_residual(be, kind, m, k, n):  # noqa: F811
+    t = TYPES[kind]
+    g = gen_of(m)
+    x, w, dy, r = rand(g, m, k, t=t), rand(g, k, n, t=t), rand(g, m, n, t=t), rand(g, m, k, t=t)
+    dx = torch.empty_like(r)
+    for out in (dx, r):
+        be.linear_act_bwd(sp(be, x), sp(be, w), sp(be, dy), m, k, n, act="silu", residual=sp(be, r), dx=sp(be, out),
+                          need_dw=False, need_db=False)
+    assert torch.equal(r, dx)

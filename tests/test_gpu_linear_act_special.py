@@ -133,3 +133,23 @@ def test_empty_storage(be):  # noqa: F811
     assert len(be.empty([0, 4])) == 0
     with pytest.raises(L.OrcaError):
         be.empty([3, -1])
+
+
+@pytest.mark.parametrize("act,below", [("relu", 0.0), ("gelu", 0.0), ("gelu_tanh", math.nan), ("silu", math.nan)])
+@pytest.mark.parametrize("kind", list(TYPES))
+def test_activations_and_slopes_at_infinities(be, kind, act, below):  # noqa: F811
+    """As the header says: +inf stays, -inf gives 0 or NaN, slopes are NaN but ReLU's."""
+    t = TYPES[kind]
+    z = torch.tensor([math.inf, -math.inf, math.nan, 1.0] * 40, device="cuda").to(t)
+    none, one = be.span(None, 0, sp(be, z).dtype), torch.ones(1, device="cuda").to(t)
+    out, dx = torch.empty_like(z), torch.empty_like(z)
+    be.linear_act_fwd(none, none, sp(be, z), 1, 0, len(z), act=act, out=sp(be, out))
+    be.linear_act_bwd(sp(be, z), sp(be, one), sp(be, torch.ones_like(z)), len(z), 1, 1, act=act, dx=sp(be, dx), need_dw=False,
+                      need_db=False)
+    nan = math.nan
+    want = [math.inf, below, 0.0 if act == "relu" else nan]
+    slope = [1.0, 0.0, 0.0] if act == "relu" else [nan, nan, nan]
+    for got, w in ((out, want), (dx, slope)):
+        got = got.view(-1, 4)[:, :3].float()
+        w = torch.tensor(w, device="cuda").expand_as(got)
+        assert torch.equal(torch.nan_to_num(got, nan=7.0, posinf=8.0), torch.nan_to_num(w, nan=7.0, posinf=8.0))
