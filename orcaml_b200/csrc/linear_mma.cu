@@ -44,14 +44,16 @@ constexpr int F32_PAIRS = 6;
 //  1024 rows, 6.1e-7 over 4096, 1.5e-6 over 16384).  The backward of 4096 x 4096 x 16384
 //  takes 884 to 905 us, 0 to 1 % more than with 16 steps; with 4 it takes 3 % more.
 //  8-bit checkpoints, whose codes flip with the sums' errors: after CKPT_CHUNK steps,
-//  1.0e-6.  4096 x 4096 x 16384 with GELU and the checkpoint decoded takes 480 us, with 8 steps 504,
-//  with 4 530; half a code is 2^-8 of the group's largest value or more.
+//  5.9e-7, as many flips as after FMAs in F32 (values off by 1.11e-4 of the norm beside the
+//  rounding to codes, after 16 steps 1.42e-4).  4096 x 4096 x 16384 with GELU and the checkpoint decoded
+//  takes 506 us, 494 with 16 steps, 512 with 8: the drains of short chunks wait for the
+//  epilogue of the tile before.
 //  16-bit results: after F16_CHUNK or BF16_CHUNK steps, off by 3e-5 or 2.5e-4 of the norm, an
 //  eighth of what rounding them is off by (2.1e-4 and 1.7e-3; over 2^20 rows one chain
 //  was off by 2.5e-4 in either type).  Sums of up to 32768 and 262144 rows are one chain in any
 //  case, which 512-row tiles need: dW of 2048 x 1024 over 2^20 rows takes 3.5 ms in BF16 and, from
 //  smaller tiles, 4.6 in F16.
-constexpr int GRAD_CHUNK = 8, CKPT_CHUNK = 16, F16_CHUNK = 512, BF16_CHUNK = 4096;
+constexpr int GRAD_CHUNK = 8, CKPT_CHUNK = 10, F16_CHUNK = 512, BF16_CHUNK = 4096;
 
 // Shared-memory matrix descriptors for the 128-byte swizzle (layout code 2).
 //  K-major: row r at 128 * r bytes, 8-row groups 1024 bytes apart (stride

@@ -19,7 +19,7 @@ import pytest
 
 torch = pytest.importorskip("torch")
 
-from tests.test_gpu_linear_act import TYPES, act64, be, check, gen_of, rand, slope64, sp, sum_error  # noqa: E402,F401
+from tests.test_gpu_linear_act import TYPES, act64, be, check, decode, gen_of, rand, slope64, sp, sum_error  # noqa: E402,F401
 
 pytestmark = pytest.mark.gpu
 
@@ -107,3 +107,21 @@ def test_16_bit_results_of_long_sums(be, kind, m, k, n):  # noqa: F811
     be.linear_act_bwd(sp(be, x), None, sp(be, dy), m, k, n, dw=sp(be, dw), need_dx=False, need_db=False)
     want = sum(x[i:i + 2 ** 16, :64].double().t() @ dy[i:i + 2 ** 16].double() for i in range(0, m, 2 ** 16))
     assert rel(dw[:64], want) <= 1.05 * rel(want.to(t), want)
+
+
+@pytest.mark.parametrize("m,k,n", [(2048, 4096, 4096), (2048, 4099, 4103)])
+def test_codes_that_flip(be, m, k, n):  # noqa: F811
+    """A code differs from the exact sum's where a border lies within the sum's error: in
+    |error| / step of the elements, |error| being 0.8 of 5.9e-7 of the norm on average.  Counted with four
+    standard deviations."""
+    g = gen_of(k)
+    x, w = rand(g, m, k, t=torch.bfloat16), rand(g, k, n, scale=k ** -0.5, t=torch.bfloat16)
+    z = torch.zeros(be.ckpt8_bytes(m, n), dtype=torch.uint8, device="cuda")
+    out = torch.empty(m, n, dtype=torch.bfloat16, device="cuda")
+    be.linear_act_fwd(sp(be, x), sp(be, w), None, m, k, n, keep="ckpt8", out=sp(be, out), z=sp(be, z))
+    got, step = decode(z, m, n)
+    z64 = x.double() @ w.double()
+    want = (z64 / step).round().clamp(-127, 127) * step
+    flips = int((got != want).sum())
+    expected = float((0.8 * 5.9e-7 * z64.pow(2).mean().sqrt() / step).sum())
+    assert flips <= expected + 4 * expected ** 0.5, (flips, expected)
