@@ -211,7 +211,8 @@ static orca_status backward(orca_ctx* ctx, const orca_span* x, const orca_span* 
                             const orca_span* db) {
   constexpr orca_dtype dtype = dtype_of<T>();
   const bool packed = x && x->dtype == ORCA_U8;
-  // dW's operand a = act(x): x itself, or a matrix that the epilogue of the dX
+  // dW's operand a = act(x), rounded to T as the forward pass rounded it (in more bits it
+  // would take a second plane, twice the product): x itself, or a matrix that the epilogue of the dX
   // product writes on the way where it reads x for the slope (4096 x 16384 GELU:
   // 935 us against 963 with a pass of its own), or a pass of its own (without an
   // activation: 919 us against 931).

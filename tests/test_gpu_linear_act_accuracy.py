@@ -30,7 +30,7 @@ def rel(got, want):
 
 # One row to several rounds of tiles, aligned rows and others.
 @pytest.mark.parametrize("m,k,n", [(1, 784, 1024), (16, 4096, 784), (64, 784, 517), (300, 4096, 520), (1100, 784, 1096),
-                                   (1100, 785, 1097), (2320, 4096, 2312)])
+                                   (1100, 785, 1097), (2320, 4096, 2312), (2320, 785, 2313)])
 def test_f32_products(be, m, k, n):  # noqa: F811
     g = gen_of(m + k + n)
     x, w, dy = rand(g, m, k), rand(g, k, n), rand(g, m, n)
@@ -42,8 +42,8 @@ def test_f32_products(be, m, k, n):  # noqa: F811
     assert max(off) <= 4e-7, off
 
 
-@pytest.mark.parametrize("m,k,n", [(1024, 512, 520), (4096, 1024, 1096), (4096, 513, 259), (16384, 512, 520),
-                                   (16384, 2048, 2056)])
+@pytest.mark.parametrize("m,k,n", [(1024, 512, 520), (4096, 1024, 1096), (4096, 513, 259), (4096, 2049, 2055),
+                                   (16384, 512, 520), (16384, 2048, 2056)])
 @pytest.mark.parametrize("kind", ["bf16", "f16"])
 def test_f32_gradients_of_16_bits(be, kind, m, k, n):  # noqa: F811
     g = gen_of(m + k)
@@ -125,3 +125,19 @@ def test_codes_that_flip(be, m, k, n):  # noqa: F811
     flips = int((got != want).sum())
     expected = float((0.8 * 5.9e-7 * z64.pow(2).mean().sqrt() / step).sum())
     assert flips <= expected + 4 * expected ** 0.5, (flips, expected)
+
+
+@pytest.mark.parametrize("kind", ["bf16", "f16"])
+def test_f32_gradients_through_an_activation(be, kind):  # noqa: F811
+    """dw's operand act(x) is rounded to the operands' type, as the forward pass rounds it,
+    also where dw is F32: by the formula at the rounded operand dw is off by what the activation's error,
+    2^-21 of |x|, moves across borders of the rounding (2^-21 |x| / ulp of the elements by an ulp:
+    below 1e-4 of the norm), and at the exact one by the rounding."""
+    t, (m, k, n) = TYPES[kind], (4096, 520, 264)
+    g = gen_of(6)
+    x, dy = rand(g, m, k, t=t), rand(g, m, n, t=t)
+    dw = torch.full((k, n), 7.0, device="cuda")
+    be.linear_act_bwd(sp(be, x), None, sp(be, dy), m, k, n, act="gelu", dw=sp(be, dw), need_dx=False, need_db=False)
+    a = act64(x.double(), "gelu")
+    assert rel(dw, a.to(t).double().t() @ dy.double()) <= 1e-4
+    assert rel(dw, a.t() @ dy.double()) <= 1.1 * rel(a.to(t), a)

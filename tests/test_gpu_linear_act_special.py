@@ -14,7 +14,7 @@ pytestmark = pytest.mark.gpu
 
 # One token and a few rows, whole and ragged tiles of many rows, rows whose
 # starts are not 16-byte aligned.
-SHAPES = [(4, 64, 64), (5, 200, 136), (300, 72, 264), (1100, 264, 1288), (1100, 265, 1287)]
+SHAPES = [(4, 64, 64), (5, 200, 136), (300, 72, 264), (1100, 264, 1288), (1100, 265, 1287), (2320, 264, 2312)]
 
 
 def values(t):
