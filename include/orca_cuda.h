@@ -343,7 +343,7 @@ orca_status orca_linear_act_fwd(orca_ctx* ctx, const orca_span* x, const orca_sp
  * not read may be NULL.  a is rounded to the operands' type, as the forward
  * pass rounds it, whatever the type of dw: through an activation an F32 dw is off by
  * that rounding, 1.7e-3 of its norm for BF16 and 2.1e-4 for F16, from the gradient at
- * the unrounded a (5e-7 from that at the rounded one).  residual [m, k] (nullable) is a gradient that reaches x's
+ * the unrounded a (1e-6 from that at the rounded one).  residual [m, k] (nullable) is a gradient that reaches x's
  * layer by another way. */
 orca_status orca_linear_act_bwd(orca_ctx* ctx, const orca_span* x, const orca_span* w,
                                 const orca_span* dy, const orca_span* residual, int64_t m,
